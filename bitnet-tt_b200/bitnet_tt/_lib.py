@@ -99,6 +99,25 @@ class DecodeDesc(ctypes.Structure):
     ]
 
 
+KV_BF16, KV_INT8 = 0, 1
+
+
+class PagedKV(ctypes.Structure):
+    """bitnet_paged_kv_t: the page pools of one layer's keys and values."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("n_kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("kv_type", ctypes.c_int),
+    ]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "bitnet_abi_version": (_c_int, []),
@@ -159,6 +178,16 @@ _SIGNATURES = {
     "bitnet_attention_prefill_varlen": (
         _c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
                  _c_void_p, _c_void_p]),
+    "bitnet_paged_append": (
+        _c_int, [ctypes.POINTER(PagedKV), _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
+                 _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p]),
+    "bitnet_paged_read": (
+        _c_int, [ctypes.POINTER(PagedKV), _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p,
+                 _c_void_p]),
+    "bitnet_paged_attention_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "bitnet_paged_attention": (
+        _c_int, [ctypes.POINTER(PagedKV), _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
+                 _c_int, _c_int, _c_int, _c_float, _c_void_p, _c_size_t, _c_void_p, _c_void_p]),
     "bitnet_selftest_bounded_wait": (_c_int, [ctypes.c_longlong, _c_void_p]),
     "bitnet_lm_head_bytes": (_c_size_t, [_c_int, _c_int]),
     "bitnet_pack_lm_head": (_c_int, [_c_void_p, _c_int, _c_int, _c_void_p, _c_void_p]),
@@ -503,3 +532,38 @@ def attention_prefill_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     check(load().bitnet_attention_prefill_varlen(ptr(q), ptr(k_cache), ptr(v_cache), b, ptr(cu_seqlens),
                                                  int(max_seqlen), n_heads, n_kv, 128, k_cache.shape[2], float(scale),
                                                  ptr(out), stream_handle()), "bitnet_attention_prefill_varlen")
+
+
+def paged_append(kv: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+                 qkv: torch.Tensor, n_heads: int, rope_cos: torch.Tensor, rope_sin: torch.Tensor, q_out: torch.Tensor,
+                 interleaved: bool = False) -> None:
+    b, max_pages = block_table.shape
+    rope_len, half = rope_cos.shape
+    check(load().bitnet_paged_append(kv, ptr(block_table), b, max_pages, ptr(cu_seqlens), ptr(kv_lens), ptr(qkv),
+                                     qkv.stride(0), qkv.shape[0], n_heads, ptr(rope_cos), ptr(rope_sin), rope_len,
+                                     2 * half, rope_cos.dtype == torch.float32, interleaved, ptr(q_out),
+                                     stream_handle()), "bitnet_paged_append")
+
+
+def paged_read(kv: PagedKV, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor,
+               k_out: torch.Tensor, v_out: torch.Tensor) -> None:
+    b, max_pages = block_table.shape
+    check(load().bitnet_paged_read(kv, ptr(block_table), b, max_pages, ptr(starts), ptr(cu_rows), k_out.shape[0],
+                                   ptr(k_out), ptr(v_out), stream_handle()), "bitnet_paged_read")
+
+
+def paged_attention_workspace_bytes(b: int, total_tokens: int, max_seqlen: int, max_kv_len: int, n_heads: int,
+                                    n_kv: int, head_dim: int) -> int:
+    return int(load().bitnet_paged_attention_workspace_bytes(b, total_tokens, max_seqlen, max_kv_len, n_heads, n_kv,
+                                                             head_dim))
+
+
+def paged_attention(kv: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+                    q: torch.Tensor, max_seqlen: int, max_kv_len: int, n_heads: int, scale: float,
+                    workspace: torch.Tensor | None, out: torch.Tensor) -> None:
+    b, max_pages = block_table.shape
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    check(load().bitnet_paged_attention(kv, ptr(block_table), b, max_pages, ptr(cu_seqlens), ptr(kv_lens), ptr(q),
+                                        q.stride(0), q.shape[0], max_seqlen, max_kv_len, n_heads, scale,
+                                        ptr(workspace), ws_bytes, ptr(out), stream_handle()),
+          "bitnet_paged_attention")

@@ -1,0 +1,181 @@
+"""Paged KV cache of one layer: pools of pages shared by sequences of any length.
+
+Where KVCache (layers/attention.py) holds max_seq_len rows for every sequence
+and takes one token per sequence or a prompt from position 0, a PagedKVCache
+holds pages: a block table names each sequence's, a call appends or attends any
+number of new tokens per sequence (a decode token, drafted tokens, a chunk of a
+prompt, none), and the pages are bf16 or int8, quantised as they are written.
+
+The arguments shared by the calls, all on the cache's device:
+  block_table  int32 [B, max_pages]: the pages of sequence b, in order; only the
+               entries that a sequence's length reaches are read
+  cu_seqlens   int32 [B + 1]: row offsets of the sequences' new tokens
+  kv_lens      int32 [B]: each sequence's keys, its new tokens included
+Work is enqueued on the device's current stream.  Shapes and types are checked
+here (ValueError) and in the library (RuntimeError); page ids, offsets and
+lengths live on the device, where a bad one is recorded
+(_lib.last_device_status) and skipped.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+def _want(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+class PagedKVCache:
+    """Pools [num_pages, num_kv_heads, page_size, head_dim] of keys and values;
+    dtype torch.bfloat16, or torch.int8 with fp32 scales [num_pages, num_kv_heads,
+    page_size]: a row's value is code * scale."""
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device=None,
+                 dtype: torch.dtype = torch.bfloat16) -> None:
+        shape = (num_pages, num_kv_heads, page_size, head_dim)
+        dev = torch.device(device if device is not None else "cuda")
+        _want(dtype in (torch.bfloat16, torch.int8), f"paged cache of {dtype}: bfloat16 or int8 expected")
+        k, v = (torch.zeros(shape, dtype=dtype, device=dev) for _ in range(2))
+        ks, vs = ((torch.zeros(shape[:3], dtype=torch.float32, device=dev) for _ in range(2))
+                  if dtype == torch.int8 else (None, None))
+        self._bind(k, v, ks, vs)
+
+    @classmethod
+    def from_tensors(cls, key_pages: torch.Tensor, value_pages: torch.Tensor, key_scale: torch.Tensor | None = None,
+                     value_scale: torch.Tensor | None = None) -> "PagedKVCache":
+        """A cache over existing pools (nothing is copied)."""
+        self = cls.__new__(cls)
+        self._bind(key_pages, value_pages, key_scale, value_scale)
+        return self
+
+    def _bind(self, k: torch.Tensor, v: torch.Tensor, ks: torch.Tensor | None, vs: torch.Tensor | None) -> None:
+        _want(k.dim() == 4 and k.shape == v.shape, "key and value pages must be equal [pages, heads, page_size, head_dim]")
+        _want(k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.int8), "pages must be bfloat16 or int8")
+        _want(k.is_contiguous() and v.is_contiguous(), "pages must be contiguous")
+        _want(k.shape[2] in PAGE_SIZES, f"page_size {k.shape[2]} is not one of {PAGE_SIZES}")
+        _want(k.shape[3] in (64, 128), f"head_dim {k.shape[3]} is not 64 or 128")
+        _want(k.device == v.device, "key and value pages must be on one device")
+        if k.dtype == torch.int8:
+            for s in (ks, vs):
+                _want(s is not None and s.dtype == torch.float32 and s.shape == k.shape[:3] and s.is_contiguous()
+                      and s.device == k.device, "int8 pages need contiguous fp32 scales [pages, heads, page_size]")
+        else:
+            _want(ks is None and vs is None, "bfloat16 pages have no scales")
+        self.key_pages, self.value_pages, self.key_scale, self.value_scale = k, v, ks, vs
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
+        self.device = k.device
+        self.dtype = k.dtype
+        self._kv = _lib.PagedKV(_lib.ptr(k), _lib.ptr(v), _lib.ptr(ks), _lib.ptr(vs), *k.shape[0:1], k.shape[2],
+                                k.shape[1], k.shape[3], _lib.KV_INT8 if k.dtype == torch.int8 else _lib.KV_BF16)
+
+    def nbytes(self) -> int:
+        ts = [t for t in (self.key_pages, self.value_pages, self.key_scale, self.value_scale) if t is not None]
+        return sum(t.numel() * t.element_size() for t in ts)
+
+    # ---- checks ------------------------------------------------------------
+    def _index(self, t: torch.Tensor, name: str, n: int | None = None) -> None:
+        if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor on {self.device}")
+        if n is not None and (t.dim() != 1 or t.shape[0] != n):
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
+
+    def _table(self, block_table: torch.Tensor, cu: torch.Tensor) -> int:
+        self._index(block_table, "block_table")
+        if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+            raise ValueError("block_table must be [sequences, pages]")
+        self._index(cu, "row offsets", block_table.shape[0] + 1)
+        return block_table.shape[0]
+
+    def _rows(self, t: torch.Tensor, name: str) -> None:
+        if t.dtype != torch.bfloat16 or t.device != self.device or t.dim() != 2 or t.stride(1) != 1:
+            raise ValueError(f"{name} must be bfloat16 rows [tokens, features] on {self.device}")
+
+    def _out(self, t: torch.Tensor | None, shape: tuple, name: str) -> torch.Tensor:
+        if t is None:
+            return torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        if t.dtype != torch.bfloat16 or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous bfloat16 {shape} on {self.device}")
+        return t
+
+    # ---- calls -------------------------------------------------------------
+    def append(self, qkv: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
+               rope_cos: torch.Tensor, rope_sin: torch.Tensor, q_out: torch.Tensor | None = None,
+               interleaved: bool = False) -> torch.Tensor:
+        """Rotates the new tokens' queries and keys (qkv rows [tokens, (n_heads +
+        2 n_kv) * head_dim], which may be strided), writes keys and values to their
+        pages and returns the queries [tokens, n_heads * head_dim].  Token i of n
+        stands at position kv_lens[b] - n + i.  rope tables: bf16 or fp32 [positions,
+        rotary_dim / 2]; rotary_dim may be less than head_dim."""
+        b = self._table(block_table, cu_seqlens)
+        self._index(kv_lens, "kv_lens", b)
+        self._rows(qkv, "qkv")
+        d = self.head_dim
+        heads, rest = divmod(qkv.shape[1], d)
+        heads -= 2 * self.num_kv_heads
+        if rest or heads < 1 or heads % self.num_kv_heads:
+            raise ValueError(f"qkv of {qkv.shape[1]} features does not hold q, k and v heads of {d} for "
+                             f"{self.num_kv_heads} KV heads")
+        for t in (rope_cos, rope_sin):
+            if (t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != rope_cos.dtype or t.dim() != 2
+                    or t.shape != rope_cos.shape or t.device != self.device or not t.is_contiguous()):
+                raise ValueError("rope tables must be two equal contiguous bf16 or fp32 [positions, rotary_dim / 2]")
+        q_out = self._out(q_out, (qkv.shape[0], heads * d), "q_out")
+        with torch.cuda.device(self.device):
+            _lib.paged_append(self._kv, block_table, cu_seqlens, kv_lens, qkv, heads, rope_cos, rope_sin, q_out,
+                              interleaved)
+        return q_out
+
+    def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
+               max_seqlen: int, max_kv_len: int, scale: float | None = None, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """Causal grouped-head attention of the new tokens' rotated queries [tokens,
+        n_heads * head_dim] over their sequences' pages.  max_seqlen and max_kv_len
+        bound the new tokens and the keys of every sequence.  scale: 1 /
+        sqrt(head_dim) by default.  workspace (attention_workspace): taken from the
+        allocator if not given."""
+        b = self._table(block_table, cu_seqlens)
+        self._index(kv_lens, "kv_lens", b)
+        self._rows(q, "q")
+        d = self.head_dim
+        heads, rest = divmod(q.shape[1], d)
+        if rest or heads < 1 or heads % self.num_kv_heads:
+            raise ValueError(f"q of {q.shape[1]} features does not hold heads of {d} for {self.num_kv_heads} KV heads")
+        out = self._out(out, (q.shape[0], heads * d), "out")
+        with torch.cuda.device(self.device):
+            if workspace is None:
+                workspace = self.attention_workspace(b, q.shape[0], max_seqlen, max_kv_len, heads)
+            elif workspace.device != self.device or not workspace.is_contiguous():
+                raise ValueError(f"workspace must be a contiguous tensor on {self.device}")
+            _lib.paged_attention(self._kv, block_table, cu_seqlens, kv_lens, q, max_seqlen, max_kv_len, heads,
+                                 d ** -0.5 if scale is None else scale, workspace, out)
+        return out
+
+    def attention_workspace(self, batch: int, total_tokens: int, max_seqlen: int, max_kv_len: int,
+                            num_heads: int) -> torch.Tensor | None:
+        """Workspace of attend() for these bounds (None when it needs none).  Calls
+        that may overlap need one each."""
+        n = _lib.paged_attention_workspace_bytes(batch, total_tokens, max_seqlen, max_kv_len, num_heads,
+                                                 self.num_kv_heads, self.head_dim)
+        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+
+    def read(self, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor, total_rows: int,
+             k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Rows starts[b] .. starts[b] + cu_rows[b + 1] - cu_rows[b] - 1 of every
+        sequence (starts None: from row 0) as packed bf16 keys and values
+        [total_rows, n_kv, head_dim]."""
+        b = self._table(block_table, cu_rows)
+        if starts is not None:
+            self._index(starts, "starts", b)
+        if total_rows < 0:
+            raise ValueError("total_rows is negative")
+        shape = (total_rows, self.num_kv_heads, self.head_dim)
+        k_out, v_out = self._out(k_out, shape, "k_out"), self._out(v_out, shape, "v_out")
+        with torch.cuda.device(self.device):
+            _lib.paged_read(self._kv, block_table, starts, cu_rows, k_out, v_out)
+        return k_out, v_out

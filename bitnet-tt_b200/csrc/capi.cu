@@ -15,6 +15,7 @@
 #include <vector>
 #include <algorithm>
 #include <cmath>
+#include <climits>
 
 #include "act_quant.cuh"
 #include "attention.cuh"
@@ -26,6 +27,8 @@
 #include "lm_head.cuh"
 #include "lm_head_tc.cuh"
 #include "pack.cuh"
+#include "paged_attention.cuh"
+#include "paged_kv.cuh"
 #include "../../include/bitnet_b200.h"
 
 using namespace bitnet;
@@ -175,7 +178,7 @@ int to_dev_segments(const bitnet_segments_t* s, int N, int epilogue, bitnet_segm
 }
 
 std::atomic<unsigned long long> g_smem_aq{0}, g_smem_aq_stage{0}, g_smem_simt[3][4], g_smem_tc[3], g_smem_lmh{0}, g_smem_att[4],
-    g_smem_apf{0};
+    g_smem_apf{0}, g_smem_pra[4];
 
 int lm_head_tile_T(int B) { return round_up(B, 16); }
 size_t lm_head_part_bytes(int B, int grid) { return (size_t)grid * B * sizeof(ArgPair); }
@@ -1128,3 +1131,220 @@ extern "C" int bitnet_decode_plan_destroy(bitnet_decode_plan_t* pl) {
   delete pl;
   return BITNET_OK;
 }
+
+// ===========================================================================
+// Paged KV cache: append, read, attention.
+// ===========================================================================
+namespace {
+
+int paged_kv_args(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages, PagedKV* out) {
+  if (!kv || !kv->k_pages || !kv->v_pages || !block_table || B <= 0 || max_pages <= 0 || kv->num_pages <= 0 ||
+      kv->n_kv_heads <= 0 || kv->n_kv_heads > 65535)
+    return BITNET_ERR_INVALID_ARGUMENT;
+  if (kv->head_dim != 64 && kv->head_dim != 128) return BITNET_ERR_INVALID_ARGUMENT;
+  if (kv->page_size < 16 || kv->page_size > 256 || (kv->page_size & (kv->page_size - 1)))
+    return BITNET_ERR_INVALID_ARGUMENT;
+  if (kv->kv_type != BITNET_KV_BF16 && kv->kv_type != BITNET_KV_INT8) return BITNET_ERR_INVALID_ARGUMENT;
+  if (kv->kv_type == BITNET_KV_INT8 && (!kv->k_scale || !kv->v_scale)) return BITNET_ERR_INVALID_ARGUMENT;
+  if ((long long)kv->num_pages > (long long)INT_MAX / kv->page_size / kv->n_kv_heads) return BITNET_ERR_INVALID_ARGUMENT;
+  if ((long long)max_pages > (long long)INT_MAX / kv->page_size) return BITNET_ERR_INVALID_ARGUMENT;
+  if (!aligned(kv->k_pages, 16) || !aligned(kv->v_pages, 16) || !aligned(block_table, 4) ||
+      !aligned(kv->k_scale, 4) || !aligned(kv->v_scale, 4))
+    return BITNET_ERR_ALIGNMENT;
+  out->k = (uint8_t*)kv->k_pages;
+  out->v = (uint8_t*)kv->v_pages;
+  out->ks = kv->k_scale;
+  out->vs = kv->v_scale;
+  out->num_pages = kv->num_pages;
+  out->page_shift = __builtin_ctz((unsigned)kv->page_size);
+  out->n_kv = kv->n_kv_heads;
+  out->table = block_table;
+  out->max_pages = max_pages;
+  return BITNET_OK;
+}
+
+template <int D, bool I8>
+int launch_paged_append(const PagedAppendParams& p, bool f32, dim3 grid, bitnet_stream_t st) {
+  return f32 ? launch(paged_append_kernel<D, I8, true>, grid, dim3(PKV_THREADS), 0, st, 1, p)
+             : launch(paged_append_kernel<D, I8, false>, grid, dim3(PKV_THREADS), 0, st, 1, p);
+}
+
+// How an attention call is cut: row blocks (grid.x) and parts of the keys.
+struct PagedPlan {
+  int blocks, nsplit, span;
+  size_t ml_bytes, bytes;  // workspace: maxima and sums, then outputs
+};
+
+// Parts of the keys for `pairs` blocks of work on `slots` CTAs at once: the s
+// with the least waves x (keys of a part + unit), `unit` the fixed cost of a
+// part in keys.  Only the s that just fill 1 .. 4 waves can be best.
+int paged_splits(long long pairs, int max_kv, int slots, int unit, int min_span) {
+  const long long smax = std::max(1, (max_kv + min_span - 1) / min_span);
+  long long best_s = 1, best = LLONG_MAX;
+  for (int w = 1; w <= 4; ++w) {
+    const long long s = std::min(smax, std::max(1LL, (long long)slots * w / pairs));
+    const long long cost = ((pairs * s + slots - 1) / slots) * ((max_kv + s - 1) / s + unit);
+    if (cost < best) best = cost, best_s = s;
+  }
+  return (int)best_s;
+}
+
+PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, int D, int sms) {
+  PagedPlan pl;
+  const long long blocks =
+      (long long)max_q * G <= PRA_R ? B : ((long long)tokens * G + PRA_R - 1) / PRA_R + B;
+  pl.blocks = (int)std::min(blocks, (long long)INT_MAX);
+  pl.nsplit = paged_splits((long long)pl.blocks * n_kv, max_kv, sms * 3, ATT_UNIT_COST, ATT_MIN_SPLIT);
+  pl.span = round_up((max_kv + pl.nsplit - 1) / pl.nsplit, PRA_TILE);
+  const size_t rows = pl.nsplit > 1 ? (size_t)pl.nsplit * pl.blocks * n_kv * PRA_R : 0;
+  pl.ml_bytes = rows * sizeof(float2);
+  pl.bytes = pl.ml_bytes + rows * D * sizeof(float);
+  return pl;
+}
+
+bool paged_attn_sizes(int B, int tokens, int max_q, int max_kv, int n_heads, int n_kv, int D) {
+  return B > 0 && tokens >= 0 && max_q >= 0 && max_kv >= 0 && n_heads > 0 && n_kv > 0 && n_heads % n_kv == 0 &&
+         n_heads / n_kv <= 64 && (D == 64 || D == 128) && (long long)tokens * n_heads <= INT_MAX / 2 &&
+         (long long)max_q * n_heads <= INT_MAX / 2 && max_kv <= INT_MAX - 4096;
+}
+
+template <int D, bool I8>
+int launch_paged_attention(const PagedAttnParams& p, bitnet_stream_t st) {
+  if (int e = ensure_smem(paged_rows_kernel<D, I8>, &g_smem_pra[(D == 128) * 2 + I8])) return e;
+  if (int e = launch(paged_rows_kernel<D, I8>, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(PRA_THREADS),
+                     PraShape<D, I8>::SMEM, st, 1, p))
+    return e;
+  if (p.nsplit == 1) return BITNET_OK;
+  const int rows = std::min(PRA_R, p.max_q * p.G);
+  return launch(paged_join_kernel<D, PRA_R>, dim3(p.blocks, p.kv.n_kv, (rows + 3) / 4), dim3(128), 0, st, 1, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int bitnet_paged_append(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
+                        const int32_t* cu_seqlens, const int32_t* kv_lens, const void* qkv, int ld_qkv,
+                        int total_tokens, int n_heads, const void* rope_cos, const void* rope_sin, int rope_len,
+                        int rotary_dim, int rope_f32, int interleaved, void* q_out, bitnet_stream_t stream) {
+  PagedAppendParams p;
+  memset(&p, 0, sizeof(p));
+  if (int e = paged_kv_args(kv, block_table, B, max_pages, &p.kv)) return e;
+  if (!cu_seqlens || !kv_lens || !rope_cos || !rope_sin || (total_tokens != 0 && (!qkv || !q_out)))
+    return BITNET_ERR_INVALID_ARGUMENT;
+  const int D = kv->head_dim;
+  if (total_tokens < 0 || n_heads <= 0 || n_heads % kv->n_kv_heads != 0 || rope_len <= 0 || rotary_dim < 16 ||
+      rotary_dim > D || rotary_dim % 16 != 0)
+    return BITNET_ERR_INVALID_ARGUMENT;
+  const long long width = ((long long)n_heads + 2LL * kv->n_kv_heads) * D;
+  if (width > ld_qkv || ld_qkv % 8 != 0) return BITNET_ERR_INVALID_ARGUMENT;
+  if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(rope_cos, 16) || !aligned(rope_sin, 16) ||
+      !aligned(cu_seqlens, 4) || !aligned(kv_lens, 4))
+    return BITNET_ERR_ALIGNMENT;
+  DevInfo* d;
+  if (int e = device_info(&d)) return e;
+  if (total_tokens == 0) return BITNET_OK;
+  p.cu = cu_seqlens;
+  p.kv_lens = kv_lens;
+  p.B = B;
+  p.tokens = total_tokens;
+  p.qkv = (const uint16_t*)qkv;
+  p.ld_qkv = ld_qkv;
+  p.n_heads = n_heads;
+  p.cos = rope_cos;
+  p.sin = rope_sin;
+  p.rope_len = rope_len;
+  p.rot = rotary_dim;
+  p.interleaved = interleaved != 0;
+  p.q_out = (uint16_t*)q_out;
+  // a token a CTA until the GPU is full, so that a decode batch is one round of loads deep
+  p.tok_per_cta = std::min(8, std::max(1, total_tokens / (d->sms * 4)));
+  const dim3 grid((total_tokens + p.tok_per_cta - 1) / p.tok_per_cta);
+  const bool f32 = rope_f32 != 0;
+  if (kv->kv_type == BITNET_KV_INT8)
+    return D == 128 ? launch_paged_append<128, true>(p, f32, grid, stream)
+                    : launch_paged_append<64, true>(p, f32, grid, stream);
+  return D == 128 ? launch_paged_append<128, false>(p, f32, grid, stream)
+                  : launch_paged_append<64, false>(p, f32, grid, stream);
+}
+
+int bitnet_paged_read(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
+                      const int32_t* starts, const int32_t* cu_rows, int total_rows, void* k_out, void* v_out,
+                      bitnet_stream_t stream) {
+  PagedReadParams p;
+  memset(&p, 0, sizeof(p));
+  if (int e = paged_kv_args(kv, block_table, B, max_pages, &p.kv)) return e;
+  if (!cu_rows || total_rows < 0 || (total_rows != 0 && (!k_out || !v_out))) return BITNET_ERR_INVALID_ARGUMENT;
+  if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(cu_rows, 4) || !aligned(starts, 4))
+    return BITNET_ERR_ALIGNMENT;
+  DevInfo* d;
+  if (int e = device_info(&d)) return e;
+  if (total_rows == 0) return BITNET_OK;
+  p.cu = cu_rows;
+  p.starts = starts;
+  p.B = B;
+  p.rows = total_rows;
+  p.k_out = (uint16_t*)k_out;
+  p.v_out = (uint16_t*)v_out;
+  const dim3 grid((total_rows - 1) / PKV_READ_ROWS + 1), block(PKV_THREADS);
+  if (kv->kv_type == BITNET_KV_INT8)
+    return kv->head_dim == 128 ? launch(paged_read_kernel<128, true>, grid, block, 0, stream, 1, p)
+                               : launch(paged_read_kernel<64, true>, grid, block, 0, stream, 1, p);
+  return kv->head_dim == 128 ? launch(paged_read_kernel<128, false>, grid, block, 0, stream, 1, p)
+                             : launch(paged_read_kernel<64, false>, grid, block, 0, stream, 1, p);
+}
+
+size_t bitnet_paged_attention_workspace_bytes(int B, int total_tokens, int max_seqlen, int max_kv_len, int n_heads,
+                                              int n_kv_heads, int head_dim) {
+  DevInfo* d;
+  const int sms = device_info(&d) == BITNET_OK ? d->sms : 148;
+  if (!paged_attn_sizes(B, total_tokens, max_seqlen, max_kv_len, n_heads, n_kv_heads, head_dim)) return 0;
+  return paged_plan(B, total_tokens, max_seqlen, max_kv_len, n_heads / n_kv_heads, n_kv_heads, head_dim, sms).bytes;
+}
+
+int bitnet_paged_attention(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
+                           const int32_t* cu_seqlens, const int32_t* kv_lens, const void* q, int ld_q,
+                           int total_tokens, int max_seqlen, int max_kv_len, int n_heads, float scale,
+                           void* workspace, size_t workspace_bytes, void* out, bitnet_stream_t stream) {
+  PagedAttnParams p;
+  memset(&p, 0, sizeof(p));
+  if (int e = paged_kv_args(kv, block_table, B, max_pages, &p.kv)) return e;
+  if (!cu_seqlens || !kv_lens || (total_tokens != 0 && (!q || !out))) return BITNET_ERR_INVALID_ARGUMENT;
+  const int D = kv->head_dim;
+  if (!paged_attn_sizes(B, total_tokens, max_seqlen, max_kv_len, n_heads, kv->n_kv_heads, D))
+    return BITNET_ERR_INVALID_ARGUMENT;
+  if ((long long)max_kv_len > (long long)max_pages * kv->page_size) return BITNET_ERR_INVALID_ARGUMENT;
+  if ((long long)n_heads * D > ld_q || ld_q % 8 != 0) return BITNET_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(cu_seqlens, 4) || !aligned(kv_lens, 4)) return BITNET_ERR_ALIGNMENT;
+  DevInfo* d;
+  if (int e = device_info(&d)) return e;
+  if (total_tokens == 0 || max_seqlen == 0) return BITNET_OK;
+  const int G = n_heads / kv->n_kv_heads;
+  const PagedPlan pl = paged_plan(B, total_tokens, max_seqlen, max_kv_len, G, kv->n_kv_heads, D, d->sms);
+  if (pl.bytes > 0) {
+    if (!workspace || workspace_bytes < pl.bytes) return BITNET_ERR_INVALID_ARGUMENT;
+    if (!aligned(workspace, 16)) return BITNET_ERR_ALIGNMENT;
+  }
+  p.cu = cu_seqlens;
+  p.kv_lens = kv_lens;
+  p.B = B;
+  p.tokens = total_tokens;
+  p.max_q = max_seqlen;
+  p.max_kv = max_kv_len;
+  p.q = (const uint16_t*)q;
+  p.ld_q = ld_q;
+  p.n_heads = n_heads;
+  p.G = G;
+  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  p.nsplit = pl.nsplit;
+  p.span = pl.span;
+  p.blocks = pl.blocks;
+  p.part_ml = (float2*)workspace;
+  p.part_o = (float*)((uint8_t*)workspace + pl.ml_bytes);
+  p.out = (uint16_t*)out;
+  if (kv->kv_type == BITNET_KV_INT8)
+    return D == 128 ? launch_paged_attention<128, true>(p, stream) : launch_paged_attention<64, true>(p, stream);
+  return D == 128 ? launch_paged_attention<128, false>(p, stream) : launch_paged_attention<64, false>(p, stream);
+}
+
+}  // extern "C"

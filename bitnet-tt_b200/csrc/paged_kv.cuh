@@ -1,0 +1,292 @@
+// Paged KV cache: what its kernels share, and the kernels that write and read it.
+//
+// A pool of pages [num_pages][n_kv_heads][page_size][head_dim] holds keys (and
+// another values) as bf16, or as int8 with one fp32 scale per (page, KV head,
+// row); the value of a code is code * scale.  Row `pos` of sequence b is row
+// pos % page_size of page block_table[b][pos / page_size].
+//
+// Page ids, offsets and lengths are device data, so the kernels check them: a
+// bad one is recorded in the device status word (DEV_ERR_BOUNDS) and the access
+// is skipped.
+#pragma once
+#include "common.cuh"
+
+namespace bitnet {
+
+struct PagedKV {
+  uint8_t* k;          // pages of keys (bf16 or int8)
+  uint8_t* v;
+  float* ks;           // int8: scales [num_pages][n_kv][page_size]
+  float* vs;
+  int num_pages, page_shift, n_kv;
+  const int32_t* table;  // [B][max_pages]
+  int max_pages;
+};
+
+// Row index (in units of head_dim elements) of row `slot` of KV head g in `page`.
+__device__ __forceinline__ size_t paged_row(const PagedKV& c, int page, int g, int slot) {
+  return ((((size_t)page * c.n_kv + g) << c.page_shift) + slot);
+}
+
+// The last b in 0 .. B-1 with cu[b] <= row, found by a whole warp: each round
+// narrows the range 32 times (two rounds up to 1024 sequences).  An empty
+// sequence is never the answer for a row that some sequence holds.
+__device__ __forceinline__ int warp_find_seq(const int32_t* cu, int B, int row, int lane) {
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int idx = lo + (lane + 1) * step;
+    const unsigned le = __ballot_sync(0xffffffffu, idx < hi && cu[idx] <= row);
+    lo += __popc(le) * step;
+    hi = min(hi, lo + step);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint32_t bf2_of(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void unpack_bf8(const uint4& w, float (&x)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(u[i] << 16);
+    x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint4 pack_bf8(const float (&x)[8]) {
+  return make_uint4(bf2_of(x[0], x[1]), bf2_of(x[2], x[3]), bf2_of(x[4], x[5]), bf2_of(x[6], x[7]));
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+// For pair j < rot/2 of a query or key head, (a, b) = dims (j, j + rot/2), or
+// (2j, 2j + 1) when interleaved:
+//     a' = a cos[pos][j] - b sin[pos][j],   b' = b cos[pos][j] + a sin[pos][j]
+// in fp32, each product and sum rounded on its own (so an int8 code is a
+// function of the inputs alone, not of how the compiler fuses), and the dims
+// from rot on copied.  A value is rounded once, to bf16 or to its int8 code: the
+// contiguous cache's kernels round after every product and sum as the bf16
+// model code does, which costs up to three roundings a value and, with an int8
+// cache, a fourth.
+//     int8: top = max(max_d |row|, 1e-5), scale = top / 127, code = rint(row * (127 / top)),
+// the floor of the framework's activation quantiser.  A row with an infinity or
+// a NaN gets the scale NaN (its values read back as NaN).
+//
+// Bound: memory.  D/8 lanes take one head of one token, 16 bytes each; the
+// partner half comes by shuffle, the row's maximum by a shuffle tree, so qkv is
+// read once and every access is 16 bytes wide (8 for int8 codes).
+struct PagedAppendParams {
+  PagedKV kv;
+  const int32_t* cu;       // [B + 1] token offsets
+  const int32_t* kv_lens;  // [B] keys including the new tokens
+  int B, tokens;
+  const uint16_t* qkv;
+  int ld_qkv, n_heads;
+  const void* cos;         // [rope_len][rot / 2], bf16 or fp32
+  const void* sin;
+  int rope_len, rot, interleaved;
+  uint16_t* q_out;         // [tokens][n_heads * D]
+  int tok_per_cta;         // 1 .. 8
+};
+
+constexpr int PKV_THREADS = 256;
+
+template <bool F32>
+__device__ __forceinline__ float rope_entry(const void* t, size_t i) {
+  return F32 ? reinterpret_cast<const float*>(t)[i] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(t)[i]);
+}
+template <bool F32>
+__device__ __forceinline__ void rope_entries8(const void* t, size_t i, float (&x)[8]) {  // i % 8 == 0
+  if (F32) {
+    const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(t) + i);
+    const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(t) + i + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+    unpack_bf8(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(t) + i), x);
+  }
+}
+
+template <int D, bool I8, bool F32>
+__global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAppendParams p) {
+  constexpr int LPH = D / 8;  // lanes of one head
+  __shared__ int s_pos[8], s_page[8];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tok0 = blockIdx.x * p.tok_per_cta;
+  const int ntok = min(p.tok_per_cta, p.tokens - tok0);
+  if (warp < ntok) {
+    const int tok = tok0 + warp;
+    const int b = warp_find_seq(p.cu, p.B, tok, lane);
+    if (lane == 0) {
+      int pos = -1, page = -1;
+      const int lo = p.cu[b], hi = p.cu[b + 1];
+      if (tok >= lo && tok < hi) {  // else a row that belongs to no sequence: left alone
+        pos = p.kv_lens[b] - (hi - lo) + (tok - lo);
+        const int pi = pos >> p.kv.page_shift;
+        if (pos < 0 || pos >= p.rope_len || pi >= p.kv.max_pages) {
+          record_error(DEV_ERR_BOUNDS, 340);
+          pos = -1;
+        } else {
+          page = p.kv.table[(size_t)b * p.kv.max_pages + pi];
+          if (page < 0 || page >= p.kv.num_pages) {
+            record_error(DEV_ERR_BOUNDS, 341);
+            pos = -1;
+          }
+        }
+      }
+      s_pos[warp] = pos;
+      s_page[warp] = page;
+    }
+  }
+  __syncthreads();
+  const int heads = p.n_heads + 2 * p.kv.n_kv, items = ntok * heads;
+  const int l = tid % LPH, d0 = l * 8;          // this lane's 8 dims
+  const int half_l = p.rot >> 4;                // lanes of half the rotated part
+  const bool in_rot = d0 < p.rot;
+  // lane (in the warp) holding the other half of the pairs
+  const int base = lane - l;
+  const int partner = base + (in_rot ? (l < half_l ? l + half_l : l - half_l) : l);
+  for (int it0 = 0; it0 < items; it0 += PKV_THREADS / LPH) {
+    const int it = it0 + tid / LPH;
+    const bool valid = it < items;
+    const int t = valid ? it / heads : 0, hh = valid ? it - t * heads : 0;
+    const int pos = s_pos[t];
+    const bool live = valid && pos >= 0;
+    float x[8];
+    {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (live) w = *reinterpret_cast<const uint4*>(p.qkv + (size_t)(tok0 + t) * p.ld_qkv + hh * D + d0);
+      unpack_bf8(w, x);
+      uint4 o;
+      o.x = __shfl_sync(0xffffffffu, w.x, partner);
+      o.y = __shfl_sync(0xffffffffu, w.y, partner);
+      o.z = __shfl_sync(0xffffffffu, w.z, partner);
+      o.w = __shfl_sync(0xffffffffu, w.w, partner);
+      if (live && in_rot && hh < p.n_heads + p.kv.n_kv) {
+        const size_t row = (size_t)pos * (p.rot >> 1);
+        if (p.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float c = rope_entry<F32>(p.cos, row + (d0 >> 1) + e), s = rope_entry<F32>(p.sin, row + (d0 >> 1) + e);
+            const float a = x[2 * e], b = x[2 * e + 1];
+            x[2 * e] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
+            x[2 * e + 1] = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+          }
+        } else {
+          float c[8], s[8], y[8];
+          const size_t j = row + (l < half_l ? d0 : d0 - (p.rot >> 1));
+          rope_entries8<F32>(p.cos, j, c);
+          rope_entries8<F32>(p.sin, j, s);
+          unpack_bf8(o, y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = l < half_l ? __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]))
+                              : __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]));
+        }
+      }
+    }
+    const int g = hh < p.n_heads ? 0 : (hh - p.n_heads) % p.kv.n_kv;
+    const bool is_v = hh >= p.n_heads + p.kv.n_kv;
+    const size_t row = live ? paged_row(p.kv, s_page[t], g, pos & ((1 << p.kv.page_shift) - 1)) : 0;
+    if (live && hh < p.n_heads)
+      *reinterpret_cast<uint4*>(p.q_out + ((size_t)(tok0 + t) * p.n_heads + hh) * D + d0) = pack_bf8(x);
+    if (I8) {
+      uint32_t top = 0;  // the largest |x| by its bits: a NaN or an infinity wins
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (live && hh >= p.n_heads) {
+        const bool finite = top < 0x7f800000u;
+        const float amax = fmaxf(__uint_as_float(top), 1e-5f), inv = __fdiv_rn(127.f, amax);
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int q = finite ? __float2int_rn(__fmul_rn(x[e], inv)) : 0;
+          w[e >> 2] |= (uint32_t)(q & 0xff) << (8 * (e & 3));
+        }
+        *reinterpret_cast<uint2*>((is_v ? p.kv.v : p.kv.k) + row * D + d0) = make_uint2(w[0], w[1]);
+        if (l == 0) (is_v ? p.kv.vs : p.kv.ks)[row] = finite ? __fdiv_rn(amax, 127.f) : __uint_as_float(0x7fc00000u);
+      }
+    } else if (live && hh >= p.n_heads) {
+      *reinterpret_cast<uint4*>((is_v ? p.kv.v : p.kv.k) + (row * D + d0) * 2) = pack_bf8(x);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read
+// ---------------------------------------------------------------------------
+// Row r of sequence b's packed rows (cu[b] .. cu[b + 1] - 1) is cache row
+// starts[b] + r - cu[b]; k_out / v_out are bf16 [rows][n_kv][D].  int8: the value
+// bf16(code * scale), rounded once.  Bound: memory, one pass; D/8 lanes a row.
+struct PagedReadParams {
+  PagedKV kv;
+  const int32_t* cu;
+  const int32_t* starts;  // nullable: 0
+  int B, rows;
+  uint16_t* k_out;
+  uint16_t* v_out;
+};
+constexpr int PKV_READ_ROWS = 8;
+
+template <int D, bool I8>
+__global__ void __launch_bounds__(PKV_THREADS) paged_read_kernel(const PagedReadParams p) {
+  constexpr int LPH = D / 8;
+  __shared__ int s_slot[PKV_READ_ROWS], s_page[PKV_READ_ROWS];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row0 = blockIdx.x * PKV_READ_ROWS, nrow = min(PKV_READ_ROWS, p.rows - row0);
+  if (warp < nrow) {
+    const int r = row0 + warp;
+    const int b = warp_find_seq(p.cu, p.B, r, lane);
+    if (lane == 0) {
+      int page = -1, slot = 0;
+      if (r >= p.cu[b] && r < p.cu[b + 1]) {
+        const long long pos = (long long)(p.starts ? p.starts[b] : 0) + (r - p.cu[b]);
+        const long long pi = pos >> p.kv.page_shift;
+        if (pos < 0 || pi >= p.kv.max_pages) {
+          record_error(DEV_ERR_BOUNDS, 342);
+        } else {
+          slot = (int)pos & ((1 << p.kv.page_shift) - 1);
+          page = p.kv.table[(size_t)b * p.kv.max_pages + pi];
+          if (page < 0 || page >= p.kv.num_pages) {
+            record_error(DEV_ERR_BOUNDS, 343);
+            page = -1;
+          }
+        }
+      }
+      s_page[warp] = page;
+      s_slot[warp] = slot;
+    }
+  }
+  __syncthreads();
+  const int per_row = 2 * p.kv.n_kv, items = nrow * per_row;
+  const int d0 = (tid % LPH) * 8;
+  for (int it = tid / LPH; it < items; it += PKV_THREADS / LPH) {
+    const int t = it / per_row, h = it - t * per_row;
+    if (s_page[t] < 0) continue;
+    const bool is_v = h >= p.kv.n_kv;
+    const int g = is_v ? h - p.kv.n_kv : h;
+    const size_t row = paged_row(p.kv, s_page[t], g, s_slot[t]);
+    const uint8_t* src = is_v ? p.kv.v : p.kv.k;
+    uint16_t* dst = (is_v ? p.v_out : p.k_out) + ((size_t)(row0 + t) * p.kv.n_kv + g) * D + d0;
+    if (I8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(src + row * D + d0);
+      const float s = (is_v ? p.kv.vs : p.kv.ks)[row];
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3))), s);
+      *reinterpret_cast<uint4*>(dst) = pack_bf8(x);
+    } else {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + (row * D + d0) * 2);
+    }
+  }
+}
+
+}  // namespace bitnet

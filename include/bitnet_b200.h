@@ -281,6 +281,80 @@ int bitnet_attention_prefill_varlen(const void* q, const void* k_cache, const vo
                                     const int32_t* cu_seqlens, int max_seqlen, int n_heads, int n_kv_heads,
                                     int head_dim, int max_len, float scale, void* out, bitnet_stream_t stream);
 
+/* ---- paged KV cache ------------------------------------------------------
+ * No counterpart in the reference's decode path (its caches are one
+ * [batch, n_kv, max_len, head_dim] tensor per layer, src/bitnet_tt/layers/
+ * attention.py:116-458): a pool of pages shared by sequences of any length, in
+ * bf16 or quantised to int8 as it is written, extended by one or many tokens per
+ * sequence and call.
+ *
+ * Keys and values are pools [num_pages][n_kv_heads][page_size][head_dim].  Row
+ * `pos` of sequence b is row pos % page_size of page
+ * block_table[b * max_pages + pos / page_size].  BITNET_KV_INT8: a code's value
+ * is code * scale, one fp32 scale per row of a KV head, [num_pages][n_kv_heads][page_size].
+ * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; page pools 16-byte
+ * aligned; num_pages * n_kv_heads * page_size < 2^31.
+ *
+ * Common arguments: block_table int32 [B][max_pages] (only entries that a
+ * sequence's length reaches are read); cu_seqlens int32 [B + 1], the packed row
+ * offsets of the sequences' new tokens (cu_seqlens[b + 1] == cu_seqlens[b]: no
+ * new token); kv_lens int32 [B], each sequence's keys INCLUDING its new tokens,
+ * so new token i of n stands at position kv_lens[b] - n + i.  All of these are
+ * device memory.  Rows from cu_seqlens[B] on (total_tokens may be larger) are
+ * left as they were.  A page id outside the pool, a position outside the table
+ * or the rotary tables, or lengths beyond the bounds passed in are device bounds
+ * errors (bitnet_last_device_status): the row or sequence is skipped, and an
+ * attention that met a bad page reads zeros there.  Sequences may share pages
+ * for reading; a row that two tokens of one call write is undefined. */
+#define BITNET_KV_BF16 0
+#define BITNET_KV_INT8 1
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  float* k_scale; /* NULL for BITNET_KV_BF16 */
+  float* v_scale;
+  int num_pages, page_size, n_kv_heads, head_dim, kv_type;
+} bitnet_paged_kv_t;
+
+/* Rotates the queries and keys of total_tokens packed qkv rows (bf16, row
+ * stride ld_qkv elements, [n_heads q | n_kv k | n_kv v] of head_dim), writes the
+ * queries to q_out (bf16 [total_tokens][n_heads * head_dim]) and the rotated keys
+ * and the values to their pages.  rope_cos / rope_sin: [rope_len][rotary_dim / 2],
+ * fp32 if rope_f32, else bf16.  rotary_dim (a multiple of 16, at most head_dim):
+ * the head's first dims, which are rotated; the rest is copied.  Pairs are dims
+ * (j, j + rotary_dim / 2), or (2j, 2j + 1) if interleaved.  The rotation is in
+ * fp32 and rounded once; bitnet_rope_append_prefill rounds after each product
+ * and sum, so their last bits differ.  int8: top = max(max |row|, 1e-5),
+ * scale = top / 127, code = rint(row * (127 / top)); a row that holds an infinity
+ * or a NaN gets the scale NaN.  qkv, q_out, rope_cos and rope_sin 16-byte
+ * aligned, ld_qkv a multiple of 8. */
+int bitnet_paged_append(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
+                        const int32_t* cu_seqlens, const int32_t* kv_lens, const void* qkv, int ld_qkv,
+                        int total_tokens, int n_heads, const void* rope_cos, const void* rope_sin, int rope_len,
+                        int rotary_dim, int rope_f32, int interleaved, void* q_out, bitnet_stream_t stream);
+/* Reads rows back: sequence b's packed rows cu_rows[b] .. cu_rows[b + 1] - 1 of
+ * k_out / v_out (bf16 [total_rows][n_kv_heads][head_dim], 16-byte aligned) are its
+ * cache rows from starts[b] (int32 [B], NULL: 0) on; int8 as bf16(code * scale). */
+int bitnet_paged_read(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
+                      const int32_t* starts, const int32_t* cu_rows, int total_rows, void* k_out, void* v_out,
+                      bitnet_stream_t stream);
+/* Causal GQA attention of the new tokens (one or many a sequence) over their
+ * sequences' pages: token i of n sees the first kv_lens[b] - n + i + 1 keys, and
+ * one that sees none (kv_lens[b] < n) gets zeros.  q: bf16, row stride ld_q
+ * elements (a multiple of 8), rotated; out: bf16 [total_tokens][n_heads * head_dim];
+ * both 16-byte aligned.  n_heads / n_kv_heads is at most 64.  max_seqlen and max_kv_len bound the new
+ * tokens and the keys of every sequence; they size the grid and the split of long
+ * contexts, so tight bounds keep both small.  Cache rows below kv_lens[b] have to
+ * be finite; whatever stands behind them does not matter.  workspace:
+ * bitnet_paged_attention_workspace_bytes (0: may be NULL), 16-byte aligned,
+ * contents irrelevant before and after; calls that may overlap need their own. */
+size_t bitnet_paged_attention_workspace_bytes(int B, int total_tokens, int max_seqlen, int max_kv_len, int n_heads,
+                                              int n_kv_heads, int head_dim);
+int bitnet_paged_attention(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
+                           const int32_t* cu_seqlens, const int32_t* kv_lens, const void* q, int ld_q,
+                           int total_tokens, int max_seqlen, int max_kv_len, int n_heads, float scale,
+                           void* workspace, size_t workspace_bytes, void* out, bitnet_stream_t stream);
+
 /* ---- lm_head / embedding table -------------------------------------------
  * The tied embedding / lm_head matrix (src/bitnet_tt/utils/weights.py:236-246)
  * is stored once, in a tiled layout read by both the lm_head and the gather. */

@@ -1,0 +1,488 @@
+"""The paged KV cache's kernels against plain implementations in 64 bits, on the
+CPU: append (rotation, quantisation, placement), read, and attention of the new
+tokens, at the lengths, masks and layouts where they can go wrong.
+
+Tolerances, derived from the arithmetic:
+* a bf16 result is off by half a step, 2^-8 of its value;
+* the rotation's two products and one sum in fp32 add at most 2^-22 (|a| + |b|)
+  (cos, sin at most 1);
+* attention: A = sum_j p_j |v_j| / sum_j p_j bounds what an error of the weights
+  does.  The score is a sum of at most 128 fp32 products, off by at most
+  128 2^-24 sum |q k| scale, below 2^-12 here (checked: sum |q k| scale < 32);
+  exp2 of it, its sum and the rescaling add less than 2^-14.  With P as a bf16
+  pair the weights carry 2^-16, as one bf16 2^-8, so the bound is
+  2^-8 |o| + (2^-11 + weight) A, the weight's step by the path that the rows take."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, I8 = torch.bfloat16, torch.int8
+
+
+def _cache(cuda, npages, page, hk, d, dtype, seed=0, fill=True):
+    from bitnet_tt.layers import PagedKVCache
+
+    c = PagedKVCache(npages, page, hk, d, cuda, dtype)
+    g = torch.Generator().manual_seed(seed)
+    if fill:
+        for t in (c.key_pages, c.value_pages):
+            x = torch.randn(t.shape, generator=g)
+            t.copy_(x if dtype == BF16 else (x * 40).round().clamp(-127, 127))
+        if dtype == I8:
+            for t in (c.key_scale, c.value_scale):
+                t.copy_(0.01 + 0.03 * torch.rand(t.shape, generator=g))
+    return c
+
+
+def _pages(kv, page, seed=0, spare=2):
+    """A block table for these lengths over a shuffled pool; entries that no length reaches are -1."""
+    per = [-(-k // page) for k in kv]
+    n = sum(per) + spare
+    order = torch.randperm(n, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    table = torch.full((len(kv), max(per + [1]) + 1), -1, dtype=torch.int32)
+    at = 0
+    for b, k in enumerate(per):
+        table[b, :k] = order[at:at + k]
+        at += k
+    return table, n
+
+
+def _cu(lens):
+    return torch.tensor([0] + list(lens)).cumsum(0).to(torch.int32)
+
+
+def _rows64(c, table, b, kv):
+    """Keys and values of sequence b's first kv rows in 64 bits: [kv, n_kv, d] each."""
+    page = c.page_size
+    out = []
+    for t, s in ((c.key_pages, c.key_scale), (c.value_pages, c.value_scale)):
+        at = table[b, : -(-kv // page)].long()
+        x = t.cpu()[at].double()
+        if s is not None:
+            x = x * s.cpu()[at].double()[..., None]
+        out.append(x.transpose(1, 2).reshape(-1, x.shape[1], x.shape[3])[:kv])
+    return out
+
+
+def _ok():
+    from bitnet_tt import _lib
+
+    st, site = _lib.last_device_status()
+    assert st == 0, f"device status {st} at site {site}"
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+def _append_case(cuda, qs, kv, hq, hk, d, page, dtype, rot, interleaved, tab, seed=0, pad=0, extra=0):
+    g = torch.Generator().manual_seed(seed)
+    table, n = _pages(kv, page, seed)
+    c = _cache(cuda, n, page, hk, d, dtype, seed)
+    before = [t.cpu().clone() if t is not None else None for t in (c.key_pages, c.value_pages, c.key_scale, c.value_scale)]
+    cu = _cu(qs)
+    toks, width = int(cu[-1]) + extra, (hq + 2 * hk) * d
+    qkv = torch.randn((toks, width + pad), generator=g).to(BF16)
+    ang = torch.arange(max(kv), dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    cos, sin = ang.cos().to(tab), ang.sin().to(tab)
+    q_out = torch.full((toks, hq * d), 7.0, dtype=BF16, device=cuda)
+    c.append(qkv.to(cuda)[:, :width], cu.to(cuda), torch.tensor(kv, dtype=torch.int32).to(cuda), table.to(cuda),
+             cos.to(cuda), sin.to(cuda), q_out, interleaved)
+    torch.cuda.synchronize()
+    _ok()
+    j = torch.arange(rot // 2)
+    ia, ib = (2 * j, 2 * j + 1) if interleaved else (j, j + rot // 2)
+    written = torch.zeros((n, page), dtype=torch.bool)
+    after = [t.cpu() if t is not None else None for t in (c.key_pages, c.value_pages, c.key_scale, c.value_scale)]
+    for b, (m, k) in enumerate(zip(qs, kv)):
+        for i in range(m):
+            pos, t = k - m + i, int(cu[b]) + i
+            x = qkv[t, :width].double().view(hq + 2 * hk, d)
+            y, slack = x.clone(), torch.zeros_like(x)
+            cs, sn = cos[pos].double(), sin[pos].double()
+            a, bb = x[: hq + hk, ia], x[: hq + hk, ib]
+            y[: hq + hk, ia], y[: hq + hk, ib] = a * cs - bb * sn, bb * cs + a * sn
+            slack[: hq + hk, ia] = slack[: hq + hk, ib] = (a.abs() + bb.abs()) * 2.0 ** -22
+            err = (q_out[t].double().cpu().view(hq, d) - y[:hq]).abs()
+            assert bool((err <= y[:hq].abs() * 2.0 ** -8 + slack[:hq]).all())
+            p, s = int(table[b, pos // page]), pos % page
+            written[p, s] = True
+            for which, lo in ((0, hq), (1, hq + hk)):
+                want, room = y[lo:lo + hk], slack[lo:lo + hk]
+                if dtype == BF16:
+                    got = after[which][p, :, s].double()
+                    assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + room).all())
+                else:
+                    scale = after[2 + which][p, :, s].double()
+                    top = want.abs().amax(-1).clamp(min=1e-5)
+                    # the maximum's own rotation error, and one fp32 division
+                    assert bool(((scale * 127 - top).abs() <= top * 2.0 ** -23 + room.amax(-1)).all())
+                    at = want * (127 / top)[:, None]
+                    code = after[which][p, :, s].double()
+                    # half a code, plus the fp32 errors of the value, the quotient and the product in codes
+                    near = 0.5 + 127 * 2.0 ** -22 + 2 * (room.amax(-1) * 127 / top)[:, None]
+                    assert bool(((code - at).abs() <= near).all())
+    # everything else is as it was
+    for was, now in zip(before, after):
+        if was is not None:
+            keep = ~written
+            assert torch.equal(was.transpose(1, 2)[keep], now.transpose(1, 2)[keep])
+    assert bool((q_out[int(cu[-1]):] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("qs,kv,heads,page,rot,interleaved,tab", [
+    ([1], [1], (20, 5, 128), 16, 128, False, BF16),                    # the first token
+    ([1, 1, 1], [17, 16, 300], (20, 5, 128), 64, 128, False, torch.float32),
+    ([5, 0, 33, 1], [5, 9, 100, 64], (4, 2, 64), 16, 64, False, torch.float32),  # a slot without tokens
+    ([7, 2], [40, 2], (4, 4, 128), 32, 64, False, BF16),               # half the head
+    ([7, 2], [40, 2], (8, 1, 64), 256, 16, True, torch.float32),       # adjacent pairs, a quarter
+    ([70, 1], [129, 130], (6, 3, 128), 128, 96, True, BF16),
+])
+def test_append_against_64_bits(cuda, qs, kv, heads, page, rot, interleaved, tab, dtype):
+    _append_case(cuda, qs, kv, *heads, page, dtype, rot, interleaved, tab, seed=len(qs) + rot)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_append_strided_rows_and_rows_behind_the_last_sequence(cuda, dtype):
+    _append_case(cuda, [3, 4], [19, 4], 4, 2, 64, 16, dtype, 64, False, torch.float32, seed=5, pad=24, extra=3)
+
+
+def test_append_many_sequences_and_tokens(cuda):
+    # more than one round of the sequence search, several tokens a CTA
+    qs = [(i * 7) % 5 for i in range(1100)]
+    qs[0] = 4000
+    kv = [max(1, q) + i % 3 for i, q in enumerate(qs)]
+    table, n = _pages(kv, 16)
+    c = _cache(cuda, n, 16, 1, 64, BF16)
+    cu = _cu(qs)
+    qkv = torch.randn((int(cu[-1]), 3 * 64), generator=torch.Generator().manual_seed(1)).to(BF16)
+    one, zero = torch.ones((max(kv), 32), device=cuda), torch.zeros((max(kv), 32), device=cuda)
+    q = c.append(qkv.to(cuda), cu.to(cuda), torch.tensor(kv, dtype=torch.int32).to(cuda), table.to(cuda), one, zero)
+    _ok()
+    assert torch.equal(q.cpu(), qkv[:, :64])  # no turn: copied
+    starts = torch.tensor([k - m for k, m in zip(kv, qs)], dtype=torch.int32).to(cuda)
+    k, v = c.read(table.to(cuda), starts, cu.to(cuda), int(cu[-1]))
+    assert torch.equal(k.cpu().view(-1, 64), qkv[:, 64:128]) and torch.equal(v.cpu().view(-1, 64), qkv[:, 128:])
+
+
+def test_append_int8_rows_of_zeros_tiny_values_and_infinities(cuda):
+    c = _cache(cuda, 3, 16, 1, 64, I8, fill=False)
+    x = torch.zeros((6, 3 * 64))
+    x[1, 64:] = 1e-7           # below the floor 1e-5: codes of at most 1
+    x[2, 64 + 5] = float("inf")
+    x[3, 128 + 9] = float("nan")
+    x[4, 64:] = 3e38
+    x[5, 64:] = torch.linspace(-1, 1, 128)
+    tab = torch.ones((6, 32), device=cuda), torch.zeros((6, 32), device=cuda)
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device=cuda)
+    args = (torch.tensor([0, 6], dtype=torch.int32, device=cuda), torch.tensor([6], dtype=torch.int32, device=cuda), table)
+    c.append(x.to(BF16).to(cuda), *args, *tab)
+    k, v = c.read(table, None, args[0], 6)
+    _ok()
+    k, v = k.float().cpu()[:, 0], v.float().cpu()[:, 0]
+    assert bool((k[0] == 0).all()) and bool((v[0] == 0).all())
+    assert float(k[1].abs().max()) <= 1e-5 / 127 * 1.01
+    assert bool(k[2].isnan().all()) and bool((v[2] == 0).all())
+    assert bool((k[3] == 0).all()) and bool(v[3].isnan().all())
+    big = float(x[4, 64].to(BF16))
+    assert bool((k[4] - big).abs().max() <= big * 2.0 ** -7)
+    want = x[5, 64:128].to(BF16).float()
+    assert float((k[5] - want).abs().max()) <= 0.5 / 127 * 1.01 + 2.0 ** -8
+
+
+# ---------------------------------------------------------------------------
+# read
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 64), (128, 256)])
+def test_read_is_the_rounded_value(cuda, d, page, dtype):
+    kv = [1, page, page + 1, 3 * page - 1, 500]
+    table, n = _pages(kv, page, 3)
+    c = _cache(cuda, n, page, 3, d, dtype, 4)
+    starts = torch.tensor([0, 1, page - 1, 5, 500], dtype=torch.int32)  # the last: no row left
+    lens = [k - int(s) for k, s in zip(kv, starts)]
+    k, v = c.read(table.to(cuda), starts.to(cuda), _cu(lens).to(cuda), sum(lens) + 2,
+                  *(torch.full((sum(lens) + 2, 3, d), 7.0, dtype=BF16, device=cuda) for _ in range(2)))
+    _ok()
+    for t, s, got in ((c.key_pages, c.key_scale, k.cpu()), (c.value_pages, c.value_scale, v.cpu())):
+        want = []
+        for b, m in enumerate(kv):
+            at = table[b, : -(-m // page)].long()
+            x = t.cpu()[at].float()
+            if s is not None:
+                x = x * s.cpu()[at][..., None]
+            want.append(x.transpose(1, 2).reshape(-1, 3, d)[int(starts[b]):m])
+        assert torch.equal(got[: sum(lens)], torch.cat(want).to(BF16))
+        assert bool((got[sum(lens):] == 7).all())
+
+
+# ---------------------------------------------------------------------------
+# attend
+# ---------------------------------------------------------------------------
+def _attend_case(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, max_q=None, max_kv=None, pad=0, extra=0, poison=True):
+    """Against the softmax in 64 bits.  The rows of the pools that no sequence
+    reaches hold NaN (bf16) or have NaN scales (int8)."""
+    g = torch.Generator().manual_seed(seed)
+    table, n = _pages(kv, page, seed)
+    c = _cache(cuda, n, page, hk, d, dtype, seed)
+    if poison:
+        used = torch.zeros((n, page), dtype=torch.bool)
+        for b, k in enumerate(kv):
+            for i in range(0, k, page):
+                used[int(table[b, i // page]), : min(page, k - i)] = True
+        for t in ((c.key_pages, c.value_pages) if dtype == BF16 else (c.key_scale, c.value_scale)):
+            t.transpose(1, 2)[~used.to(cuda)] = float("nan")
+    cu = _cu(qs)
+    toks = int(cu[-1]) + extra
+    q = torch.randn((toks, hq * d + pad), generator=g).to(BF16)
+    out = torch.full((toks, hq * d), 7.0, dtype=BF16, device=cuda)
+    c.attend(q.to(cuda)[:, : hq * d], cu.to(cuda), torch.tensor(kv, dtype=torch.int32).to(cuda), table.to(cuda),
+             max_q or max(qs), max_kv or max(kv), out=out)
+    torch.cuda.synchronize()
+    _ok()
+    assert bool((out[int(cu[-1]):] == 7).all())
+    got = out.double().cpu().view(toks, hq, d)
+    grp = hq // hk
+    for b, (m, k) in enumerate(zip(qs, kv)):
+        if m == 0:
+            continue
+        kk, vv = _rows64(c, table, b, k)
+        # one bf16 weight where the tensor-memory kernel takes the rows, a pair below
+        weight = 2.0 ** -8 if m * grp > 16 else 2.0 ** -16
+        see = torch.arange(k)[None] < (k - m + torch.arange(m)[:, None] + 1)
+        for h in range(hq):
+            qq = q[int(cu[b]):int(cu[b + 1]), h * d:(h + 1) * d].double()
+            assert k == 0 or float((qq.abs() @ kk[:, h // grp].abs().T).max()) * d ** -0.5 < 32
+            s = (qq @ kk[:, h // grp].T * d ** -0.5).masked_fill(~see, -float("inf"))
+            top = s.amax(-1, keepdim=True).clamp(min=-1e300) if k else torch.zeros((m, 1))
+            p = torch.exp(s - top)
+            p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+            want, spread = p @ vv[:, h // grp], p @ vv[:, h // grp].abs()
+            err = (got[int(cu[b]):int(cu[b + 1]), h] - want).abs()
+            room = want.abs() * 2.0 ** -8 + (2.0 ** -11 + weight) * spread
+            worst = float((err - room).max())
+            assert worst <= 0, f"sequence {b} head {h}: {worst} over the bound"
+
+
+HEAD_LAYOUTS = [(20, 5, 128), (4, 2, 64), (4, 4, 128), (16, 2, 64), (3, 1, 128), (17, 1, 64)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("heads", HEAD_LAYOUTS)
+def test_attend_one_token(cuda, heads, dtype):
+    # one key, the ends of tiles and pages, an idle slot, an odd length
+    qs = [1, 1, 1, 1, 0, 1, 1]
+    _attend_case(cuda, qs, [1, 16, 17, 64, 30, 129, 333], *heads, 16, dtype, seed=heads[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_attend_page_sizes(cuda, page, dtype):
+    _attend_case(cuda, [1, 2, 3, 0, 40], [300, 255, 256, 77, 513], 8, 2, 128, page, dtype, seed=page)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("heads", HEAD_LAYOUTS)
+def test_attend_chunks(cuda, heads, dtype):
+    # whole prompts and chunks of one, of odd lengths, beside single tokens
+    _attend_case(cuda, [130, 1, 65, 0, 7, 33], [130, 200, 400, 10, 7, 34], *heads, 64, dtype, seed=heads[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_attend_long_chunks_cross_tiles(cuda, dtype):
+    _attend_case(cuda, [257, 300], [700, 300], 4, 1, 64, 16, dtype, seed=9)
+    _attend_case(cuda, [129, 1000], [1290, 1000], 2, 2, 128, 128, dtype, seed=10)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("qs,kv", [([1], [5000]), ([3, 1], [4097, 2]), ([20], [6000]), ([1, 64], [9000, 70])])
+def test_attend_splits_long_contexts(cuda, qs, kv, dtype):
+    from bitnet_tt import _lib
+
+    assert _lib.paged_attention_workspace_bytes(len(qs), sum(qs), max(qs), max(kv), 8, 2, 128) > 0
+    _attend_case(cuda, qs, kv, 8, 2, 128, 32, dtype, seed=kv[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_attend_loose_bounds_strided_queries_and_rows_behind(cuda, dtype):
+    _attend_case(cuda, [2, 5], [70, 5], 4, 2, 64, 16, dtype, seed=3, max_q=40, max_kv=80, pad=40, extra=3)
+    _attend_case(cuda, [1, 1], [70, 5], 4, 2, 64, 16, dtype, seed=3, max_q=1, max_kv=80, pad=8, extra=2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("qs,kv", [([3, 2], [1, 0]), ([40, 50], [20, 0]), ([1], [0])])
+def test_attend_tokens_that_see_nothing_get_zeros(cuda, qs, kv, dtype):
+    # more new tokens than keys: the first ones stand before the first key
+    _attend_case(cuda, qs, kv, 4, 2, 128, 16, dtype, seed=1, max_kv=32)
+
+
+def test_attend_many_sequences(cuda):
+    # more than 32 sequences in the block search, chunks among single tokens
+    qs = [1] * 70 + [30] + [0] * 5 + [1] * 20 + [65]
+    kv = [(37 * i) % 190 + q + 1 for i, q in enumerate(qs)]
+    _attend_case(cuda, qs, kv, 4, 2, 64, 16, BF16, seed=2)
+    _attend_case(cuda, [min(q, 1) for q in qs], kv, 4, 2, 64, 16, I8, seed=2)
+
+
+def test_attend_sequences_may_share_pages(cuda):
+    """Two sequences with a common prefix page and the same last token agree."""
+    c = _cache(cuda, 6, 16, 2, 64, BF16, 8)
+    table = torch.tensor([[3, 1], [3, 4]], dtype=torch.int32, device=cuda)
+    c.key_pages[4], c.value_pages[4] = c.key_pages[1], c.value_pages[1]
+    q = torch.randn((1, 4 * 64), generator=torch.Generator().manual_seed(2)).to(BF16).to(cuda).expand(2, -1).contiguous()
+    o = c.attend(q, torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda),
+                 torch.tensor([25, 25], dtype=torch.int32, device=cuda), table, 1, 25)
+    _ok()
+    assert torch.equal(o[0], o[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_attend_does_not_depend_on_the_batch_around_it(cuda, dtype):
+    """The same call twice gives the same bits."""
+    table, n = _pages([3000, 50], 64)
+    c = _cache(cuda, n, 64, 2, 128, dtype, 1)
+    q = torch.randn((41, 8 * 128), generator=torch.Generator().manual_seed(4)).to(BF16).to(cuda)
+    args = (q, _cu([1, 40]).to(cuda), torch.tensor([3000, 50], dtype=torch.int32, device=cuda), table.to(cuda), 40, 3000)
+    a, b = c.attend(*args), c.attend(*args)
+    _ok()
+    assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# device data that does not hold, streams and graphs
+# ---------------------------------------------------------------------------
+def _bounds(run):
+    from bitnet_tt import _lib
+
+    run()
+    st, site = _lib.last_device_status()
+    assert st == -1 and 340 <= site < 360, (st, site)
+    _ok()  # cleared
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_bad_pages_and_lengths_are_reported_and_skipped(cuda, nq, dtype):
+    i32 = dict(dtype=torch.int32, device=cuda)
+    c = _cache(cuda, 6, 16, 2, 64, dtype, 8)
+    before = c.key_pages.clone()
+    qkv = torch.zeros((2 * nq, 8 * 64), dtype=BF16, device=cuda)
+    q = torch.ones((2 * nq, 4 * 64), dtype=BF16, device=cuda)
+    tab = torch.ones((64, 32), device=cuda), torch.zeros((64, 32), device=cuda)
+    cu, lens = torch.tensor([0, nq, 2 * nq], **i32), torch.tensor([48, 48], **i32)
+    for bad in (-1, 6, 1 << 30, -(1 << 31)):
+        table = torch.full((2, 3), bad, **i32)
+        _bounds(lambda: c.append(qkv, cu, lens, table, *tab))
+        _bounds(lambda: c.attend(q, cu, lens, table, nq, 48))
+        _bounds(lambda: c.read(table, None, torch.tensor([0, 48, 96], **i32), 96))
+    table = torch.tensor([[0, 1, 2], [3, 4, 5]], **i32)
+    for kv in ([-5, -5], [49, 49], [1 << 30, 1 << 30]):
+        out = torch.full((2 * nq, 4 * 64), 7.0, dtype=BF16, device=cuda)
+        _bounds(lambda: c.append(qkv, cu, torch.tensor(kv, **i32), table, *tab))
+        _bounds(lambda: c.attend(q, cu, torch.tensor(kv, **i32), table, nq, 48, out=out))
+        assert bool((out == 7).all())
+    for offsets in ([0, nq, 2 * nq + 1], [0, -1, nq], [nq + 1, nq + 2, nq + 3] if nq == 1 else [0, 81, 90]):
+        _bounds(lambda: c.attend(q, torch.tensor(offsets, **i32), lens, table, nq, 48))
+    _bounds(lambda: c.read(table, torch.tensor([1, 47], **i32), torch.tensor([0, 48, 96], **i32), 96))
+    _bounds(lambda: c.append(qkv, cu, torch.tensor([nq, nq - 1], **i32), table, *tab))
+    if nq > 1:
+        short = torch.ones((8, 32), device=cuda), torch.zeros((8, 32), device=cuda)
+        _bounds(lambda: c.append(qkv, cu, lens, table, *short))
+    del before
+
+
+def test_library_refusals_reach_the_caller(cuda):
+    c = _cache(cuda, 6, 16, 2, 64, BF16)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    q = torch.zeros((1, 4 * 64), dtype=BF16, device=cuda)
+    table, cu, lens = torch.zeros((1, 2), **i32), torch.tensor([0, 1], **i32), torch.tensor([4], **i32)
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        c.attend(q, cu, lens, table, 1, 33)  # more keys than the table's pages hold
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        big = torch.zeros((1, 512), **i32)
+        c.attend(q, cu, lens, big, 1, 8192, workspace=torch.empty(16, dtype=torch.uint8, device=cuda))
+    with pytest.raises(RuntimeError, match="aligned"):
+        odd = torch.zeros(4 * 64 + 8, dtype=BF16, device=cuda)[1:257].view(1, 256)
+        c.attend(odd, cu, lens, table, 1, 4)
+    assert c.attend(q[:0], torch.zeros(2, **i32), lens, table, 1, 4).shape == (0, 256)
+    assert c.read(table, None, torch.zeros(2, **i32), 0)[0].shape == (0, 2, 64)
+    _ok()
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_append_then_attend_captured_and_replayed_on_another_stream(cuda, dtype):
+    """A decode loop: the captured pair extends and attends as the eager calls do,
+    with lengths and queries changed in place between replays."""
+    hq, hk, d, page, b = 8, 2, 128, 16, 3
+    i32 = dict(dtype=torch.int32, device=cuda)
+    kv0 = [600, 3, 31]
+    table, n = _pages([k + 8 for k in kv0], page, 5)
+    eager, graph = (_cache(cuda, n, page, hk, d, dtype, 6) for _ in range(2))
+    table = table.to(cuda)
+    ang = torch.arange(700, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+    cos, sin = ang.cos().float().to(cuda), ang.sin().float().to(cuda)
+    cu, lens = _cu([1] * b).to(cuda), torch.tensor(kv0, **i32)
+    qkv = torch.zeros((b, (hq + 2 * hk) * d), dtype=BF16, device=cuda)
+    q, out = (torch.zeros((b, hq * d), dtype=BF16, device=cuda) for _ in range(2))
+
+    def step(c):
+        lens.add_(1)
+        c.append(qkv, cu, lens, table, cos, sin, q)
+        c.attend(q, cu, lens, table, 1, 616, out=out)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(graph)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        step(graph)
+    for t, s_ in ((eager.key_pages, graph.key_pages), (eager.value_pages, graph.value_pages),
+                  (eager.key_scale, graph.key_scale), (eager.value_scale, graph.value_scale)):
+        if t is not None:
+            t.copy_(s_)
+    lens.copy_(torch.tensor(kv0, **i32))
+    gen = torch.Generator().manual_seed(9)
+    rows = [torch.randn(qkv.shape, generator=gen).to(BF16).to(cuda) for _ in range(5)]
+    want = []
+    for r in rows:
+        qkv.copy_(r)
+        step(eager)
+        want.append(out.clone())
+    lens.copy_(torch.tensor(kv0, **i32))
+    for r, w in zip(rows, want):
+        qkv.copy_(r)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, w)
+    assert torch.equal(eager.key_pages, graph.key_pages) and torch.equal(eager.value_pages, graph.value_pages)
+    _ok()
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """The last pages of a pool of more than 2^32 bytes per tensor."""
+    free = torch.cuda.mem_get_info()[0]
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    from bitnet_tt.layers import PagedKVCache
+
+    n = (5 << 30) // (256 * 5 * 128 * 2)  # 5 GiB a pool: 2.7e9 values
+    c = PagedKVCache(n, 256, 5, 128, cuda, BF16)
+    table = torch.tensor([[n - 1, 0, n - 2]], dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn((600, 30 * 128), generator=g).to(BF16).to(cuda)
+    one, zero = torch.ones((600, 64), device=cuda), torch.zeros((600, 64), device=cuda)
+    cu, lens = torch.tensor([0, 600], dtype=torch.int32, device=cuda), torch.tensor([600], dtype=torch.int32, device=cuda)
+    q = c.append(qkv, cu, lens, table, one, zero)
+    k, v = c.read(table, None, cu, 600)
+    assert torch.equal(k.view(600, -1), qkv[:, 2560:3200]) and torch.equal(v.view(600, -1), qkv[:, 3200:])
+    small = PagedKVCache(3, 256, 5, 128, cuda, BF16)
+    at = torch.tensor([[2, 0, 1]], dtype=torch.int32, device=cuda)
+    small.append(qkv, cu, lens, at, one, zero)
+    assert torch.equal(c.attend(q, cu, lens, table, 600, 600), small.attend(q, cu, lens, at, 600, 600))
+    last = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
+    assert torch.equal(c.attend(q[-1:], last, lens, table, 1, 600), small.attend(q[-1:], last, lens, at, 1, 600))
+    _ok()
