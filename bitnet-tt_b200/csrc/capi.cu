@@ -28,6 +28,7 @@
 #include "lm_head_tc.cuh"
 #include "pack.cuh"
 #include "paged_attention.cuh"
+#include "paged_chunk.cuh"
 #include "paged_kv.cuh"
 #include "../../include/bitnet_b200.h"
 
@@ -178,7 +179,7 @@ int to_dev_segments(const bitnet_segments_t* s, int N, int epilogue, bitnet_segm
 }
 
 std::atomic<unsigned long long> g_smem_aq{0}, g_smem_aq_stage{0}, g_smem_simt[3][4], g_smem_tc[3], g_smem_lmh{0}, g_smem_att[4],
-    g_smem_apf{0}, g_smem_pra[4];
+    g_smem_apf{0}, g_smem_pra[4], g_smem_pch[4];
 
 int lm_head_tile_T(int B) { return round_up(B, 16); }
 size_t lm_head_part_bytes(int B, int grid) { return (size_t)grid * B * sizeof(ArgPair); }
@@ -1169,10 +1170,16 @@ int launch_paged_append(const PagedAppendParams& p, bool f32, dim3 grid, bitnet_
              : launch(paged_append_kernel<D, I8, false>, grid, dim3(PKV_THREADS), 0, st, 1, p);
 }
 
-// How an attention call is cut: row blocks (grid.x) and parts of the keys.
-struct PagedPlan {
+// How an attention call is cut for one of its kernels: row blocks (grid.x; 0: not
+// launched) and parts of the keys, and where its partial results lie.
+struct PagedCut {
   int blocks, nsplit, span;
-  size_t ml_bytes, bytes;  // workspace: maxima and sums, then outputs
+  size_t ml, o;  // offsets in the workspace
+};
+struct PagedPlan {
+  PagedCut rows, chunk;
+  int small;
+  size_t bytes;
 };
 
 // Parts of the keys for `pairs` blocks of work on `slots` CTAs at once: the s
@@ -1191,14 +1198,26 @@ int paged_splits(long long pairs, int max_kv, int slots, int unit, int min_span)
 
 PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, int D, int sms) {
   PagedPlan pl;
-  const long long blocks =
-      (long long)max_q * G <= PRA_R ? B : ((long long)tokens * G + PRA_R - 1) / PRA_R + B;
-  pl.blocks = (int)std::min(blocks, (long long)INT_MAX);
-  pl.nsplit = paged_splits((long long)pl.blocks * n_kv, max_kv, sms * 3, ATT_UNIT_COST, ATT_MIN_SPLIT);
-  pl.span = round_up((max_kv + pl.nsplit - 1) / pl.nsplit, PRA_TILE);
-  const size_t rows = pl.nsplit > 1 ? (size_t)pl.nsplit * pl.blocks * n_kv * PRA_R : 0;
-  pl.ml_bytes = rows * sizeof(float2);
-  pl.bytes = pl.ml_bytes + rows * D * sizeof(float);
+  memset(&pl, 0, sizeof(pl));
+  size_t at = 0;
+  auto cut = [&](PagedCut& c, long long blocks, int R, int slots, int unit, int min_span, int round) {
+    c.blocks = (int)std::min(blocks, (long long)INT_MAX);
+    c.nsplit = paged_splits((long long)c.blocks * n_kv, max_kv, slots, unit, min_span);
+    c.span = round_up(std::max(1, (max_kv + c.nsplit - 1) / c.nsplit), round);
+    const size_t rows = c.nsplit > 1 ? (size_t)c.nsplit * c.blocks * n_kv * R : 0;
+    c.ml = at;
+    c.o = c.ml + rows * sizeof(float2);
+    at = c.o + rows * D * sizeof(float);
+  };
+  const bool chunks = (long long)max_q * G > PRA_R;
+  // Where most sequences may be as long as the longest, the chunk kernel takes the
+  // short ones along: a launch for none or few of them costs more than they do.
+  pl.small = chunks && (long long)tokens * 2 < (long long)B * max_q ? PRA_R : 0;
+  if (!chunks || pl.small) cut(pl.rows, B, PRA_R, sms * 3, ATT_UNIT_COST, ATT_MIN_SPLIT, PRA_TILE);
+  if (chunks)
+    cut(pl.chunk, ((long long)tokens * G + PCH_R - 1) / PCH_R + std::min((long long)B, (long long)tokens), PCH_R, sms,
+        256, 512, PCH_KB);
+  pl.bytes = at;
   return pl;
 }
 
@@ -1208,15 +1227,91 @@ bool paged_attn_sizes(int B, int tokens, int max_q, int max_kv, int n_heads, int
          (long long)max_q * n_heads <= INT_MAX / 2 && max_kv <= INT_MAX - 4096;
 }
 
-template <int D, bool I8>
-int launch_paged_attention(const PagedAttnParams& p, bitnet_stream_t st) {
-  if (int e = ensure_smem(paged_rows_kernel<D, I8>, &g_smem_pra[(D == 128) * 2 + I8])) return e;
-  if (int e = launch(paged_rows_kernel<D, I8>, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(PRA_THREADS),
-                     PraShape<D, I8>::SMEM, st, 1, p))
-    return e;
+// The driver's tensor-map encoder, looked up once (the library links no driver).
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int encode_tiled(EncodeTiled* out) {
+  static std::atomic<void*> fn{nullptr};
+  void* f = fn.load();
+  if (f == nullptr) {
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaGetDriverEntryPointByVersion(cuTensorMapEncodeTiled)");
+    if (found != cudaDriverEntryPointSuccess || f == nullptr)
+      return cuda_fail(cudaErrorNotSupported, "cuTensorMapEncodeTiled");
+    fn.store(f);
+  }
+  *out = reinterpret_cast<EncodeTiled>(f);
+  return BITNET_OK;
+}
+
+// A bf16 pool as rows of head_dim; a box is 64 dims of the rows of a page (at most
+// a key tile), swizzled as the MMA reads them.
+int paged_map(CUtensorMap* m, const PagedKV& kv, const void* pool, int D) {
+  EncodeTiled enc;
+  if (int e = encode_tiled(&enc)) return e;
+  const cuuint64_t dims[2] = {(cuuint64_t)D, ((cuuint64_t)kv.num_pages * kv.n_kv) << kv.page_shift};
+  const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)std::min(1 << kv.page_shift, PCH_KB)}, elem[2] = {1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return BITNET_OK;
+  snprintf(g_cuda_msg, sizeof(g_cuda_msg), "cuTensorMapEncodeTiled: error %d", (int)r);
+  return BITNET_ERR_CUDA;
+}
+
+void paged_apply(PagedAttnParams* p, const PagedCut& c, void* workspace) {
+  p->blocks = c.blocks;
+  p->nsplit = c.nsplit;
+  p->span = c.span;
+  p->part_ml = (float2*)((uint8_t*)workspace + c.ml);
+  p->part_o = (float*)((uint8_t*)workspace + c.o);
+}
+
+template <int D, int R>
+int launch_paged_join(const PagedAttnParams& p, bitnet_stream_t st) {
   if (p.nsplit == 1) return BITNET_OK;
-  const int rows = std::min(PRA_R, p.max_q * p.G);
-  return launch(paged_join_kernel<D, PRA_R>, dim3(p.blocks, p.kv.n_kv, (rows + 3) / 4), dim3(128), 0, st, 1, p);
+  const int rows = (int)std::min((long long)R, (long long)p.max_q * p.G);
+  return launch(paged_join_kernel<D, R>, dim3(p.blocks, p.kv.n_kv, (rows + 3) / 4), dim3(128), 0, st, 1, p);
+}
+
+template <int D, bool I8>
+int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspace, bitnet_stream_t st) {
+  constexpr int idx = (D == 128) * 2 + I8;
+  p.small = pl.small;
+  if (pl.chunk.blocks > 0) {
+    using S = PchShape<D, I8>;
+    auto k = paged_chunk_kernel<D, I8>;
+    static std::atomic<int> regs{0};  // the register shares are part of the launch's registers
+    if (regs.load() == 0) {
+      cudaFuncAttributes fa;
+      const cudaError_t e = cudaFuncGetAttributes(&fa, k);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+      regs.store(fa.numRegs);
+    }
+    if (regs.load() != S::REGS_LAUNCH) return cuda_fail(cudaErrorInvalidConfiguration, "paged_chunk_kernel registers");
+    if (int e = ensure_smem(k, &g_smem_pch[idx])) return e;
+    CUtensorMap mk, mv;
+    memset(&mk, 0, sizeof(mk));
+    memset(&mv, 0, sizeof(mv));
+    if (!I8) {
+      if (int e = paged_map(&mk, p.kv, p.kv.k, D)) return e;
+      if (int e = paged_map(&mv, p.kv, p.kv.v, D)) return e;
+    }
+    paged_apply(&p, pl.chunk, workspace);
+    if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(S::THREADS), S::SMEM, st, 1, p, mk, mv)) return e;
+    if (int e = launch_paged_join<D, PCH_R>(p, st)) return e;
+  }
+  if (pl.rows.blocks > 0) {
+    auto k = paged_rows_kernel<D, I8>;
+    if (int e = ensure_smem(k, &g_smem_pra[idx])) return e;
+    paged_apply(&p, pl.rows, workspace);
+    if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(PRA_THREADS), PraShape<D, I8>::SMEM, st, 1, p)) return e;
+    if (int e = launch_paged_join<D, PRA_R>(p, st)) return e;
+  }
+  return BITNET_OK;
 }
 
 }  // namespace
@@ -1315,6 +1410,7 @@ int bitnet_paged_attention(const bitnet_paged_kv_t* kv, const int32_t* block_tab
     return BITNET_ERR_INVALID_ARGUMENT;
   if ((long long)max_kv_len > (long long)max_pages * kv->page_size) return BITNET_ERR_INVALID_ARGUMENT;
   if ((long long)n_heads * D > ld_q || ld_q % 8 != 0) return BITNET_ERR_INVALID_ARGUMENT;
+  if (!(scale > 0.f) || scale > 1e30f) return BITNET_ERR_INVALID_ARGUMENT;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(cu_seqlens, 4) || !aligned(kv_lens, 4)) return BITNET_ERR_ALIGNMENT;
   DevInfo* d;
   if (int e = device_info(&d)) return e;
@@ -1336,15 +1432,12 @@ int bitnet_paged_attention(const bitnet_paged_kv_t* kv, const int32_t* block_tab
   p.n_heads = n_heads;
   p.G = G;
   p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  p.nsplit = pl.nsplit;
-  p.span = pl.span;
-  p.blocks = pl.blocks;
-  p.part_ml = (float2*)workspace;
-  p.part_o = (float*)((uint8_t*)workspace + pl.ml_bytes);
   p.out = (uint16_t*)out;
   if (kv->kv_type == BITNET_KV_INT8)
-    return D == 128 ? launch_paged_attention<128, true>(p, stream) : launch_paged_attention<64, true>(p, stream);
-  return D == 128 ? launch_paged_attention<128, false>(p, stream) : launch_paged_attention<64, false>(p, stream);
+    return D == 128 ? launch_paged_attention<128, true>(p, pl, workspace, stream)
+                    : launch_paged_attention<64, true>(p, pl, workspace, stream);
+  return D == 128 ? launch_paged_attention<128, false>(p, pl, workspace, stream)
+                  : launch_paged_attention<64, false>(p, pl, workspace, stream);
 }
 
 }  // extern "C"

@@ -8,7 +8,8 @@
 //
 // The G = n_heads / n_kv query heads of a KV head share its keys, so a block of
 // work is a run of packed rows of one (sequence, KV head): row r is token r / G,
-// head g G + r % G.
+// head g G + r % G.  Sequences of up to 16 rows (decode, a few drafted tokens) go to
+// paged_rows_kernel here, longer ones to paged_chunk_kernel (paged_chunk.cuh).
 #pragma once
 #include "attention.cuh"
 #include "common.cuh"
@@ -26,6 +27,7 @@ struct PagedAttnParams {
   float scale_log2;    // scale * log2(e)
   int nsplit, span;    // the keys are cut into nsplit parts of span keys
   int blocks;          // grid.x: row blocks, an upper bound
+  int small;           // chunk kernel: sequences of up to this many rows are not its own
   float2* part_ml;     // [nsplit][blocks][n_kv][R] (maximum, sum)
   float* part_o;       // [nsplit][blocks][n_kv][R][D], unnormalised
   uint16_t* out;       // [tokens][n_heads * D]
@@ -39,36 +41,10 @@ struct PagedBlock {
   int kend;    // keys that the block's last row sees, not below 0
 };
 
-// Finds block `bx` (of up to R rows) over all sequences; whole warp.  With one
-// block a sequence at most (max_q * G <= R) block bx is sequence bx.  False when
-// there is no such block, or when the sequence's lengths do not hold.
+// Rows row0 .. of sequence b in a block of up to R rows.  False when the sequence
+// has no new token, or when its lengths do not hold.
 template <int R>
-__device__ __forceinline__ bool paged_block(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
-  int b = bx, blk = 0;
-  if (p.max_q * p.G > R) {
-    bool found = false;
-    for (int b0 = 0; b0 < p.B && !found; b0 += 32) {
-      const int i = b0 + lane;
-      const int n = i < p.B ? min(max(p.cu[i + 1] - p.cu[i], 0), p.max_q) : 0;
-      const int nb = (n * p.G + R - 1) / R;
-      int sum = nb;
-#pragma unroll
-      for (int o2 = 1; o2 < 32; o2 <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o2);
-        if (lane >= o2) sum += v;
-      }
-      const unsigned above = __ballot_sync(0xffffffffu, sum > bx);
-      if (above) {
-        const int src = __ffs(above) - 1;
-        b = b0 + src;
-        blk = bx - __shfl_sync(0xffffffffu, sum - nb, src);
-        found = true;
-      } else {
-        bx -= __shfl_sync(0xffffffffu, sum, 31);
-      }
-    }
-    if (!found) return false;
-  }
+__device__ __forceinline__ bool paged_block_of(const PagedAttnParams& p, int b, int row0, int lane, PagedBlock& o) {
   const int lo = p.cu[b], n = p.cu[b + 1] - lo, kv = p.kv_lens[b];
   if (n == 0) return false;
   if (n < 0 || n > p.max_q || lo < 0 || lo > p.tokens - n || kv < 0 || kv > p.max_kv) {
@@ -76,12 +52,44 @@ __device__ __forceinline__ bool paged_block(const PagedAttnParams& p, int bx, in
     return false;
   }
   o.b = b;
-  o.row0 = blk * R;
-  o.nrows = min(R, n * p.G - o.row0);
+  o.row0 = row0;
+  o.nrows = min(R, n * p.G - row0);
   o.tok0 = lo;
   o.past = kv - n;
-  o.kend = max(0, o.past + (o.row0 + o.nrows - 1) / p.G + 1);
+  o.kend = max(0, o.past + (row0 + o.nrows - 1) / p.G + 1);
   return true;
+}
+
+// Sequences of up to R rows: block b is sequence b; the others are not this
+// kernel's.
+template <int R>
+__device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int b, int lane, PagedBlock& o) {
+  if ((long long)(p.cu[b + 1] - p.cu[b]) * p.G > R && p.max_q * p.G > R) return false;
+  return paged_block_of<R>(p, b, 0, lane, o);
+}
+
+// Block bx of the R-row blocks of all sequences of more than p.small rows, in
+// order; whole warp.
+template <int R>
+__device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int i = b0 + lane;
+    const int rows = (i < p.B ? min(max(p.cu[i + 1] - p.cu[i], 0), p.max_q) : 0) * p.G;
+    const int nb = rows > p.small ? (rows + R - 1) / R : 0;
+    int sum = nb;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    const unsigned above = __ballot_sync(0xffffffffu, sum > bx);
+    if (above) {
+      const int src = __ffs(above) - 1;
+      return paged_block_of<R>(p, b0 + src, (bx - __shfl_sync(0xffffffffu, sum - nb, src)) * R, lane, o);
+    }
+    bx -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
 }
 
 __device__ __forceinline__ int paged_parts(const PagedAttnParams& p, int kend) {
@@ -161,7 +169,7 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
   pdl_trigger();
   pdl_wait();
   PagedBlock blk;
-  if (!paged_block<PRA_R>(p, blockIdx.x, lane, blk)) return;
+  if (!paged_block_direct<PRA_R>(p, blockIdx.x, lane, blk)) return;
   const int g = blockIdx.y, sp = blockIdx.z;
   const int nparts = paged_parts(p, blk.kend);
   if (sp >= nparts) return;
@@ -420,7 +428,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
   pdl_trigger();
   pdl_wait();
   PagedBlock blk;
-  if (!paged_block<R>(p, blockIdx.x, lane, blk)) return;
+  if (!(R == PRA_R ? paged_block_direct<R>(p, blockIdx.x, lane, blk) : paged_block_search<R>(p, blockIdx.x, lane, blk)))
+    return;
   const int nparts = paged_parts(p, blk.kend);
   if (nparts == 1 || r >= blk.nrows) return;
   const size_t step = (size_t)p.blocks * p.kv.n_kv;

@@ -303,8 +303,8 @@ int bitnet_attention_prefill_varlen(const void* q, const void* k_cache, const vo
  * device memory.  Rows from cu_seqlens[B] on (total_tokens may be larger) are
  * left as they were.  A page id outside the pool, a position outside the table
  * or the rotary tables, or lengths beyond the bounds passed in are device bounds
- * errors (bitnet_last_device_status): the row or sequence is skipped, and an
- * attention that met a bad page reads zeros there.  Sequences may share pages
+ * errors (bitnet_last_device_status): the row or sequence is skipped; of a sequence
+ * with a bad page the attention's rows are undefined.  Sequences may share pages
  * for reading; a row that two tokens of one call write is undefined. */
 #define BITNET_KV_BF16 0
 #define BITNET_KV_INT8 1
@@ -342,7 +342,7 @@ int bitnet_paged_read(const bitnet_paged_kv_t* kv, const int32_t* block_table, i
  * sequences' pages: token i of n sees the first kv_lens[b] - n + i + 1 keys, and
  * one that sees none (kv_lens[b] < n) gets zeros.  q: bf16, row stride ld_q
  * elements (a multiple of 8), rotated; out: bf16 [total_tokens][n_heads * head_dim];
- * both 16-byte aligned.  n_heads / n_kv_heads is at most 64.  max_seqlen and max_kv_len bound the new
+ * both 16-byte aligned.  n_heads / n_kv_heads is at most 64; scale is positive.  max_seqlen and max_kv_len bound the new
  * tokens and the keys of every sequence; they size the grid and the split of long
  * contexts, so tight bounds keep both small.  Cache rows below kv_lens[b] have to
  * be finite; whatever stands behind them does not matter.  workspace:

@@ -60,7 +60,9 @@ OWN = {
                                ({"q": 8}, -2), ({"out": 8}, -2), ({"kv_lens": 2}, -2), ({"ld_q": 255}, -1),
                                ({"ld_q": 248}, -1), ({"ld_q": 260}, -1), ({"total_tokens": -1}, -1),
                                ({"max_seqlen": -1}, -1), ({"max_kv_len": -1}, -1), ({"max_kv_len": 65}, -1),
-                               ({"n_heads": 3}, -1), ({"n_heads": 0}, -1), ({"n_heads": 130, "ld_q": 8320}, -1)],
+                               ({"n_heads": 3}, -1), ({"n_heads": 0}, -1), ({"n_heads": 130, "ld_q": 8320}, -1),
+                               ({"scale": 0.0}, -1), ({"scale": -1.0}, -1), ({"scale": float("nan")}, -1),
+                               ({"scale": float("inf")}, -1)],
 }
 
 

@@ -358,7 +358,7 @@ def _bounds(run):
 
     run()
     st, site = _lib.last_device_status()
-    assert st == -1 and 340 <= site < 360, (st, site)
+    assert st == -1 and 340 <= site < 380, (st, site)
     _ok()  # cleared
 
 
