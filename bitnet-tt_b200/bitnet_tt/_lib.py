@@ -254,6 +254,11 @@ def stream_handle(stream: torch.cuda.Stream | None = None) -> int:
     return s.cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of device `index` as a handle, without a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def last_device_status() -> tuple[int, int]:
     site = _c_int(0)
     st = load().bitnet_last_device_status(ctypes.byref(site))
@@ -534,22 +539,31 @@ def attention_prefill_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                                                  ptr(out), stream_handle()), "bitnet_attention_prefill_varlen")
 
 
-def paged_append(kv: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+# The paged cache's calls are short on the GPU (a decode step's append takes 3 us),
+# so these wrappers keep the host's share small: the caller (layers/paged_kv.py)
+# checks its tensors, the stream comes as the raw handle, and the library is
+# looked up once.  index: the device of the cache, which must be current.
+def paged_append(kv: PagedKV, index: int, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
                  qkv: torch.Tensor, n_heads: int, rope_cos: torch.Tensor, rope_sin: torch.Tensor, q_out: torch.Tensor,
                  interleaved: bool = False) -> None:
     b, max_pages = block_table.shape
     rope_len, half = rope_cos.shape
-    check(load().bitnet_paged_append(kv, ptr(block_table), b, max_pages, ptr(cu_seqlens), ptr(kv_lens), ptr(qkv),
-                                     qkv.stride(0), qkv.shape[0], n_heads, ptr(rope_cos), ptr(rope_sin), rope_len,
-                                     2 * half, rope_cos.dtype == torch.float32, interleaved, ptr(q_out),
-                                     stream_handle()), "bitnet_paged_append")
+    st = (_lib or load()).bitnet_paged_append(
+        kv, block_table.data_ptr(), b, max_pages, cu_seqlens.data_ptr(), kv_lens.data_ptr(), qkv.data_ptr(),
+        qkv.stride(0), qkv.shape[0], n_heads, rope_cos.data_ptr(), rope_sin.data_ptr(), rope_len, 2 * half,
+        rope_cos.dtype is torch.float32, interleaved, q_out.data_ptr(), raw_stream(index))
+    if st:
+        check(st, "bitnet_paged_append")
 
 
-def paged_read(kv: PagedKV, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor,
+def paged_read(kv: PagedKV, index: int, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor,
                k_out: torch.Tensor, v_out: torch.Tensor) -> None:
     b, max_pages = block_table.shape
-    check(load().bitnet_paged_read(kv, ptr(block_table), b, max_pages, ptr(starts), ptr(cu_rows), k_out.shape[0],
-                                   ptr(k_out), ptr(v_out), stream_handle()), "bitnet_paged_read")
+    st = (_lib or load()).bitnet_paged_read(
+        kv, block_table.data_ptr(), b, max_pages, None if starts is None else starts.data_ptr(), cu_rows.data_ptr(),
+        k_out.shape[0], k_out.data_ptr(), v_out.data_ptr(), raw_stream(index))
+    if st:
+        check(st, "bitnet_paged_read")
 
 
 def paged_attention_workspace_bytes(b: int, total_tokens: int, max_seqlen: int, max_kv_len: int, n_heads: int,
@@ -558,12 +572,13 @@ def paged_attention_workspace_bytes(b: int, total_tokens: int, max_seqlen: int, 
                                                              head_dim))
 
 
-def paged_attention(kv: PagedKV, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
+def paged_attention(kv: PagedKV, index: int, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
                     q: torch.Tensor, max_seqlen: int, max_kv_len: int, n_heads: int, scale: float,
                     workspace: torch.Tensor | None, out: torch.Tensor) -> None:
     b, max_pages = block_table.shape
-    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    check(load().bitnet_paged_attention(kv, ptr(block_table), b, max_pages, ptr(cu_seqlens), ptr(kv_lens), ptr(q),
-                                        q.stride(0), q.shape[0], max_seqlen, max_kv_len, n_heads, scale,
-                                        ptr(workspace), ws_bytes, ptr(out), stream_handle()),
-          "bitnet_paged_attention")
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
+    st = (_lib or load()).bitnet_paged_attention(
+        kv, block_table.data_ptr(), b, max_pages, cu_seqlens.data_ptr(), kv_lens.data_ptr(), q.data_ptr(), q.stride(0),
+        q.shape[0], max_seqlen, max_kv_len, n_heads, scale, ws, ws_bytes, out.data_ptr(), raw_stream(index))
+    if st:
+        check(st, "bitnet_paged_attention")

@@ -19,6 +19,8 @@ lengths live on the device, where a bad one is recorded
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -70,6 +72,7 @@ class PagedKVCache:
         self.key_pages, self.value_pages, self.key_scale, self.value_scale = k, v, ks, vs
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         self.device = k.device
+        self._index = k.get_device()
         self.dtype = k.dtype
         self._kv = _lib.PagedKV(_lib.ptr(k), _lib.ptr(v), _lib.ptr(ks), _lib.ptr(vs), *k.shape[0:1], k.shape[2],
                                 k.shape[1], k.shape[3], _lib.KV_INT8 if k.dtype == torch.int8 else _lib.KV_BF16)
@@ -79,29 +82,45 @@ class PagedKVCache:
         return sum(t.numel() * t.element_size() for t in ts)
 
     # ---- checks ------------------------------------------------------------
-    def _index(self, t: torch.Tensor, name: str, n: int | None = None) -> None:
-        if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 tensor on {self.device}")
-        if n is not None and (t.dim() != 1 or t.shape[0] != n):
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
+    # Each call tests everything in one expression; what is wrong is found out
+    # only when something is.
+    def _index_ok(self, t: torch.Tensor) -> bool:
+        return t.dtype is torch.int32 and t.get_device() == self._index and t.is_contiguous()
 
-    def _table(self, block_table: torch.Tensor, cu: torch.Tensor) -> int:
-        self._index(block_table, "block_table")
-        if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+    def _rows_ok(self, t: torch.Tensor) -> bool:
+        return t.dtype is torch.bfloat16 and t.get_device() == self._index and t.dim() == 2 and t.stride(1) == 1
+
+    def _refuse_index(self, block_table: torch.Tensor, **vectors: torch.Tensor) -> None:
+        for name, t in {"block_table": block_table, **vectors}.items():
+            if not self._index_ok(t):
+                raise ValueError(f"{name} must be a contiguous int32 tensor on {self.device}")
+        if block_table.dim() != 2 or min(block_table.shape) < 1:
             raise ValueError("block_table must be [sequences, pages]")
-        self._index(cu, "row offsets", block_table.shape[0] + 1)
-        return block_table.shape[0]
+        shapes = ", ".join(f"{n} {tuple(t.shape)}" for n, t in vectors.items())
+        raise ValueError(f"{shapes} do not belong to a block_table of {block_table.shape[0]} sequences")
 
-    def _rows(self, t: torch.Tensor, name: str) -> None:
-        if t.dtype != torch.bfloat16 or t.device != self.device or t.dim() != 2 or t.stride(1) != 1:
-            raise ValueError(f"{name} must be bfloat16 rows [tokens, features] on {self.device}")
+    def _heads(self, features: int, shared: int, name: str) -> int:
+        heads, rest = divmod(features, self.head_dim)
+        heads -= shared
+        if rest or heads < 1 or heads % self.num_kv_heads:
+            raise ValueError(f"{name} of {features} features does not hold heads of {self.head_dim} for "
+                             f"{self.num_kv_heads} KV heads")
+        return heads
 
     def _out(self, t: torch.Tensor | None, shape: tuple, name: str) -> torch.Tensor:
         if t is None:
             return torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        if t.dtype != torch.bfloat16 or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+        if t.dtype is not torch.bfloat16 or t.get_device() != self._index or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous bfloat16 {shape} on {self.device}")
         return t
+
+    def _launch(self, call, *args) -> None:
+        """call(*args) with the cache's device current."""
+        if torch._C._cuda_getDevice() == self._index:
+            call(self._kv, self._index, *args)
+        else:
+            with torch.cuda.device(self._index):
+                call(self._kv, self._index, *args)
 
     # ---- calls -------------------------------------------------------------
     def append(self, qkv: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
@@ -112,23 +131,21 @@ class PagedKVCache:
         pages and returns the queries [tokens, n_heads * head_dim].  Token i of n
         stands at position kv_lens[b] - n + i.  rope tables: bf16 or fp32 [positions,
         rotary_dim / 2]; rotary_dim may be less than head_dim."""
-        b = self._table(block_table, cu_seqlens)
-        self._index(kv_lens, "kv_lens", b)
-        self._rows(qkv, "qkv")
-        d = self.head_dim
-        heads, rest = divmod(qkv.shape[1], d)
-        heads -= 2 * self.num_kv_heads
-        if rest or heads < 1 or heads % self.num_kv_heads:
-            raise ValueError(f"qkv of {qkv.shape[1]} features does not hold q, k and v heads of {d} for "
-                             f"{self.num_kv_heads} KV heads")
-        for t in (rope_cos, rope_sin):
-            if (t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != rope_cos.dtype or t.dim() != 2
-                    or t.shape != rope_cos.shape or t.device != self.device or not t.is_contiguous()):
-                raise ValueError("rope tables must be two equal contiguous bf16 or fp32 [positions, rotary_dim / 2]")
-        q_out = self._out(q_out, (qkv.shape[0], heads * d), "q_out")
-        with torch.cuda.device(self.device):
-            _lib.paged_append(self._kv, block_table, cu_seqlens, kv_lens, qkv, heads, rope_cos, rope_sin, q_out,
-                              interleaved)
+        n = kv_lens.numel()
+        if not (self._index_ok(block_table) and self._index_ok(cu_seqlens) and self._index_ok(kv_lens)
+                and block_table.dim() == 2 and block_table.shape[0] == n and cu_seqlens.numel() == n + 1 and n):
+            self._refuse_index(block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens)
+        if not self._rows_ok(qkv):
+            raise ValueError(f"qkv must be bfloat16 rows [tokens, features] on {self.device}")
+        tokens, features = qkv.shape
+        heads = self._heads(features, 2 * self.num_kv_heads, "qkv")
+        tab = rope_cos.dtype
+        if not ((tab is torch.float32 or tab is torch.bfloat16) and rope_sin.dtype is tab and rope_cos.dim() == 2
+                and rope_cos.shape == rope_sin.shape and rope_cos.get_device() == self._index
+                and rope_sin.get_device() == self._index and rope_cos.is_contiguous() and rope_sin.is_contiguous()):
+            raise ValueError("rope tables must be two equal contiguous bf16 or fp32 [positions, rotary_dim / 2]")
+        q_out = self._out(q_out, (tokens, heads * self.head_dim), "q_out")
+        self._launch(_lib.paged_append, block_table, cu_seqlens, kv_lens, qkv, heads, rope_cos, rope_sin, q_out, interleaved)
         return q_out
 
     def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
@@ -139,29 +156,29 @@ class PagedKVCache:
         bound the new tokens and the keys of every sequence.  scale: 1 /
         sqrt(head_dim) by default.  workspace (attention_workspace): taken from the
         allocator if not given."""
-        b = self._table(block_table, cu_seqlens)
-        self._index(kv_lens, "kv_lens", b)
-        self._rows(q, "q")
-        d = self.head_dim
-        heads, rest = divmod(q.shape[1], d)
-        if rest or heads < 1 or heads % self.num_kv_heads:
-            raise ValueError(f"q of {q.shape[1]} features does not hold heads of {d} for {self.num_kv_heads} KV heads")
-        out = self._out(out, (q.shape[0], heads * d), "out")
-        with torch.cuda.device(self.device):
-            if workspace is None:
-                workspace = self.attention_workspace(b, q.shape[0], max_seqlen, max_kv_len, heads)
-            elif workspace.device != self.device or not workspace.is_contiguous():
-                raise ValueError(f"workspace must be a contiguous tensor on {self.device}")
-            _lib.paged_attention(self._kv, block_table, cu_seqlens, kv_lens, q, max_seqlen, max_kv_len, heads,
-                                 d ** -0.5 if scale is None else scale, workspace, out)
+        n = kv_lens.numel()
+        if not (self._index_ok(block_table) and self._index_ok(cu_seqlens) and self._index_ok(kv_lens)
+                and block_table.dim() == 2 and block_table.shape[0] == n and cu_seqlens.numel() == n + 1 and n):
+            self._refuse_index(block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens)
+        if not self._rows_ok(q):
+            raise ValueError(f"q must be bfloat16 rows [tokens, features] on {self.device}")
+        tokens, features = q.shape
+        heads = self._heads(features, 0, "q")
+        out = self._out(out, (tokens, features), "out")
+        if workspace is None:
+            workspace = self.attention_workspace(n, tokens, max_seqlen, max_kv_len, heads)
+        elif workspace.get_device() != self._index or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {self.device}")
+        self._launch(_lib.paged_attention, block_table, cu_seqlens, kv_lens, q, max_seqlen, max_kv_len, heads,
+                     self.head_dim ** -0.5 if scale is None else scale, workspace, out)
         return out
 
     def attention_workspace(self, batch: int, total_tokens: int, max_seqlen: int, max_kv_len: int,
                             num_heads: int) -> torch.Tensor | None:
         """Workspace of attend() for these bounds (None when it needs none).  Calls
         that may overlap need one each."""
-        n = _lib.paged_attention_workspace_bytes(batch, total_tokens, max_seqlen, max_kv_len, num_heads,
-                                                 self.num_kv_heads, self.head_dim)
+        n = _workspace_bytes(self._index, batch, total_tokens, max_seqlen, max_kv_len, num_heads, self.num_kv_heads,
+                             self.head_dim)
         return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
 
     def read(self, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor, total_rows: int,
@@ -169,13 +186,20 @@ class PagedKVCache:
         """Rows starts[b] .. starts[b] + cu_rows[b + 1] - cu_rows[b] - 1 of every
         sequence (starts None: from row 0) as packed bf16 keys and values
         [total_rows, n_kv, head_dim]."""
-        b = self._table(block_table, cu_rows)
-        if starts is not None:
-            self._index(starts, "starts", b)
+        n = cu_rows.numel() - 1
+        if not (self._index_ok(block_table) and self._index_ok(cu_rows) and block_table.dim() == 2
+                and block_table.shape[0] == n and n
+                and (starts is None or (self._index_ok(starts) and starts.numel() == n))):
+            self._refuse_index(block_table, cu_rows=cu_rows, **({} if starts is None else {"starts": starts}))
         if total_rows < 0:
             raise ValueError("total_rows is negative")
         shape = (total_rows, self.num_kv_heads, self.head_dim)
         k_out, v_out = self._out(k_out, shape, "k_out"), self._out(v_out, shape, "v_out")
-        with torch.cuda.device(self.device):
-            _lib.paged_read(self._kv, block_table, starts, cu_rows, k_out, v_out)
+        self._launch(_lib.paged_read, block_table, starts, cu_rows, k_out, v_out)
         return k_out, v_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(index: int, *sizes: int) -> int:
+    with torch.cuda.device(index):
+        return _lib.paged_attention_workspace_bytes(*sizes)
