@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 #include <climits>
+#include <cstdlib>
 
 #include "act_quant.cuh"
 #include "attention.cuh"
@@ -179,7 +180,7 @@ int to_dev_segments(const bitnet_segments_t* s, int N, int epilogue, bitnet_segm
 }
 
 std::atomic<unsigned long long> g_smem_aq{0}, g_smem_aq_stage{0}, g_smem_simt[3][4], g_smem_tc[3], g_smem_lmh{0}, g_smem_att[4],
-    g_smem_apf{0}, g_smem_pra[4], g_smem_pch[4];
+    g_smem_apf{0}, g_smem_pra[8], g_smem_pch[4];
 
 int lm_head_tile_T(int B) { return round_up(B, 16); }
 size_t lm_head_part_bytes(int B, int grid) { return (size_t)grid * B * sizeof(ArgPair); }
@@ -1176,22 +1177,28 @@ struct PagedCut {
   int blocks, nsplit, span;
   size_t ml, o;  // offsets in the workspace
 };
+constexpr int PAGED_ROWS_MOST = 32;
 struct PagedPlan {
   PagedCut rows, chunk;
-  int small;
+  int r, most, per;  // rows kernel: rows of a block (8 or 16), of its longest sequence, blocks of that
+  int small;  // sequences of up to this many rows are not the chunk kernel's
   size_t bytes;
 };
 
-// Parts of the keys for `pairs` blocks of work on `slots` CTAs at once: the s
-// with the least waves x (keys of a part + unit), `unit` the fixed cost of a
-// part in keys.  Only the s that just fill 1 .. 4 waves can be best.
-int paged_splits(long long pairs, int max_kv, int slots, int unit, int min_span) {
-  const long long smax = std::max(1, (max_kv + min_span - 1) / min_span);
-  long long best_s = 1, best = LLONG_MAX;
-  for (int w = 1; w <= 4; ++w) {
-    const long long s = std::min(smax, std::max(1LL, (long long)slots * w / pairs));
-    const long long cost = ((pairs * s + slots - 1) / slots) * ((max_kv + s - 1) / s + unit);
-    if (cost < best) best = cost, best_s = s;
+// Parts of the keys for `pairs` blocks of work on `slots` CTAs at once: the s of
+// the least modelled time, in keys of one CTA.  A part costs its keys plus `unit`
+// (prologue, partial results), joining parts costs `join`.  While all parts run at
+// once the longest counts; beyond that the sum over the slots, and half a part
+// for the uneven end (contexts differ).
+int paged_splits(long long pairs, int max_kv, int slots, int unit, int join, int min_span) {
+  const long long smax = std::max(1, (max_kv + min_span - 1) / min_span), fill = std::max(1LL, slots / pairs);
+  long long best_s = 1;
+  double best = 1e300;
+  for (int c = 1; c <= 9; ++c) {
+    const long long s = std::min(smax, c <= 8 ? (long long)c : fill);
+    const double part = (double)max_kv / s + unit;
+    const double t = (pairs * s <= slots ? part : pairs * s * part / slots + part / 2) + (s > 1 ? join : 0);
+    if (t < best) best = t, best_s = s;
   }
   return (int)best_s;
 }
@@ -1200,23 +1207,30 @@ PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, 
   PagedPlan pl;
   memset(&pl, 0, sizeof(pl));
   size_t at = 0;
-  auto cut = [&](PagedCut& c, long long blocks, int R, int slots, int unit, int min_span, int round) {
+  auto cut = [&](PagedCut& c, long long blocks, int R, int slots, int unit, int join, int min_span, int round) {
     c.blocks = (int)std::min(blocks, (long long)INT_MAX);
-    c.nsplit = paged_splits((long long)c.blocks * n_kv, max_kv, slots, unit, min_span);
+    c.nsplit = paged_splits((long long)c.blocks * n_kv, max_kv, slots, unit, join, min_span);
+    if (R <= 16 && getenv("XS")) c.nsplit = atoi(getenv("XS"));
+    if (R == PCH_R && getenv("XC")) c.nsplit = atoi(getenv("XC"));
     c.span = round_up(std::max(1, (max_kv + c.nsplit - 1) / c.nsplit), round);
     const size_t rows = c.nsplit > 1 ? (size_t)c.nsplit * c.blocks * n_kv * R : 0;
     c.ml = at;
     c.o = c.ml + rows * sizeof(float2);
     at = c.o + rows * D * sizeof(float);
   };
-  const bool chunks = (long long)max_q * G > PRA_R;
+  const long long rows = (long long)max_q * G;
+  const int most_rows = getenv("XM") ? atoi(getenv("XM")) : PAGED_ROWS_MOST;
+  const bool chunks = rows > most_rows;
+  pl.r = (chunks ? G : rows) > 8 ? 16 : 8;
+  pl.most = chunks ? pl.r : (int)std::max(1LL, rows);
+  pl.per = (pl.most + pl.r - 1) / pl.r;
   // Where most sequences may be as long as the longest, the chunk kernel takes the
   // short ones along: a launch for none or few of them costs more than they do.
-  pl.small = chunks && (long long)tokens * 2 < (long long)B * max_q ? PRA_R : 0;
-  if (!chunks || pl.small) cut(pl.rows, B, PRA_R, sms * 3, ATT_UNIT_COST, ATT_MIN_SPLIT, PRA_TILE);
+  pl.small = chunks && (long long)tokens * 2 < (long long)B * max_q ? pl.r : 0;
+  if (!chunks || pl.small) cut(pl.rows, (long long)B * pl.per, pl.r, sms * 3, 128, 200, 128, 32);
   if (chunks)
     cut(pl.chunk, ((long long)tokens * G + PCH_R - 1) / PCH_R + std::min((long long)B, (long long)tokens), PCH_R, sms,
-        256, 512, PCH_KB);
+        512, 256, 512, PCH_KB);
   pl.bytes = at;
   return pl;
 }
@@ -1270,17 +1284,28 @@ void paged_apply(PagedAttnParams* p, const PagedCut& c, void* workspace) {
   p->part_o = (float*)((uint8_t*)workspace + c.o);
 }
 
-template <int D, int R>
+template <int D, int R, int W>
 int launch_paged_join(const PagedAttnParams& p, bitnet_stream_t st) {
   if (p.nsplit == 1) return BITNET_OK;
-  const int rows = (int)std::min((long long)R, (long long)p.max_q * p.G);
-  return launch(paged_join_kernel<D, R>, dim3(p.blocks, p.kv.n_kv, (rows + 3) / 4), dim3(128), 0, st, 1, p);
+  const int rows = (int)std::min((long long)R, (long long)p.max_q * p.G), per = 4 / W;
+  return launch(paged_join_kernel<D, R, W>, dim3(p.blocks, p.kv.n_kv, (rows + per - 1) / per), dim3(128), 0, st, 1, p);
+}
+
+template <int D, bool I8, int H>
+int launch_paged_rows(PagedAttnParams p, bitnet_stream_t st) {
+  using S = PraShape<D, I8, H>;
+  auto k = paged_rows_kernel<D, I8, H>;
+  if (int e = ensure_smem(k, &g_smem_pra[((D == 128) * 2 + I8) * 2 + H - 1])) return e;
+  if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(PRA_THREADS), S::SMEM, st, 1, p)) return e;
+  return launch_paged_join<D, S::R, 4>(p, st);
 }
 
 template <int D, bool I8>
 int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspace, bitnet_stream_t st) {
   constexpr int idx = (D == 128) * 2 + I8;
   p.small = pl.small;
+  p.most = pl.most;
+  p.per = pl.per;
   if (pl.chunk.blocks > 0) {
     using S = PchShape<D, I8>;
     auto k = paged_chunk_kernel<D, I8>;
@@ -1302,14 +1327,11 @@ int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspa
     }
     paged_apply(&p, pl.chunk, workspace);
     if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(S::THREADS), S::SMEM, st, 1, p, mk, mv)) return e;
-    if (int e = launch_paged_join<D, PCH_R>(p, st)) return e;
+    if (int e = launch_paged_join<D, PCH_R, 1>(p, st)) return e;
   }
   if (pl.rows.blocks > 0) {
-    auto k = paged_rows_kernel<D, I8>;
-    if (int e = ensure_smem(k, &g_smem_pra[idx])) return e;
     paged_apply(&p, pl.rows, workspace);
-    if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(PRA_THREADS), PraShape<D, I8>::SMEM, st, 1, p)) return e;
-    if (int e = launch_paged_join<D, PRA_R>(p, st)) return e;
+    return pl.r == 8 ? launch_paged_rows<D, I8, 1>(p, st) : launch_paged_rows<D, I8, 2>(p, st);
   }
   return BITNET_OK;
 }

@@ -8,9 +8,11 @@
 //
 // The G = n_heads / n_kv query heads of a KV head share its keys, so a block of
 // work is a run of packed rows of one (sequence, KV head): row r is token r / G,
-// head g G + r % G.  Sequences of up to 16 rows (decode, a few drafted tokens) go to
-// paged_rows_kernel here, longer ones to paged_chunk_kernel (paged_chunk.cuh).
+// head g G + r % G.  Sequences of up to 8 or 16 rows (decode, a few drafted tokens) go
+// to paged_rows_kernel here, longer ones to paged_chunk_kernel (paged_chunk.cuh).
 #pragma once
+#include <climits>
+
 #include "attention.cuh"
 #include "common.cuh"
 #include "paged_kv.cuh"
@@ -28,6 +30,7 @@ struct PagedAttnParams {
   int nsplit, span;    // the keys are cut into nsplit parts of span keys
   int blocks;          // grid.x: row blocks, an upper bound
   int small;           // chunk kernel: sequences of up to this many rows are not its own
+  int most, per;       // rows kernel: rows of its longest sequences, and blocks of each
   float2* part_ml;     // [nsplit][blocks][n_kv][R] (maximum, sum)
   float* part_o;       // [nsplit][blocks][n_kv][R][D], unnormalised
   uint16_t* out;       // [tokens][n_heads * D]
@@ -60,12 +63,15 @@ __device__ __forceinline__ bool paged_block_of(const PagedAttnParams& p, int b, 
   return true;
 }
 
-// Sequences of up to R rows: block b is sequence b; the others are not this
-// kernel's.
+// Blocks of sequences of up to p.most rows, p.per blocks a sequence; the others
+// are not this kernel's.
 template <int R>
-__device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int b, int lane, PagedBlock& o) {
-  if ((long long)(p.cu[b + 1] - p.cu[b]) * p.G > R && p.max_q * p.G > R) return false;
-  return paged_block_of<R>(p, b, 0, lane, o);
+__device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
+  const int b = bx / p.per, row0 = (bx - b * p.per) * R;
+  const long long rows = (long long)(p.cu[b + 1] - p.cu[b]) * p.G;
+  if (rows > p.most && (long long)p.max_q * p.G > p.most) return false;
+  if (row0 > 0 && row0 >= rows) return false;
+  return paged_block_of<R>(p, b, row0, lane, o);
 }
 
 // Block bx of the R-row blocks of all sequences of more than p.small rows, in
@@ -97,34 +103,47 @@ __device__ __forceinline__ int paged_parts(const PagedAttnParams& p, int kend) {
 }
 
 // ---------------------------------------------------------------------------
-// up to 16 rows: mma.sync
+// up to 8 or 16 rows: mma.sync
 // ---------------------------------------------------------------------------
-// A CTA of 4 warps takes 16 rows of one (sequence, KV head) over one part of
-// the keys; warp w the 16-key tiles w, w + 4, ...  A tile lies in one page.  Its
-// K and V rows come by 16-byte cp.async into buffers of the warp's own, 16 KB in
-// flight a warp, so no barrier is needed inside the loop.  S = Q K^T and
-// O += P V run on m16n8k16 with fp32 sums; P enters as a bf16 pair hi + lo.
+// A CTA of 4 warps takes up to 8 H rows of one (sequence, KV head) over one part of
+// the keys; warp w the tiles w, w + 4, ... of 16 keys (int8: 32).  K
+// and V rows come by 16-byte cp.async into buffers of the warp's own, 16 KB in
+// flight a warp, so no barrier is needed inside the loop.  Products run on
+// m16n8k16 with fp32 sums: S = Q K^T, then for H = 1 (8 rows) O^T += V^T P^T, whose
+// output columns are the 8 rows, for H = 2 O += P V.  As in paged_chunk.cuh the
+// maximum is lazy: O and the sums are rescaled when it grew by more than 2^8.
+// bf16 caches: P enters as a bf16 pair hi + lo (16 significant bits).
 //
-// int8: codes become bf16 exactly in registers.  For the byte u of a code,
-// bf16 128 + (u & 127) and 128 + (u & 128) are both bit patterns
-// (0x4300 | bits), and their difference is the code: three instructions for two
-// codes.  The order of dims (S) and of output columns (O) is permuted so that
-// each thread's bytes are what its fragments need.  The keys' scales multiply
-// the scores, the values' scales the probabilities.
-constexpr int PRA_R = 16;
-constexpr int PRA_TILE = 16;
+// int8: the kernel would be bound by the integer pipe, which turns codes into
+// 16-bit floats, so it works in f16, where that costs three operations for four
+// codes: (w & 0x00FF00FF) ^ 0x64806480 holds 1152 + code twice, and subtracting
+// 1152 is exact (and runs elsewhere).  The bf16 form cost five and two; 256
+// ragged sequences of up to 4K keys took 256 us with it.
+//  * Q in f16: scaled by a power of two per row so that its largest value is
+//    2^13 .. 2^14, which keeps every bit of elements down to 2^-27 of it.
+//  * P in f16, 11 significant bits.  The values' scales vs_j can differ by any
+//    factor, so the weights p_j vs_j have a running maximum of their own: they are
+//    exp2(x_j + log2 vs_j - mv + 7) next to the sum's exp2(x_j - m).  With the 7
+//    the largest weight lies in 2^7 .. 2^15, and the step of the smallest f16, 2^-24,
+//    is below 2^-31 of it.
+//  * Dims of S and output columns of O are permuted so that each thread's bytes
+//    are what its fragments need.
 constexpr int PRA_WARPS = 4;
 constexpr int PRA_THREADS = PRA_WARPS * 32;
+constexpr float PRA_GROWTH = 8.f;
+constexpr float PRA_LIFT = 7.f;
 
-template <int D, bool I8>
+template <int D, bool I8, int H>
 struct PraShape {
+  static constexpr int R = 8 * H;                        // rows
+  static constexpr int KT = I8 ? 32 : 16;                // keys of a tile
   static constexpr int ROW = D * (I8 ? 1 : 2);           // bytes of a row
   static constexpr int CPR = ROW / 16;                   // 16-byte chunks of a row
-  static constexpr int HALF = PRA_TILE * ROW;            // K (or V) of a tile
-  static constexpr int BUF = 2 * HALF + (I8 ? 128 : 0);  // + 16 key and 16 value scales
+  static constexpr int HALF = KT * ROW;                  // K (or V) of a tile
+  static constexpr int BUF = 2 * HALF + (I8 ? 256 : 0);  // + 32 key and 32 value scales
   static constexpr int NBUF = 8192 / HALF;
   static constexpr int SMEM_TILES = PRA_WARPS * NBUF * BUF;
-  static constexpr int SMEM_MERGE = PRA_WARPS * PRA_R * (D + 2) * 4;
+  static constexpr int SMEM_MERGE = PRA_WARPS * R * (D + 2) * 4;
   static constexpr int SMEM = SMEM_TILES > SMEM_MERGE ? SMEM_TILES : SMEM_MERGE;
 };
 
@@ -138,14 +157,43 @@ __device__ __forceinline__ uint32_t pra_off(int r, int c) {
   return (uint32_t)(r * CPR * 16 + ((c ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// the codes in bytes 0 and 2 of w as an f16 pair
+__device__ __forceinline__ uint32_t codes_f2(uint32_t w) {
   uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"((w & 0x00FF00FFu) ^ 0x64806480u), "r"(0x64806480u));
   return d;
 }
-// the codes in bytes 0 and 2 of w as a bf16 pair
-__device__ __forceinline__ uint32_t codes_bf2(uint32_t w) {
-  return bf2_sub((w & 0x007F007Fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u);
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  if (F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async4_zfill(uint32_t dst, const void* src, uint32_t src_bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
@@ -160,30 +208,40 @@ __device__ __forceinline__ void split_bf2(float a, float b, uint32_t& hi, uint32
   hi = bf2_of(a, b);
   lo = bf2_of(__fsub_rn(a, __uint_as_float(hi << 16)), __fsub_rn(b, __uint_as_float(hi & 0xFFFF0000u)));
 }
+// The maximum of a running softmax after one more tile, and the factor that
+// what was summed under the old one takes (1 while it stays).
+__device__ __forceinline__ float pra_grow(float& m, float top) {
+  const float mn = fmaxf(m, top);
+  const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
+  m = mn;
+  return f;
+}
 
-template <int D, bool I8>
+template <int D, bool I8, int H>
 __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedAttnParams p) {
-  using S = PraShape<D, I8>;
+  using S = PraShape<D, I8, H>;
+  constexpr int KT = S::KT, NT = KT / 8;  // n-tiles of 8 keys
   extern __shared__ __align__(128) uint8_t smem_pra[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   pdl_wait();
   PagedBlock blk;
-  if (!paged_block_direct<PRA_R>(p, blockIdx.x, lane, blk)) return;
+  if (!paged_block_direct<S::R>(p, blockIdx.x, lane, blk)) return;
   const int g = blockIdx.y, sp = blockIdx.z;
   const int nparts = paged_parts(p, blk.kend);
   if (sp >= nparts) return;
   const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);  // this part's keys
-  const int ntiles = max(0, (k1 - k0 + PRA_TILE - 1) / PRA_TILE);
+  const int ntiles = max(0, (k1 - k0 + KT - 1) / KT);
   const int ntw = ntiles > warp ? (ntiles - warp + PRA_WARPS - 1) / PRA_WARPS : 0;
   const uint32_t buf0 = smem_u32(smem_pra) + warp * S::NBUF * S::BUF;
   const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
   const int slot_mask = (1 << p.kv.page_shift) - 1;
 
-  int pages = -1;  // lane l: the page of this warp's tile (i / 32) * 32 + l
+  constexpr int HT = KT / 16;  // 16-key pieces of a tile: each lies in one page
+  int pages = -1;              // lane l: the page of piece l % HT of this warp's tile (i / (32 / HT)) * (32 / HT) + l / HT
   auto issue = [&](int i) {
-    if ((i & 31) == 0) {
-      const int t0 = k0 + (warp + (i + lane) * PRA_WARPS) * PRA_TILE;
+    if (i % (32 / HT) == 0) {
+      const int t0 = k0 + (warp + (i + lane / HT) * PRA_WARPS) * KT + (lane % HT) * 16;
       pages = -1;
       if (t0 < k1) {
         pages = table[t0 >> p.kv.page_shift];
@@ -193,24 +251,40 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
         }
       }
     }
-    const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-    const int t0 = k0 + (warp + i * PRA_WARPS) * PRA_TILE;
-    const int nk = page < 0 ? 0 : min(PRA_TILE, k1 - t0);
-    const size_t row0 = paged_row(p.kv, max(page, 0), g, t0 & slot_mask);
+    const int t0 = k0 + (warp + i * PRA_WARPS) * KT;
     const uint32_t base = buf0 + (i % S::NBUF) * S::BUF;
 #pragma unroll
-    for (int k = 0; k < S::CPR; ++k) {
-      const int x = lane + 32 * k;
-      const bool is_v = x >= PRA_TILE * S::CPR;
-      const int row = (x / S::CPR) % PRA_TILE, c = x % S::CPR;
-      const uint8_t* src = (is_v ? p.kv.v : p.kv.k) + (row0 + (row < nk ? row : 0)) * S::ROW + c * 16;
-      const uint32_t off = is_v ? S::HALF + pra_off<S::CPR, false>(row, c) : pra_off<S::CPR, I8>(row, c);
-      cp_async16_zfill(base + off, src, row < nk ? 16u : 0u);
-    }
-    if (I8) {
-      const int row = lane & 15;
-      const float* src = (lane < 16 ? p.kv.ks : p.kv.vs) + row0 + (row < nk ? row : 0);
-      cp_async4_zfill(base + 2 * S::HALF + lane * 4, src, row < nk ? 4u : 0u);
+    for (int ht = 0; ht < HT; ++ht) {
+      const int page = __shfl_sync(0xffffffffu, pages, (i % (32 / HT)) * HT + ht);
+      const int nk = page < 0 ? 0 : k1 - t0 - 16 * ht;  // live rows, 16 or more: all
+      const size_t row0 = paged_row(p.kv, max(page, 0), g, (t0 + 16 * ht) & slot_mask);
+      // chunk lane % CPR of the rows lane / CPR + k * (32 / CPR): the addresses of the
+      // copies differ by constants (the swizzle repeats every 8 rows)
+      const uint8_t* src_k = p.kv.k + row0 * S::ROW + lane * 16;
+      const uint8_t* src_v = p.kv.v + row0 * S::ROW + lane * 16;
+      constexpr int RPC = 32 / S::CPR;  // rows of one copy instruction
+#pragma unroll
+      for (int k = 0; k < S::CPR / 2; ++k) {
+        const int row = lane / S::CPR + k * RPC, c = lane % S::CPR;
+        constexpr int REP = RPC >= 8 ? 1 : 8 / RPC;
+        const int low = lane / S::CPR + (k % REP) * RPC;  // row % 8
+        const uint32_t rest = (16 * ht + (k / REP) * REP * RPC) * S::ROW;
+        const uint32_t at_k = base + pra_off<S::CPR, I8>(low, c) + rest;
+        const uint32_t at_v = base + S::HALF + pra_off<S::CPR, false>(low, c) + rest;
+        if (nk >= 16) {
+          cp_async16(at_k, src_k + k * 512);
+          cp_async16(at_v, src_v + k * 512);
+        } else {
+          const uint32_t bytes = row < nk ? 16u : 0u;
+          cp_async16_zfill(at_k, bytes ? src_k + k * 512 : p.kv.k, bytes);
+          cp_async16_zfill(at_v, bytes ? src_v + k * 512 : p.kv.v, bytes);
+        }
+      }
+      if (I8) {
+        const int row = lane & 15;
+        const float* src = (lane < 16 ? p.kv.ks : p.kv.vs) + row0 + (row < nk ? row : 0);
+        cp_async4_zfill(base + 2 * S::HALF + (lane >> 4) * 128 + (16 * ht + row) * 4, src, row < nk ? 4u : 0u);
+      }
     }
   };
 #pragma unroll
@@ -219,35 +293,59 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
     cp_async_commit();
   }
 
-  // query fragments of rows qr and qr + 8
+  // query fragments of rows qr (and qr + 8)
   const int qr = lane >> 2, qc = lane & 3;
-  uint32_t qa[D / 16][4];
-  int lim[2];  // keys that the two rows see
+  uint32_t qa[D / 16][2 * H];  // [.][h]: the first pair, [.][H + h]: the second
+  int lim[H];                  // keys that the rows see
+  float fac[H];                // scale * log2(e), for int8 with Q's power of two taken out
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < H; ++h) {
     const int r = blk.row0 + qr + 8 * h;
     const bool in = qr + 8 * h < blk.nrows;
     const int tok = r / p.G, head = g * p.G + r - tok * p.G;
-    lim[h] = in ? blk.past + tok + 1 : 0;
+    lim[h] = in ? blk.past + tok + 1 : INT_MAX;
+    fac[h] = p.scale_log2;
     const uint16_t* row = p.q + (size_t)(blk.tok0 + (in ? tok : 0)) * p.ld_q + (in ? head : 0) * D;
+    if (I8) {
+      // dims 64 (ks / 4) + 16 qc + 4 (ks % 4) + e: e = 0, 2 in the first pair, 1, 3 in the second
+      uint2 w[D / 16];
+      uint32_t top = 0;
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) {
-      if (I8) {
-        // dims 64 (ks / 4) + 16 qc + 4 (ks % 4) + e: e = 0, 2 in the first pair, 1, 3 in the second
-        uint2 w = make_uint2(0, 0);
-        if (in) w = *reinterpret_cast<const uint2*>(row + 64 * (ks / 4) + 16 * qc + 4 * (ks % 4));
-        qa[ks][h] = __byte_perm(w.x, w.y, 0x5410);
-        qa[ks][2 + h] = __byte_perm(w.x, w.y, 0x7632);
-      } else {
+      for (int ks = 0; ks < D / 16; ++ks) {
+        w[ks] = make_uint2(0, 0);
+        if (in) w[ks] = *reinterpret_cast<const uint2*>(row + 64 * (ks / 4) + 16 * qc + 4 * (ks % 4));
+        top = max(max(top, w[ks].x & 0x7fffu), (w[ks].x >> 16) & 0x7fffu);
+        top = max(max(top, w[ks].y & 0x7fffu), (w[ks].y >> 16) & 0x7fffu);
+      }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t up = 267u - max(top >> 7, 20u);  // exponent field of 2^13 / 2^floor(log2 max)
+      const float f = __uint_as_float(up << 23);
+      fac[h] *= __uint_as_float((254u - up) << 23);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const float e0 = __uint_as_float(w[ks].x << 16), e1 = __uint_as_float(w[ks].x & 0xFFFF0000u);
+        const float e2 = __uint_as_float(w[ks].y << 16), e3 = __uint_as_float(w[ks].y & 0xFFFF0000u);
+        qa[ks][h] = f16x2_of(e0 * f, e2 * f);
+        qa[ks][H + h] = f16x2_of(e1 * f, e3 * f);
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
         qa[ks][h] = in ? *reinterpret_cast<const uint32_t*>(row + 16 * ks + 2 * qc) : 0u;
-        qa[ks][2 + h] = in ? *reinterpret_cast<const uint32_t*>(row + 16 * ks + 8 + 2 * qc) : 0u;
+        qa[ks][H + h] = in ? *reinterpret_cast<const uint32_t*>(row + 16 * ks + 8 + 2 * qc) : 0u;
       }
     }
   }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[D / 8][4];
+  const int lim_lo = blk.past + blk.row0 / p.G + 1;  // the first row's: it sees the fewest
+  float m[H], l[H], mv[H];  // maximum and this lane's share of the sum; maximum of the weights (int8)
 #pragma unroll
-  for (int j = 0; j < D / 8; ++j)
+  for (int h = 0; h < H; ++h) m[h] = mv[h] = -INFINITY, l[h] = 0.f;
+  // H = 1: O^T, m-tile j = dims, columns = rows 2 qc, + 1.  H = 2: O, n-tile j = dims, rows qr, qr + 8.
+  constexpr int NO = H == 1 ? D / 16 : D / 8;
+  float o[NO][4];
+#pragma unroll
+  for (int j = 0; j < NO; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
   const int mi = lane >> 3, mr = lane & 7;
@@ -256,111 +354,177 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
     cp_async_wait<S::NBUF - 1>();
     __syncwarp();
     const uint32_t kb = buf0 + (i % S::NBUF) * S::BUF, vb = kb + S::HALF;
-    const int t0 = k0 + (warp + i * PRA_WARPS) * PRA_TILE;
-    float s[2][4];  // keys 8 n + 2 qc, + 1 of rows qr (0, 1) and qr + 8 (2, 3)
+    const int t0 = k0 + (warp + i * PRA_WARPS) * KT;
+    float s[NT][4];  // keys 8 n + 2 qc, + 1 of rows qr (0, 1) and qr + 8 (2, 3)
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+    auto qk = [&](float(&d)[4], int ks, uint32_t b0, uint32_t b1) {
+      mma_16816<I8>(d, qa[ks][0], H == 2 ? qa[ks][1] : 0u, qa[ks][H], H == 2 ? qa[ks][H + H - 1] : 0u, b0, b1);
+    };
     if (I8) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h) {
+        for (int n = 0; n < NT; ++n) {
           uint32_t w[4];
           const uint32_t a = kb + pra_off<S::CPR, true>(8 * n + qr, 4 * h + qc);
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_bf16_16816_full(s[n], qa[4 * h + k][0], qa[4 * h + k][1], qa[4 * h + k][2], qa[4 * h + k][3],
-                                codes_bf2(w[k]), codes_bf2(w[k] >> 8));
+          for (int k = 0; k < 4; ++k) qk(s[n], 4 * h + k, codes_f2(w[k]), codes_f2(w[k] >> 8));
         }
     } else {
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         uint32_t b0, b1, b2, b3;
         ldsm_x4(kb + pra_off<S::CPR, false>((mi >> 1) * 8 + mr, 2 * ks + (mi & 1)), b0, b1, b2, b3);
-        mma_bf16_16816_full(s[0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b0, b1);
-        mma_bf16_16816_full(s[1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], b2, b3);
+        qk(s[0], ks, b0, b1);
+        qk(s[1], ks, b2, b3);
       }
     }
-    float2 kscale[2], vscale[2];
-    if (I8) {
+    // scores in base 2; v: log2 of the values' scales
+    const bool masked = t0 + KT > min(lim_lo, k1);
+    float2 v[NT];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const uint32_t a = kb + 2 * S::HALF + (8 * n + 2 * qc) * 4;
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(kscale[n].x), "=f"(kscale[n].y) : "r"(a));
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(vscale[n].x), "=f"(vscale[n].y) : "r"(a + 64));
-      }
-    }
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = t0 + 8 * n + 2 * qc + (e & 1);
-        float x = s[n][e] * p.scale_log2;
-        if (I8) x *= (e & 1) ? kscale[n].y : kscale[n].x;
-        s[n][e] = key < lim[e >> 1] ? x : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[n][e]);
-      }
-    float corr[2], ref[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-      const float mn = fmaxf(m[h], mx[h]);
-      ref[h] = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet
-      corr[h] = exp2f(m[h] - ref[h]);
-      m[h] = mn;
-      l[h] *= corr[h];
-    }
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = s[n][e];
-        float w = exp2f(x - ref[e >> 1]);
-        l[e >> 1] += w;
-        // a masked key's scale may be anything
-        if (I8) w = x == -INFINITY ? 0.f : w * ((e & 1) ? vscale[n].y : vscale[n].x);
-        s[n][e] = w;
-      }
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      o[j][0] *= corr[0];
-      o[j][1] *= corr[0];
-      o[j][2] *= corr[1];
-      o[j][3] *= corr[1];
-    }
-    uint32_t ph[4], pl[4];  // (row qr, keys 2 qc), (qr + 8, 2 qc), (qr, 8 + 2 qc), (qr + 8, 8 + 2 qc)
-    split_bf2(s[0][0], s[0][1], ph[0], pl[0]);
-    split_bf2(s[0][2], s[0][3], ph[1], pl[1]);
-    split_bf2(s[1][0], s[1][1], ph[2], pl[2]);
-    split_bf2(s[1][2], s[1][3], ph[3], pl[3]);
-#pragma unroll
-    for (int jj = 0; jj < S::CPR / 2; ++jj) {
-      // transposed 8 x 8 matrices: (keys 0-7, chunk 2 jj), (keys 8-15, 2 jj), (keys 0-7, 2 jj + 1), (keys 8-15, 2 jj + 1)
-      uint32_t b0, b1, b2, b3;
-      ldsm_x4_t(vb + pra_off<S::CPR, false>((mi & 1) * 8 + mr, 2 * jj + (mi >> 1)), b0, b1, b2, b3);
+    for (int n = 0; n < NT; ++n) {
+      float2 k;
       if (I8) {
-        // a chunk holds 16 dims: its even dims are one n-tile, its odd dims the next
+        const uint32_t a = kb + 2 * S::HALF + (8 * n + 2 * qc) * 4;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(k.x), "=f"(k.y) : "r"(a));
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[n].x), "=f"(v[n].y) : "r"(a + 128));
+        v[n].x = lg2(v[n].x), v[n].y = lg2(v[n].y);
+      }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t x0 = c ? b2 : b0, x1 = c ? b3 : b1;
+      for (int e = 0; e < 2 * H; ++e) {
+        s[n][e] *= fac[e >> 1];
+        if (I8) s[n][e] *= (e & 1) ? k.y : k.x;
+      }
+    }
+    auto hidden = [&](int n, int e) { return t0 + 8 * n + 2 * qc + (e & 1) >= min(lim[e >> 1], k1); };
+    if (masked) {
 #pragma unroll
-          for (int odd = 0; odd < 2; ++odd) {
-            const uint32_t v0 = codes_bf2(odd ? x0 >> 8 : x0), v1 = codes_bf2(odd ? x1 >> 8 : x1);
-            float(&acc)[4] = o[4 * jj + 2 * c + odd];
-            mma_bf16_16816_full(acc, ph[0], ph[1], ph[2], ph[3], v0, v1);
-            mma_bf16_16816_full(acc, pl[0], pl[1], pl[2], pl[3], v0, v1);
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2 * H; ++e)
+          if (hidden(n, e)) s[n][e] = -INFINITY;
+    }
+    // int8: a hidden key's value scale may be anything, so its maximum (a NaN is passed over) only
+    // sets a reference, and its weight is cleared below
+    float top[H], topv[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      top[h] = topv[h] = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        top[h] = fmaxf(fmaxf(top[h], s[n][2 * h]), s[n][2 * h + 1]);
+        if (I8) topv[h] = fmaxf(fmaxf(topv[h], s[n][2 * h] + v[n].x), s[n][2 * h + 1] + v[n].y);
+      }
+    }
+    bool grown = false;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      grown = grown || top[h] > m[h] + PRA_GROWTH;
+      if (I8) {
+        topv[h] = fmaxf(topv[h], __shfl_xor_sync(0xffffffffu, topv[h], 1));
+        topv[h] = fmaxf(topv[h], __shfl_xor_sync(0xffffffffu, topv[h], 2));
+        grown = grown || topv[h] > mv[h] + PRA_GROWTH;
+      }
+    }
+    if (__any_sync(0xffffffffu, grown)) {
+      float f[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        f[h] = pra_grow(m[h], top[h]);
+        l[h] *= f[h];
+        if (I8) f[h] = pra_grow(mv[h], topv[h]);
+      }
+      if (H == 1) {  // the states of rows 2 qc and 2 qc + 1 are in lanes 8 qc and 8 qc + 4
+        const float lo = __shfl_sync(0xffffffffu, f[0], 8 * qc), hi = __shfl_sync(0xffffffffu, f[0], 8 * qc + 4);
+#pragma unroll
+        for (int j = 0; j < NO; ++j) o[j][0] *= lo, o[j][1] *= hi, o[j][2] *= lo, o[j][3] *= hi;
+      } else {
+#pragma unroll
+        for (int j = 0; j < NO; ++j) o[j][0] *= f[0], o[j][1] *= f[0], o[j][2] *= f[H - 1], o[j][3] *= f[H - 1];
+      }
+    }
+    float ref[H], refv[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      ref[h] = m[h] == -INFINITY ? 0.f : m[h];  // a row that has seen no key yet
+      refv[h] = mv[h] == -INFINITY ? 0.f : mv[h] - PRA_LIFT;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2 * H; ++e) {
+        const int h = e >> 1;
+        const float x = s[n][e], w = ex2(x - ref[h]);
+        l[h] += w;
+        s[n][e] = I8 ? ex2(x + ((e & 1) ? v[n].y : v[n].x) - refv[h]) : w;
+      }
+    if (I8 && masked) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2 * H; ++e)
+          if (hidden(n, e)) s[n][e] = 0.f;
+    }
+#pragma unroll
+    for (int kk = 0; kk < KT / 16; ++kk) {  // 16 keys
+      // rows qr: keys 2 qc, + 1 of the first and the second 8; then rows qr + 8
+      uint32_t ph[2 * H], pl[2 * H];
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float a = s[2 * kk + n][2 * h], b = s[2 * kk + n][2 * h + 1];
+          if (I8) ph[2 * h + n] = f16x2_of(a, b);
+          else split_bf2(a, b, ph[2 * h + n], pl[2 * h + n]);
+        }
+      // O += (rows) P V, or O^T with V^T as the left operand
+      auto pv = [&](float(&d)[4], uint32_t v0, uint32_t v1, const uint32_t(&w)[2 * H]) {
+        mma_16816<I8>(d, w[0], H == 2 ? w[H] : 0u, w[1], H == 2 ? w[H + 1] : 0u, v0, v1);
+      };
+      const int key = 16 * kk;
+      if (I8) {
+#pragma unroll
+        for (int jj = 0; jj < S::CPR / 2; ++jj) {
+          // transposed 8 x 8 pairs of bytes: (keys 0-7, chunk 2 jj), (8-15, 2 jj), (0-7, 2 jj + 1), (8-15, 2 jj + 1)
+          uint32_t x[4];
+          ldsm_x4_t(vb + pra_off<S::CPR, false>(key + (mi & 1) * 8 + mr, 2 * jj + (mi >> 1)), x[0], x[1], x[2], x[3]);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {  // a chunk holds 16 dims: even ones, odd ones
+            const uint32_t e0 = codes_f2(x[2 * c]), o0 = codes_f2(x[2 * c] >> 8);
+            const uint32_t e1 = codes_f2(x[2 * c + 1]), o1 = codes_f2(x[2 * c + 1] >> 8);
+            if (H == 1) {
+              mma_16816<I8>(o[2 * jj + c], e0, o0, e1, o1, ph[0], ph[1]);
+            } else {
+              pv(o[(4 * jj + 2 * c) % NO], e0, e1, ph);
+              pv(o[(4 * jj + 2 * c + 1) % NO], o0, o1, ph);
+            }
           }
         }
       } else {
-        mma_bf16_16816_full(o[2 * jj], ph[0], ph[1], ph[2], ph[3], b0, b1);
-        mma_bf16_16816_full(o[2 * jj + 1], ph[0], ph[1], ph[2], ph[3], b2, b3);
-        mma_bf16_16816_full(o[2 * jj], pl[0], pl[1], pl[2], pl[3], b0, b1);
-        mma_bf16_16816_full(o[2 * jj + 1], pl[0], pl[1], pl[2], pl[3], b2, b3);
+#pragma unroll
+        for (int jj = 0; jj < S::CPR / 2; ++jj) {
+          uint32_t a0, a1, a2, a3;
+          if (H == 1) {
+            // (keys 0-7, chunk 2 jj), (0-7, 2 jj + 1), (8-15, 2 jj), (8-15, 2 jj + 1)
+            ldsm_x4_t(vb + pra_off<S::CPR, false>(key + (mi >> 1) * 8 + mr, 2 * jj + (mi & 1)), a0, a1, a2, a3);
+            mma_16816<I8>(o[jj], a0, a1, a2, a3, ph[0], ph[1]);
+            mma_16816<I8>(o[jj], a0, a1, a2, a3, pl[0], pl[1]);
+          } else {
+            // (keys 0-7, chunk 2 jj), (8-15, 2 jj), (0-7, 2 jj + 1), (8-15, 2 jj + 1)
+            ldsm_x4_t(vb + pra_off<S::CPR, false>(key + (mi & 1) * 8 + mr, 2 * jj + (mi >> 1)), a0, a1, a2, a3);
+            pv(o[(2 * jj) % NO], a0, a1, ph);
+            pv(o[(2 * jj + 1) % NO], a2, a3, ph);
+            pv(o[(2 * jj) % NO], a0, a1, pl);
+            pv(o[(2 * jj + 1) % NO], a2, a3, pl);
+          }
+        }
       }
     }
     __syncwarp();
@@ -370,22 +534,39 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
   cp_async_wait<0>();
   __syncthreads();  // the tiles' memory is free
 
-  // the warps' states: [warp][row] (m, l), then [warp][row][D]
+  // the warps' states: [warp][row] (m, l), then [warp][row][D], outputs under m
   float2* sm_ml = reinterpret_cast<float2*>(smem_pra);
-  float* sm_o = reinterpret_cast<float*>(sm_ml + PRA_WARPS * PRA_R);
+  float* sm_o = reinterpret_cast<float*>(sm_ml + PRA_WARPS * S::R);
+  float fv[H];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < H; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    if (qc == 0) sm_ml[warp * PRA_R + qr + 8 * h] = make_float2(m[h], l[h]);
+    if (qc == 0) sm_ml[warp * S::R + qr + 8 * h] = make_float2(m[h], l[h]);
+    fv[h] = !I8 ? 1.f : (mv[h] == -INFINITY ? 0.f : ex2(mv[h] - PRA_LIFT - m[h]));
+  }
+  if (H == 1) {
+    const float lo = __shfl_sync(0xffffffffu, fv[0], 8 * qc), hi = __shfl_sync(0xffffffffu, fv[0], 8 * qc + 4);
+    float* d0 = sm_o + (size_t)(warp * S::R + 2 * qc) * D;
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      // int8: n-tile j holds the dims of parity j % 2 of chunk j / 2
-      const int d = I8 ? 16 * (j >> 1) + 4 * qc + (j & 1) : 8 * j + 2 * qc;
-      float* dst = sm_o + (size_t)(warp * PRA_R + qr + 8 * h) * D + d;
-      dst[0] = o[j][2 * h];
-      dst[I8 ? 2 : 1] = o[j][2 * h + 1];
+    for (int j = 0; j < NO; ++j) {
+      const int a = I8 ? 16 * j + 2 * qr : 16 * j + qr, b = I8 ? a + 1 : a + 8;
+      d0[a] = o[j][0] * lo;
+      d0[D + a] = o[j][1] * hi;
+      d0[b] = o[j][2] * lo;
+      d0[D + b] = o[j][3] * hi;
     }
+  } else {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int j = 0; j < NO; ++j) {
+        // int8: n-tile j holds the dims of parity j % 2 of chunk j / 2
+        const int d = I8 ? 16 * (j >> 1) + 4 * qc + (j & 1) : 8 * j + 2 * qc;
+        float* dst = sm_o + (size_t)(warp * S::R + qr + 8 * h) * D + d;
+        dst[0] = o[j][2 * h] * fv[h];
+        dst[I8 ? 2 : 1] = o[j][2 * h + 1] * fv[h];
+      }
   }
   __syncthreads();
   const size_t pb = ((size_t)sp * p.blocks + blockIdx.x) * p.kv.n_kv + g;
@@ -393,14 +574,14 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
     const int r = idx / (D / 4), d = (idx % (D / 4)) * 4;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < PRA_WARPS; ++w) M = fmaxf(M, sm_ml[w * PRA_R + r].x);
+    for (int w = 0; w < PRA_WARPS; ++w) M = fmaxf(M, sm_ml[w * S::R + r].x);
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
     float den = 0.f;
 #pragma unroll
     for (int w = 0; w < PRA_WARPS; ++w) {
-      const float2 ml = sm_ml[w * PRA_R + r];
-      const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-      const float4 a = *reinterpret_cast<const float4*>(sm_o + (size_t)(w * PRA_R + r) * D + d);
+      const float2 ml = sm_ml[w * S::R + r];
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      const float4 a = *reinterpret_cast<const float4*>(sm_o + (size_t)(w * S::R + r) * D + d);
       num.x = fmaf(a.x, f, num.x), num.y = fmaf(a.y, f, num.y);
       num.z = fmaf(a.z, f, num.z), num.w = fmaf(a.w, f, num.w);
       den = fmaf(ml.y, f, den);
@@ -411,8 +592,8 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
       uint16_t* dst = p.out + ((size_t)(blk.tok0 + tok) * p.n_heads + g * p.G + row - tok * p.G) * D + d;
       *reinterpret_cast<uint2*>(dst) = make_uint2(bf2_of(num.x * inv, num.y * inv), bf2_of(num.z * inv, num.w * inv));
     } else {
-      if (d == 0) p.part_ml[pb * PRA_R + r] = make_float2(M, den);
-      *reinterpret_cast<float4*>(p.part_o + (pb * PRA_R + r) * D + d) = num;
+      if (d == 0) p.part_ml[pb * S::R + r] = make_float2(M, den);
+      *reinterpret_cast<float4*>(p.part_o + (pb * S::R + r) * D + d) = num;
     }
   }
 }
@@ -420,37 +601,56 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
 // ---------------------------------------------------------------------------
 // joining the parts
 // ---------------------------------------------------------------------------
-// One warp a row: weighs the parts' unnormalised outputs by exp2(m_part - max).
-// A block whose keys fit in one part was written by its own CTA.
-template <int D, int R>
+// W warps a row, each the parts w, w + W, ...: they weigh the parts'
+// unnormalised outputs by exp2(m_part - max).  A block whose keys fit in one
+// part was written by its own CTA.  A few rows in many parts take W = 4, so that
+// the chain of loads is short; many rows in few parts W = 1.
+template <int D, int R, int W>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p) {
-  const int lane = threadIdx.x & 31, r = blockIdx.z * 4 + (threadIdx.x >> 5), g = blockIdx.y;
+  constexpr int V = D / 32;
+  __shared__ float s_num[4][D], s_den[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r = blockIdx.z * (4 / W) + warp / W, w = warp % W, g = blockIdx.y;
   pdl_trigger();
   pdl_wait();
   PagedBlock blk;
-  if (!(R == PRA_R ? paged_block_direct<R>(p, blockIdx.x, lane, blk) : paged_block_search<R>(p, blockIdx.x, lane, blk)))
+  if (!(R <= 16 ? paged_block_direct<R>(p, blockIdx.x, lane, blk) : paged_block_search<R>(p, blockIdx.x, lane, blk)))
     return;
   const int nparts = paged_parts(p, blk.kend);
-  if (nparts == 1 || r >= blk.nrows) return;
+  if (nparts == 1) return;
   const size_t step = (size_t)p.blocks * p.kv.n_kv;
   const size_t pb = (size_t)blockIdx.x * p.kv.n_kv + g;
-  float M = -INFINITY;
-  for (int s = lane; s < nparts; s += 32) M = fmaxf(M, p.part_ml[(pb + s * step) * R + r].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  constexpr int V = D / 32;
-  float num[V], den = 0.f;
+  float num[V], den = 0.f, M = -INFINITY;
 #pragma unroll
   for (int e = 0; e < V; ++e) num[e] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < nparts; ++s) {
-    const size_t at = (pb + s * step) * R + r;
-    const float2 ml = p.part_ml[at];
-    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-    den = fmaf(ml.y, f, den);
+  if (r < blk.nrows) {
+    for (int s = lane; s < nparts; s += 32) M = fmaxf(M, p.part_ml[(pb + s * step) * R + r].x);
 #pragma unroll
-    for (int e = 0; e < V; ++e) num[e] = fmaf(p.part_o[at * D + lane * V + e], f, num[e]);
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll 4
+    for (int s = w; s < nparts; s += W) {
+      const size_t at = (pb + s * step) * R + r;
+      const float2 ml = p.part_ml[at];
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+      den = fmaf(ml.y, f, den);
+#pragma unroll
+      for (int e = 0; e < V; ++e) num[e] = fmaf(p.part_o[at * D + lane * V + e], f, num[e]);
+    }
   }
+  if (W > 1) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) s_num[warp][lane * V + e] = num[e];
+    if (lane == 0) s_den[warp] = den;
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int x = 1; x < W; ++x) {
+      den += s_den[warp + x];
+#pragma unroll
+      for (int e = 0; e < V; ++e) num[e] += s_num[warp + x][lane * V + e];
+    }
+  }
+  if (r >= blk.nrows) return;
   const float inv = M == -INFINITY ? 0.f : 1.f / den;
   const int row = blk.row0 + r, tok = row / p.G;
   uint32_t* dst = reinterpret_cast<uint32_t*>(

@@ -54,6 +54,18 @@ struct PchShape {
 static_assert(256 * 208 + 128 * 88 <= 384 * 168, "register shares within the launch's");
 static_assert(256 * 176 + 128 * 56 + 128 * 104 <= 512 * 128, "register shares within the launch's");
 
+__device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// The codes in bytes 0 and 2 of w as a bf16 pair: for the byte u of a code,
+// bf16 128 + (u & 127) and 128 + (u & 128) are both bit patterns (0x4300 | bits),
+// and their difference is the code.
+__device__ __forceinline__ uint32_t codes_bf2(uint32_t w) {
+  return bf2_sub((w & 0x007F007Fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u);
+}
+
 struct PchCtrl {
   uint64_t full[PCH_MAX_SLOTS], empty[PCH_MAX_SLOTS];
   uint64_t s_full[2], p_ready[2], o_full[2], tail, drain;
@@ -115,11 +127,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;

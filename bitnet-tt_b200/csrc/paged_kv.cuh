@@ -75,9 +75,10 @@ __device__ __forceinline__ uint4 pack_bf8(const float (&x)[8]) {
 // the floor of the framework's activation quantiser.  A row with an infinity or
 // a NaN gets the scale NaN (its values read back as NaN).
 //
-// Bound: memory.  D/8 lanes take one head of one token, 16 bytes each; the
-// partner half comes by shuffle, the row's maximum by a shuffle tree, so qkv is
-// read once and every access is 16 bytes wide (8 for int8 codes).
+// Bound: memory.  D/16 lanes take one head of one token, each the two 16-byte
+// chunks that hold eight pairs (or two chunks of the dims that only move), so a
+// rotation needs no shuffle and reads each table entry once; the row's maximum
+// is a short shuffle tree.  Two heads a lane are loaded before the first is worked on.
 struct PagedAppendParams {
   PagedKV kv;
   const int32_t* cu;       // [B + 1] token offsets
@@ -95,10 +96,6 @@ struct PagedAppendParams {
 constexpr int PKV_THREADS = 256;
 
 template <bool F32>
-__device__ __forceinline__ float rope_entry(const void* t, size_t i) {
-  return F32 ? reinterpret_cast<const float*>(t)[i] : bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(t)[i]);
-}
-template <bool F32>
 __device__ __forceinline__ void rope_entries8(const void* t, size_t i, float (&x)[8]) {  // i % 8 == 0
   if (F32) {
     const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(t) + i);
@@ -109,9 +106,20 @@ __device__ __forceinline__ void rope_entries8(const void* t, size_t i, float (&x
   }
 }
 
+// The chunks (of 8 dims) that lane l of a head takes: c0 and c1 hold the pairs
+// (d, d + rot / 2) of half layouts; adjacent pairs lie within a chunk.
+__device__ __forceinline__ void append_chunks(int l, int rot, bool interleaved, int& c0, int& c1, bool& turns) {
+  const int h = rot >> 4;  // lanes that turn
+  turns = l < h;
+  c0 = turns && !interleaved ? l : 2 * l;
+  c1 = turns && !interleaved ? l + h : 2 * l + 1;
+}
+
 template <int D, bool I8, bool F32>
 __global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAppendParams p) {
-  constexpr int LPH = D / 8;  // lanes of one head
+  constexpr int LPH = D / 16;                 // lanes of one head
+  constexpr int GROUPS = PKV_THREADS / LPH;   // heads at once
+  constexpr int U = 2;                        // heads of a lane in flight
   __shared__ int s_pos[8], s_page[8];
   pdl_trigger();
   pdl_wait();
@@ -144,76 +152,87 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAp
   }
   __syncthreads();
   const int heads = p.n_heads + 2 * p.kv.n_kv, items = ntok * heads;
-  const int l = tid % LPH, d0 = l * 8;          // this lane's 8 dims
-  const int half_l = p.rot >> 4;                // lanes of half the rotated part
-  const bool in_rot = d0 < p.rot;
-  // lane (in the warp) holding the other half of the pairs
-  const int base = lane - l;
-  const int partner = base + (in_rot ? (l < half_l ? l + half_l : l - half_l) : l);
-  for (int it0 = 0; it0 < items; it0 += PKV_THREADS / LPH) {
-    const int it = it0 + tid / LPH;
-    const bool valid = it < items;
-    const int t = valid ? it / heads : 0, hh = valid ? it - t * heads : 0;
-    const int pos = s_pos[t];
-    const bool live = valid && pos >= 0;
-    float x[8];
-    {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (live) w = *reinterpret_cast<const uint4*>(p.qkv + (size_t)(tok0 + t) * p.ld_qkv + hh * D + d0);
-      unpack_bf8(w, x);
-      uint4 o;
-      o.x = __shfl_sync(0xffffffffu, w.x, partner);
-      o.y = __shfl_sync(0xffffffffu, w.y, partner);
-      o.z = __shfl_sync(0xffffffffu, w.z, partner);
-      o.w = __shfl_sync(0xffffffffu, w.w, partner);
-      if (live && in_rot && hh < p.n_heads + p.kv.n_kv) {
+  int c0, c1;
+  bool turns;
+  append_chunks(tid % LPH, p.rot, p.interleaved, c0, c1, turns);
+  for (int it0 = tid / LPH; it0 - tid / LPH < items; it0 += U * GROUPS) {
+    uint4 w0[U], w1[U];
+    int tk[U], hd[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int it = it0 + u * GROUPS;
+      const int t = it < items ? it / heads : 0;
+      hd[u] = it - t * heads;
+      tk[u] = it < items && s_pos[t] >= 0 ? t : -1;
+      w0[u] = w1[u] = make_uint4(0, 0, 0, 0);
+      if (tk[u] >= 0) {
+        const uint16_t* src = p.qkv + (size_t)(tok0 + t) * p.ld_qkv + hd[u] * D;
+        w0[u] = *reinterpret_cast<const uint4*>(src + c0 * 8);
+        w1[u] = *reinterpret_cast<const uint4*>(src + c1 * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = max(tk[u], 0), hh = hd[u], pos = s_pos[t];
+      const bool live = tk[u] >= 0, is_q = hh < p.n_heads, is_v = hh >= p.n_heads + p.kv.n_kv;
+      float x[8], y[8];
+      unpack_bf8(w0[u], x);
+      unpack_bf8(w1[u], y);
+      if (live && turns && !is_v) {
         const size_t row = (size_t)pos * (p.rot >> 1);
+        float c[8], s[8];
+        rope_entries8<F32>(p.cos, row + (tid % LPH) * 8, c);
+        rope_entries8<F32>(p.sin, row + (tid % LPH) * 8, s);
         if (p.interleaved) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float c = rope_entry<F32>(p.cos, row + (d0 >> 1) + e), s = rope_entry<F32>(p.sin, row + (d0 >> 1) + e);
-            const float a = x[2 * e], b = x[2 * e + 1];
-            x[2 * e] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-            x[2 * e + 1] = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+            const float a = x[2 * e], b = x[2 * e + 1], a2 = y[2 * e], b2 = y[2 * e + 1];
+            x[2 * e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+            x[2 * e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+            y[2 * e] = __fsub_rn(__fmul_rn(a2, c[4 + e]), __fmul_rn(b2, s[4 + e]));
+            y[2 * e + 1] = __fadd_rn(__fmul_rn(b2, c[4 + e]), __fmul_rn(a2, s[4 + e]));
           }
         } else {
-          float c[8], s[8], y[8];
-          const size_t j = row + (l < half_l ? d0 : d0 - (p.rot >> 1));
-          rope_entries8<F32>(p.cos, j, c);
-          rope_entries8<F32>(p.sin, j, s);
-          unpack_bf8(o, y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = l < half_l ? __fsub_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]))
-                              : __fadd_rn(__fmul_rn(x[e], c[e]), __fmul_rn(y[e], s[e]));
+          for (int e = 0; e < 8; ++e) {
+            const float a = x[e], b = y[e];
+            x[e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+            y[e] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+          }
         }
       }
-    }
-    const int g = hh < p.n_heads ? 0 : (hh - p.n_heads) % p.kv.n_kv;
-    const bool is_v = hh >= p.n_heads + p.kv.n_kv;
-    const size_t row = live ? paged_row(p.kv, s_page[t], g, pos & ((1 << p.kv.page_shift) - 1)) : 0;
-    if (live && hh < p.n_heads)
-      *reinterpret_cast<uint4*>(p.q_out + ((size_t)(tok0 + t) * p.n_heads + hh) * D + d0) = pack_bf8(x);
-    if (I8) {
-      uint32_t top = 0;  // the largest |x| by its bits: a NaN or an infinity wins
+      const int g = is_q ? 0 : (is_v ? hh - p.n_heads - p.kv.n_kv : hh - p.n_heads);
+      const size_t row = live ? paged_row(p.kv, s_page[t], g, pos & ((1 << p.kv.page_shift) - 1)) : 0;
+      uint8_t* pool = is_v ? p.kv.v : p.kv.k;
+      if (I8) {
+        uint32_t top = 0;  // the largest |x| by its bits: a NaN or an infinity wins
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+        for (int e = 0; e < 8; ++e)
+          top = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(y[e]) & 0x7fffffffu));
 #pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (live && hh >= p.n_heads) {
-        const bool finite = top < 0x7f800000u;
-        const float amax = fmaxf(__uint_as_float(top), 1e-5f), inv = __fdiv_rn(127.f, amax);
-        uint32_t w[2] = {0, 0};
+        for (int o = LPH / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (live && !is_q) {
+          const bool finite = top < 0x7f800000u;
+          const float amax = fmaxf(__uint_as_float(top), 1e-5f), inv = __fdiv_rn(127.f, amax);
+          uint32_t q[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int q = finite ? __float2int_rn(__fmul_rn(x[e], inv)) : 0;
-          w[e >> 2] |= (uint32_t)(q & 0xff) << (8 * (e & 3));
+          for (int e = 0; e < 8; ++e) {
+            const int a = finite ? __float2int_rn(__fmul_rn(x[e], inv)) : 0;
+            const int b = finite ? __float2int_rn(__fmul_rn(y[e], inv)) : 0;
+            q[e >> 2] |= (uint32_t)(a & 0xff) << (8 * (e & 3));
+            q[2 + (e >> 2)] |= (uint32_t)(b & 0xff) << (8 * (e & 3));
+          }
+          *reinterpret_cast<uint2*>(pool + row * D + c0 * 8) = make_uint2(q[0], q[1]);
+          *reinterpret_cast<uint2*>(pool + row * D + c1 * 8) = make_uint2(q[2], q[3]);
+          if (tid % LPH == 0)
+            (is_v ? p.kv.vs : p.kv.ks)[row] = finite ? __fdiv_rn(amax, 127.f) : __uint_as_float(0x7fc00000u);
         }
-        *reinterpret_cast<uint2*>((is_v ? p.kv.v : p.kv.k) + row * D + d0) = make_uint2(w[0], w[1]);
-        if (l == 0) (is_v ? p.kv.vs : p.kv.ks)[row] = finite ? __fdiv_rn(amax, 127.f) : __uint_as_float(0x7fc00000u);
       }
-    } else if (live && hh >= p.n_heads) {
-      *reinterpret_cast<uint4*>((is_v ? p.kv.v : p.kv.k) + (row * D + d0) * 2) = pack_bf8(x);
+      if (live && (is_q || !I8)) {
+        uint16_t* dst = is_q ? p.q_out + ((size_t)(tok0 + t) * p.n_heads + hh) * D : reinterpret_cast<uint16_t*>(pool) + row * D;
+        *reinterpret_cast<uint4*>(dst + c0 * 8) = pack_bf8(x);
+        *reinterpret_cast<uint4*>(dst + c1 * 8) = pack_bf8(y);
+      }
     }
   }
 }
@@ -223,7 +242,8 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAp
 // ---------------------------------------------------------------------------
 // Row r of sequence b's packed rows (cu[b] .. cu[b + 1] - 1) is cache row
 // starts[b] + r - cu[b]; k_out / v_out are bf16 [rows][n_kv][D].  int8: the value
-// bf16(code * scale), rounded once.  Bound: memory, one pass; D/8 lanes a row.
+// bf16(code * scale), rounded once.  Bound: memory, one pass; a lane moves 16 bytes
+// of a row, four rows' worth in flight.
 struct PagedReadParams {
   PagedKV kv;
   const int32_t* cu;
@@ -232,18 +252,20 @@ struct PagedReadParams {
   uint16_t* k_out;
   uint16_t* v_out;
 };
-constexpr int PKV_READ_ROWS = 8;
+constexpr int PKV_READ_ROWS = 16;
 
 template <int D, bool I8>
 __global__ void __launch_bounds__(PKV_THREADS) paged_read_kernel(const PagedReadParams p) {
-  constexpr int LPH = D / 8;
+  constexpr int LPH = D / (I8 ? 16 : 8);  // lanes of a row, 16 bytes each
+  constexpr int GROUPS = PKV_THREADS / LPH;
+  constexpr int U = 4;
   __shared__ int s_slot[PKV_READ_ROWS], s_page[PKV_READ_ROWS];
   pdl_trigger();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int row0 = blockIdx.x * PKV_READ_ROWS, nrow = min(PKV_READ_ROWS, p.rows - row0);
-  if (warp < nrow) {
-    const int r = row0 + warp;
+  for (int i = tid >> 5; i < nrow; i += PKV_THREADS / 32) {
+    const int r = row0 + i;
     const int b = warp_find_seq(p.cu, p.B, r, lane);
     if (lane == 0) {
       int page = -1, slot = 0;
@@ -261,30 +283,46 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_read_kernel(const PagedRead
           }
         }
       }
-      s_page[warp] = page;
-      s_slot[warp] = slot;
+      s_page[i] = page;
+      s_slot[i] = slot;
     }
   }
   __syncthreads();
   const int per_row = 2 * p.kv.n_kv, items = nrow * per_row;
-  const int d0 = (tid % LPH) * 8;
-  for (int it = tid / LPH; it < items; it += PKV_THREADS / LPH) {
-    const int t = it / per_row, h = it - t * per_row;
-    if (s_page[t] < 0) continue;
-    const bool is_v = h >= p.kv.n_kv;
-    const int g = is_v ? h - p.kv.n_kv : h;
-    const size_t row = paged_row(p.kv, s_page[t], g, s_slot[t]);
-    const uint8_t* src = is_v ? p.kv.v : p.kv.k;
-    uint16_t* dst = (is_v ? p.v_out : p.k_out) + ((size_t)(row0 + t) * p.kv.n_kv + g) * D + d0;
-    if (I8) {
-      const uint2 w = *reinterpret_cast<const uint2*>(src + row * D + d0);
-      const float s = (is_v ? p.kv.vs : p.kv.ks)[row];
-      float x[8];
+  const int l = tid % LPH;
+  for (int it0 = tid / LPH; it0 < items; it0 += U * GROUPS) {
+    uint4 w[U];
+    float sc[U];
+    uint16_t* dst[U];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3))), s);
-      *reinterpret_cast<uint4*>(dst) = pack_bf8(x);
-    } else {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + (row * D + d0) * 2);
+    for (int u = 0; u < U; ++u) {
+      const int it = it0 + u * GROUPS;
+      const int t = it < items ? it / per_row : 0, h = it - t * per_row;
+      dst[u] = nullptr;
+      if (it < items && s_page[t] >= 0) {
+        const bool is_v = h >= p.kv.n_kv;
+        const int g = is_v ? h - p.kv.n_kv : h;
+        const size_t row = paged_row(p.kv, s_page[t], g, s_slot[t]);
+        w[u] = *reinterpret_cast<const uint4*>((is_v ? p.kv.v : p.kv.k) + row * (I8 ? D : 2 * D) + l * 16);
+        if (I8) sc[u] = (is_v ? p.kv.vs : p.kv.ks)[row];
+        dst[u] = (is_v ? p.v_out : p.k_out) + ((size_t)(row0 + t) * p.kv.n_kv + g) * D;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (dst[u] == nullptr) continue;
+      if (I8) {
+        const uint32_t c[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)(int8_t)(c[2 * h + (e >> 2)] >> (8 * (e & 3))), sc[u]);
+          *reinterpret_cast<uint4*>(dst[u] + l * 16 + h * 8) = pack_bf8(x);
+        }
+      } else {
+        *reinterpret_cast<uint4*>(dst[u] + l * 8) = w[u];
+      }
     }
   }
 }

@@ -9,9 +9,13 @@ Tolerances, derived from the arithmetic:
 * attention: A = sum_j p_j |v_j| / sum_j p_j bounds what an error of the weights
   does.  The score is a sum of at most 128 fp32 products, off by at most
   128 2^-24 sum |q k| scale, below 2^-12 here (checked: sum |q k| scale < 32);
-  exp2 of it, its sum and the rescaling add less than 2^-14.  With P as a bf16
-  pair the weights carry 2^-16, as one bf16 2^-8, so the bound is
-  2^-8 |o| + (2^-11 + weight) A, the weight's step by the path that the rows take."""
+  exp2 of it, its sum and the rescaling add less than 2^-14.  A weight is off by
+  half a step of its type: 2^-8 as one bf16 (more than 8 rows of a KV head), else
+  2^-11 as f16 (int8 caches) or 2^-16 as a bf16 pair, so the bound is
+  2^-8 |o| + (2^-11 + weight) A.  f16 has a smallest step too, 2^-24: a weight
+  w_j = p_j vs_j is off by up to half of it at a scale where the largest is at
+  least 2^7, by 2^-32 max w, which its code c_j multiplies: + 2^-32 max w sum |c_j|.
+  (Where one key has nearly all the weight and its code is 0, that is all there is.)"""
 
 import pytest
 import torch
@@ -64,6 +68,12 @@ def _rows64(c, table, b, kv):
             x = x * s.cpu()[at].double()[..., None]
         out.append(x.transpose(1, 2).reshape(-1, x.shape[1], x.shape[3])[:kv])
     return out
+
+
+def _scales(c, table, b, kv):
+    """The value scales of sequence b's first kv rows, [kv, n_kv] in 64 bits."""
+    at = table[b, : -(-kv // c.page_size)].long()
+    return c.value_scale.cpu()[at].double().transpose(1, 2).reshape(-1, c.num_kv_heads)[:kv]
 
 
 def _ok():
@@ -249,8 +259,7 @@ def _attend_case(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, max_q=None, max_k
         if m == 0:
             continue
         kk, vv = _rows64(c, table, b, k)
-        # one bf16 weight where the tensor-memory kernel takes the rows, a pair below
-        weight = 2.0 ** -8 if m * grp > 16 else 2.0 ** -16
+        weight = 2.0 ** -8 if m * grp > 8 else (2.0 ** -11 if dtype == I8 else 2.0 ** -16)
         see = torch.arange(k)[None] < (k - m + torch.arange(m)[:, None] + 1)
         for h in range(hq):
             qq = q[int(cu[b]):int(cu[b + 1]), h * d:(h + 1) * d].double()
@@ -262,6 +271,9 @@ def _attend_case(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, max_q=None, max_k
             want, spread = p @ vv[:, h // grp], p @ vv[:, h // grp].abs()
             err = (got[int(cu[b]):int(cu[b + 1]), h] - want).abs()
             room = want.abs() * 2.0 ** -8 + (2.0 ** -11 + weight) * spread
+            if dtype == I8 and m * grp <= 8 and k > 0:
+                codes = vv[:, h // grp].abs() / _scales(c, table, b, k)[:, h // grp, None]
+                room = room + 2.0 ** -32 * (p * _scales(c, table, b, k)[:, h // grp]).amax(-1, keepdim=True) * codes.sum(0)
             worst = float((err - room).max())
             assert worst <= 0, f"sequence {b} head {h}: {worst} over the bound"
 
