@@ -16,7 +16,6 @@
 #include <algorithm>
 #include <cmath>
 #include <climits>
-#include <cstdlib>
 
 #include "act_quant.cuh"
 #include "attention.cuh"
@@ -1185,19 +1184,25 @@ struct PagedPlan {
   size_t bytes;
 };
 
-// Parts of the keys for `pairs` blocks of work on `slots` CTAs at once: the s of
-// the least modelled time, in keys of one CTA.  A part costs its keys plus `unit`
-// (prologue, partial results), joining parts costs `join`.  While all parts run at
-// once the longest counts; beyond that the sum over the slots, and half a part
-// for the uneven end (contexts differ).
-int paged_splits(long long pairs, int max_kv, int slots, int unit, int join, int min_span) {
-  const long long smax = std::max(1, (max_kv + min_span - 1) / min_span), fill = std::max(1LL, slots / pairs);
+// Parts of the keys for `pairs` blocks of work: the s of the least modelled time,
+// in keys of a CTA that has an SM to itself.  A part costs its keys plus `unit`
+// (prologue, epilogue), and `extra` when its results are partial; joining costs
+// `join`.  `resident` CTAs share an SM: two or three together take 1.25 or 1.6 times
+// as long as one (they hide each other's waits until the SM's rate is reached), and
+// beyond that what each SM has to do counts, with half a part for the uneven end.
+// Measured with the rows kernel: 16 sequences x 2 blocks x 2050 keys 42 / 31 / 26 /
+// 24 / 28 us at s = 1 .. 5, one sequence of 131072 keys 115 / 64 / 63 / 65 us at s =
+// 32 / 64 / 88 / 128.
+int paged_splits(long long pairs, int max_kv, int sms, int resident, int unit, int extra, int join, int min_span) {
+  const long long smax = std::max(1, (max_kv + min_span - 1) / min_span);
   long long best_s = 1;
   double best = 1e300;
-  for (int c = 1; c <= 9; ++c) {
-    const long long s = std::min(smax, c <= 8 ? (long long)c : fill);
-    const double part = (double)max_kv / s + unit;
-    const double t = (pairs * s <= slots ? part : pairs * s * part / slots + part / 2) + (s > 1 ? join : 0);
+  for (int c = 1; c <= 14; ++c) {
+    const long long s = std::min(smax, c <= 8 ? (long long)c : std::max(1LL, (c - 8) * (long long)sms / pairs));
+    const double part = (double)((max_kv + s - 1) / s + unit + (s > 1 ? extra : 0));
+    const double k = (double)(pairs * s) / sms;  // parts of an SM
+    const double t = (k <= 1 ? 1.0 : resident > 1 && k <= 2 ? 1.25 : resident > 1 && k <= 3 ? 1.6
+                      : resident > 1 ? k * (1.6 / 3) + 0.5 : k + 0.5) * part + (s > 1 ? join : 0);
     if (t < best) best = t, best_s = s;
   }
   return (int)best_s;
@@ -1207,11 +1212,9 @@ PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, 
   PagedPlan pl;
   memset(&pl, 0, sizeof(pl));
   size_t at = 0;
-  auto cut = [&](PagedCut& c, long long blocks, int R, int slots, int unit, int join, int min_span, int round) {
+  auto cut = [&](PagedCut& c, long long blocks, int R, int resident, int unit, int extra, int join, int min_span, int round) {
     c.blocks = (int)std::min(blocks, (long long)INT_MAX);
-    c.nsplit = paged_splits((long long)c.blocks * n_kv, max_kv, slots, unit, join, min_span);
-    if (R <= 16 && getenv("XS")) c.nsplit = atoi(getenv("XS"));
-    if (R == PCH_R && getenv("XC")) c.nsplit = atoi(getenv("XC"));
+    c.nsplit = paged_splits((long long)c.blocks * n_kv, max_kv, sms, resident, unit, extra, join, min_span);
     c.span = round_up(std::max(1, (max_kv + c.nsplit - 1) / c.nsplit), round);
     const size_t rows = c.nsplit > 1 ? (size_t)c.nsplit * c.blocks * n_kv * R : 0;
     c.ml = at;
@@ -1219,7 +1222,7 @@ PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, 
     at = c.o + rows * D * sizeof(float);
   };
   const long long rows = (long long)max_q * G;
-  const int most_rows = getenv("XM") ? atoi(getenv("XM")) : PAGED_ROWS_MOST;
+  const int most_rows = PAGED_ROWS_MOST;
   const bool chunks = rows > most_rows;
   pl.r = (chunks ? G : rows) > 8 ? 16 : 8;
   pl.most = chunks ? pl.r : (int)std::max(1LL, rows);
@@ -1227,10 +1230,10 @@ PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, 
   // Where most sequences may be as long as the longest, the chunk kernel takes the
   // short ones along: a launch for none or few of them costs more than they do.
   pl.small = chunks && (long long)tokens * 2 < (long long)B * max_q ? pl.r : 0;
-  if (!chunks || pl.small) cut(pl.rows, (long long)B * pl.per, pl.r, sms * 3, 128, 200, 128, 32);
+  if (!chunks || pl.small) cut(pl.rows, (long long)B * pl.per, pl.r, 3, 128, 0, 200, 128, 32);
   if (chunks)
-    cut(pl.chunk, ((long long)tokens * G + PCH_R - 1) / PCH_R + std::min((long long)B, (long long)tokens), PCH_R, sms,
-        512, 256, 512, PCH_KB);
+    cut(pl.chunk, ((long long)tokens * G + PCH_R - 1) / PCH_R + std::min((long long)B, (long long)tokens), PCH_R, 1,
+        256, 512, 256, 512, PCH_KB);
   pl.bytes = at;
   return pl;
 }
