@@ -1150,7 +1150,7 @@ int paged_kv_args(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B
   if ((long long)kv->num_pages > (long long)INT_MAX / kv->page_size / kv->n_kv_heads) return BITNET_ERR_INVALID_ARGUMENT;
   if ((long long)max_pages > (long long)INT_MAX / kv->page_size) return BITNET_ERR_INVALID_ARGUMENT;
   if (!aligned(kv->k_pages, 16) || !aligned(kv->v_pages, 16) || !aligned(block_table, 4) ||
-      !aligned(kv->k_scale, 4) || !aligned(kv->v_scale, 4))
+      !aligned(kv->k_scale, 16) || !aligned(kv->v_scale, 16))
     return BITNET_ERR_ALIGNMENT;
   out->k = (uint8_t*)kv->k_pages;
   out->v = (uint8_t*)kv->v_pages;
@@ -1312,14 +1312,6 @@ int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspa
   if (pl.chunk.blocks > 0) {
     using S = PchShape<D, I8>;
     auto k = paged_chunk_kernel<D, I8>;
-    static std::atomic<int> regs{0};  // the register shares are part of the launch's registers
-    if (regs.load() == 0) {
-      cudaFuncAttributes fa;
-      const cudaError_t e = cudaFuncGetAttributes(&fa, k);
-      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
-      regs.store(fa.numRegs);
-    }
-    if (regs.load() != S::REGS_LAUNCH) return cuda_fail(cudaErrorInvalidConfiguration, "paged_chunk_kernel registers");
     if (int e = ensure_smem(k, &g_smem_pch[idx])) return e;
     CUtensorMap mk, mv;
     memset(&mk, 0, sizeof(mk));

@@ -54,6 +54,7 @@ __device__ __forceinline__ bool paged_block_of(const PagedAttnParams& p, int b, 
     if (lane == 0) record_error(DEV_ERR_BOUNDS, 350);
     return false;
   }
+  if (row0 >= n * p.G) return false;
   o.b = b;
   o.row0 = row0;
   o.nrows = min(R, n * p.G - row0);
@@ -70,14 +71,56 @@ __device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int
   const int b = bx / p.per, row0 = (bx - b * p.per) * R;
   const long long rows = (long long)(p.cu[b + 1] - p.cu[b]) * p.G;
   if (rows > p.most && (long long)p.max_q * p.G > p.most) return false;
-  if (row0 > 0 && row0 >= rows) return false;
   return paged_block_of<R>(p, b, row0, lane, o);
 }
 
-// Block bx of the R-row blocks of all sequences of more than p.small rows, in
-// order; whole warp.
+// The R-row blocks of all sequences of more than p.small rows, numbered so that
+// those with more keys come first (CTAs start in that order, so the long ones do
+// not end last); whole warp.  Blocks are ranked by their 128-key tiles: the rank
+// of block bx is found by bisection over the number of tiles, counting the blocks
+// with at least that many by arithmetic (a sequence's later blocks see more).
+// Equal ranks are in the order of sequences.  Up to 32 sequences; beyond that the
+// blocks are in the order of sequences alone, the last first.
 template <int R>
 __device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
+  if (p.B <= 32) {
+    int rows = 0, past = 0;
+    if (lane < p.B) {
+      const int n = min(max(p.cu[lane + 1] - p.cu[lane], 0), p.max_q);
+      past = min(p.kv_lens[lane], p.max_kv) - n;
+      rows = n * p.G > p.small ? n * p.G : 0;
+    }
+    const int nb = (rows + R - 1) / R;
+    // this sequence's blocks of at least t tiles: those whose last row's token is y or later
+    auto count = [&](int t) {
+      const long long y = (long long)(t - 1) * 128 - past;
+      if (t <= 0 || y <= 0 || nb == 0) return nb;
+      const long long first = y * p.G;  // the first row of token y
+      return first >= rows ? 0 : nb - (int)(first / R);
+    };
+    if (bx >= (int)__reduce_add_sync(0xffffffffu, (unsigned)nb)) return false;
+    int lo = 0, hi = (p.max_kv + 127) / 128 + 1;  // more than bx blocks have lo tiles, not more have hi
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int)__reduce_add_sync(0xffffffffu, (unsigned)count(mid)) > bx) lo = mid;
+      else hi = mid;
+    }
+    // among the blocks of exactly lo tiles
+    const int above = count(lo + 1), here = count(lo) - above;
+    int rank = bx - (int)__reduce_add_sync(0xffffffffu, (unsigned)above), sum = here;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, sum > rank);
+    if (!over) return false;
+    const int src = __ffs(over) - 1;
+    rank -= __shfl_sync(0xffffffffu, sum - here, src);
+    const int last = __shfl_sync(0xffffffffu, nb - 1 - above, src);
+    return paged_block_of<R>(p, src, (last - rank) * R, lane, o);
+  }
+  bx = p.blocks - 1 - bx;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int i = b0 + lane;
     const int rows = (i < p.B ? min(max(p.cu[i + 1] - p.cu[i], 0), p.max_q) : 0) * p.G;

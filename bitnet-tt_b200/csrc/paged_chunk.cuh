@@ -2,27 +2,41 @@
 // tensor cores (what paged_attention.cuh says of rows, blocks and parts holds).
 //
 // A CTA takes up to 256 packed rows of one (sequence, KV head), as two tiles of
-// 128 rows, over one part of the keys, 128 keys at a time:
-//   S_t = Q_t K^T     128 x 128 fp32 in tensor memory, Q_t and K from shared memory
-//   P_t = exp2(scale log2(e) S_t - m), written over S_t as bf16
+// 128 rows, over one part of the keys, 64 keys a step:
+//   S_t = Q_t K^T     128 x 64 fp32 in tensor memory, Q_t and K from shared memory
+//   P_t = exp2(scale log2(e) S_t - m), written over S_t as 16-bit floats
 //   O_t += P_t V      P_t from tensor memory, V (keys x dims) from shared memory
+// Tensor memory (512 columns) holds two S of each row tile and the two O.  So S of
+// the next step is there when the softmax of one is done, and neither waits for
+// the other: with one S of 128 keys a tile, the products that follow a softmax and
+// the signals between them (about 1300 cycles) stood in every step's chain, and
+// two 4096-token chunks over 16384 keys took 690 us.  The price is that 64-key
+// score products read Q twice as often: 48 cycles each (shared memory's rate)
+// instead of half of 64.
 // Roles, one warp each unless said otherwise:
 //   warps 0-3, 4-7   softmax of tile 0 and of tile 1: a thread owns a row (a lane of
 //                    tensor memory), so maxima and sums need no shuffles
-//   warp 8           issues the MMAs: O_0, S_0 of the next keys, O_1, S_1; while one tile's
-//                    products run, the other tile's softmax does
+//   warps 8, 10      issue the MMAs of tile 0 and of tile 1: O_t of a step, then S_t of the step
+//                    after next.  Two, because the tensor cores queue few MMAs: a look at a
+//                    barrier costs the issuing warp about 100 cycles even when it is complete,
+//                    and with one warp those were gaps (980 cycles a tile and step for 640 of work)
 //   warp 9 (bf16)    loads K and V tiles by TMA, a box per page, into a ring of slots
-//   warps 12-15 (int8)  load codes and write them to the slots as bf16 (exact)
+//   warps 12-15 (int8)  load codes and write them to the slots as f16
 // The softmax's maximum is lazy: O and the sum are rescaled only when a row's
 // maximum grew by more than 2^8, so weights reach at most 2^8 and the pass over
-// O is rare.  P is rounded to bf16 (half a step, 2^-9 of a weight on average
-// less), the output's own precision; sums and outputs are fp32.
+// O is rare (it waits for the products in flight).  P is rounded to bf16 (half a step: 2^-8 of a weight), the output's
+// own precision; sums and outputs are fp32.  The exponentials are what a tile
+// costs most: 16 a cycle and SM against 4096 products.  A quarter of them is
+// therefore computed on the multiply-add units (ex2_poly2).
 //
-// int8: a code is a bf16 value, so the products see the codes exactly; the
-// keys' scales multiply the scores, the values' scales the weights, both in
-// fp32.  Codes come out of their words as (0, 2) and (1, 3) pairs, so every four
-// dims of the slots stand in the order 0, 2, 1, 3: Q is laid out the same way,
-// and the output is put back when it is stored.
+// int8: everything is f16.  The keys' codes are f16 values exactly, and their
+// scales multiply the scores in fp32, where an error would be raised to a power.
+// The values are code * scale, rounded to f16 (2^-11) at a power of two taken from
+// the largest scale of the part, which keeps rows down to 2^-21 of it at that
+// precision.  Q is scaled by a power of two per row (exact), P has f16's 11 bits.
+// Codes come out of their words as (0, 2) and (1, 3) pairs, so every four dims of
+// the slots stand in the order 0, 2, 1, 3: Q is laid out the same way, and the
+// output is put back when it is stored.
 #pragma once
 #include <cuda.h>
 
@@ -31,57 +45,88 @@
 namespace bitnet {
 
 constexpr int PCH_R = 256;   // rows of a CTA
-constexpr int PCH_KB = 128;  // keys of a tile
+constexpr int PCH_KB = 128;  // keys of a tile (a slot of K or V)
+constexpr int PCH_STEP = 64; // keys of a step
 constexpr int PCH_MAX_SLOTS = 8;
+constexpr float PCH_GROWTH = 8.f;
 
 template <int D, bool I8>
 struct PchShape {
   static constexpr int THREADS = I8 ? 512 : 384;
   static constexpr int TILE = 128 * D * 2;          // bytes of Q_t, K or V as bf16
   static constexpr int NSLOT = D == 64 ? 8 : (I8 ? 4 : 5);
-  // Scales [RING tiles][128 keys', 128 values'].  When the codes of key tile j are in their
-  // slot, the value slot of tile j - RING has been released, after both softmaxes of that tile.
+  // int8: the keys' scales [RING tiles][128], then the rows' factors [256].  When the codes of
+  // key tile j are in their slot, the value slot of tile j - RING has been released, after both
+  // softmaxes of that tile.
   static constexpr int RING = NSLOT / 2 + 1;
-  static constexpr int SCALES = I8 ? RING * 1024 : 0;
-  static constexpr int CTRL = 256;
-  static constexpr int SMEM = 2 * TILE + NSLOT * TILE + SCALES + CTRL;
-  // registers a thread: the launch gives 168 (384 threads) or 128 (512 threads)
-  static constexpr int REGS_SOFTMAX = I8 ? 176 : 208;
-  static constexpr int REGS_MMA = I8 ? 56 : 88;
-  static constexpr int REGS_CONVERT = 104;
-  static constexpr int REGS_LAUNCH = I8 ? 128 : 168;
+  static constexpr int EXTRA = I8 ? RING * 512 + 1024 : 0;
+  // Weights are exp2(x - m + LIFT): with f16's range the smallest step is below 2^-31 of the largest.
+  static constexpr float LIFT = I8 ? 7.f : 0.f;
+  static constexpr int CTRL = 512;
+  static constexpr int SMEM = 2 * TILE + NSLOT * TILE + EXTRA + CTRL;
 };
-static_assert(256 * 208 + 128 * 88 <= 384 * 168, "register shares within the launch's");
-static_assert(256 * 176 + 128 * 56 + 128 * 104 <= 512 * 128, "register shares within the launch's");
 
-__device__ __forceinline__ uint32_t bf2_sub(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+// One lane of a converged warp.  The MMAs and their commits are issued under it:
+// under `lane == 0` the compiler has to allow for several lanes with different
+// operands, and an MMA took about 75 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// The codes in bytes 0 and 2 of w as a bf16 pair: for the byte u of a code,
-// bf16 128 + (u & 127) and 128 + (u & 128) are both bit patterns (0x4300 | bits),
-// and their difference is the code.
-__device__ __forceinline__ uint32_t codes_bf2(uint32_t w) {
-  return bf2_sub((w & 0x007F007Fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u);
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
 }
+// 2^y for two values without the exponential unit: n = round(y) by adding 1.5 * 2^23,
+// 2^(y - n) by a cubic (fitted for the least largest relative error on [-1/2, 1/2]:
+// 7.5e-5, an eighth of a bf16's half step), and n added to the exponent.  y is held at
+// -126 and above, where the result is as good as 0.
+__device__ __forceinline__ void ex2_poly2(uint64_t y, float& a, float& b) {
+  uint32_t lo, hi;
+  f2_split(y, lo, hi);
+  float x0, x1;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(__uint_as_float(lo)), "f"(-126.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(__uint_as_float(hi)), "f"(-126.f));
+  y = f2_make(__float_as_uint(x0), __float_as_uint(x1));
+  const uint64_t t = f2_add(y, f2_splat(12582912.f));
+  const uint64_t f = f2_fma(f2_add(t, f2_splat(-12582912.f)), f2_splat(-1.f), y);
+  uint64_t p = f2_fma(f2_splat(0.05517166852951050f), f, f2_splat(0.2426111251115799f));
+  p = f2_fma(p, f, f2_splat(0.6932609677314758f));
+  p = f2_fma(p, f, f2_splat(0.9999280571937561f));
+  uint32_t p0, p1, t0, t1;
+  f2_split(p, p0, p1);
+  f2_split(t, t0, t1);
+  a = __uint_as_float(p0 + (t0 << 23));
+  b = __uint_as_float(p1 + (t1 << 23));
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// The exponent field of the power of two 2^k / 2^floor(log2 x), x by its fp32 bits.
+__device__ __forceinline__ uint32_t pow2_field(uint32_t bits, int k) { return 254u + k - max(bits >> 23, 32u); }
 
 struct PchCtrl {
   uint64_t full[PCH_MAX_SLOTS], empty[PCH_MAX_SLOTS];
-  uint64_t s_full[2], p_ready[2], o_full[2], tail, drain;
+  uint64_t s_full[2][2], p_ready[2][2];  // [row tile][step % 2]
+  uint64_t o_done[2][2], drain[2], tail; // o_done: O_t holds the step
   uint32_t tmem;
   int abort_flag;
+  uint32_t v_top;  // int8: the largest value scale of the part, by its bits
 };
-static_assert(sizeof(PchCtrl) <= 256, "control block");
-
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
+static_assert(sizeof(PchCtrl) <= 512, "control block");
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -128,12 +173,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 template <int D, bool I8>
 __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     paged_chunk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap map_k,
@@ -144,7 +183,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   uint8_t* sm_q = smem_pch;
   uint8_t* sm_slots = sm_q + 2 * S::TILE;
   float* sm_scale = reinterpret_cast<float*>(sm_slots + S::NSLOT * S::TILE);
-  PchCtrl* ctrl = reinterpret_cast<PchCtrl*>(sm_slots + S::NSLOT * S::TILE + S::SCALES);
+  float* sm_fac = sm_scale + S::RING * 128;
+  PchCtrl* ctrl = reinterpret_cast<PchCtrl*>(sm_slots + S::NSLOT * S::TILE + S::EXTRA);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
   pdl_wait();
@@ -156,32 +196,36 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   const int nparts = paged_parts(p, blk.kend);
   if (sp >= nparts) return;
   const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);
-  // 128-key tiles of the two row tiles (the second sees at least the first's keys)
+  // 64-key steps of the two row tiles (the second sees at least the first's keys)
   const int end0 = min(k1, max(0, blk.past + (blk.row0 + min(blk.nrows, 128) - 1) / p.G + 1));
-  const int n0 = max(0, (end0 - k0 + PCH_KB - 1) / PCH_KB);
-  const int n1 = blk.nrows > 128 ? max(0, (k1 - k0 + PCH_KB - 1) / PCH_KB) : 0;
-  const int ntile = max(n0, n1);
+  const int n0 = max(0, (end0 - k0 + PCH_STEP - 1) / PCH_STEP);
+  const int n1 = blk.nrows > 128 ? max(0, (k1 - k0 + PCH_STEP - 1) / PCH_STEP) : 0;
+  const int nstep = max(n0, n1), ntile = (nstep + 1) / 2;
 
   volatile int* abort_flag = &ctrl->abort_flag;
   if (tid == 0) {
     for (int s = 0; s < S::NSLOT; ++s) {
       mbar_init(&ctrl->full[s], I8 ? 4 : 1);
-      mbar_init(&ctrl->empty[s], 1);
+      mbar_init(&ctrl->empty[s], n1 > 0 ? 2 : 1);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&ctrl->s_full[t], 1);
-      mbar_init(&ctrl->p_ready[t], 4);
-      mbar_init(&ctrl->o_full[t], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&ctrl->s_full[t][h], 1);
+        mbar_init(&ctrl->p_ready[t][h], 4);
+        mbar_init(&ctrl->o_done[t][h], 1);
+      }
+      mbar_init(&ctrl->drain[t], 1);
     }
     mbar_init(&ctrl->tail, 1);
-    mbar_init(&ctrl->drain, 1);
     ctrl->abort_flag = 0;
+    ctrl->v_top = 0;
     fence_mbar_init();
   }
   if (warp == 8) {
     tmem_alloc(&ctrl->tmem, 512);
     tmem_relinquish();
   }
+  if (I8) __syncthreads();
   // Q, 16 bytes at a time, into the swizzled tiles (rows past the block: zeros)
   for (int i = tid; i < 2 * 128 * (D / 8); i += S::THREADS) {
     const int r = i / (D / 8), c = i % (D / 8);
@@ -191,20 +235,51 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       const int row = blk.row0 + r, tok = row / p.G;
       w = *reinterpret_cast<const uint4*>(p.q + (size_t)(blk.tok0 + tok) * p.ld_q +
                                           (size_t)(g * p.G + row - tok * p.G) * D + c * 8);
-      if (I8)
-        w = make_uint4(__byte_perm(w.x, w.y, 0x5410), __byte_perm(w.x, w.y, 0x7632), __byte_perm(w.z, w.w, 0x5410),
-                       __byte_perm(w.z, w.w, 0x7632));
+    }
+    if (I8) {  // D / 8 neighbouring lanes hold a row: its largest value goes to 2^13 .. 2^14
+      float x[8];
+      unpack_bf8(w, x);
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = D / 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const uint32_t field = pow2_field(top, 13);
+      const float f = __uint_as_float(field << 23);
+      w = make_uint4(f16x2_of(x[0] * f, x[2] * f), f16x2_of(x[1] * f, x[3] * f), f16x2_of(x[4] * f, x[6] * f),
+                     f16x2_of(x[5] * f, x[7] * f));
+      if (c == 0) sm_fac[r] = __uint_as_float((254u - field) << 23);
     }
     const int rr = r & 127;
     *reinterpret_cast<uint4*>(sm_q + (r >> 7) * S::TILE + (c >> 3) * HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = w;
+  }
+  if (I8) {  // the largest value scale of the part's rows, four rows (of one page) a load
+    const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
+    float top = 0.f;
+#pragma unroll 4
+    for (int key = k0 + 4 * tid; key < k1; key += 4 * S::THREADS) {
+      const int page = table[key >> p.kv.page_shift];
+      if (page < 0 || page >= p.kv.num_pages) continue;  // reported by the loads below
+      const float4 v = *reinterpret_cast<const float4*>(
+          p.kv.vs + paged_row(p.kv, page, g, key & ((1 << p.kv.page_shift) - 1)));
+      top = fmaxf(top, v.x);
+      if (key + 1 < k1) top = fmaxf(top, v.y);
+      if (key + 2 < k1) top = fmaxf(top, v.z);
+      if (key + 3 < k1) top = fmaxf(top, v.w);
+    }
+    const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (lane == 0) atomicMax(&ctrl->v_top, t);
   }
   fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = ctrl->tmem;
+  // All 512 columns are this CTA's, so they start at 0: a constant, as the MMAs' operands
+  // should be (below).
+  constexpr uint32_t tbase = 0;
 
   auto wait = [&](uint64_t* bar, uint32_t parity, int site) -> bool {
+    if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
     if (!mbar_wait(bar, parity, site)) {
       *abort_flag = 1;
@@ -214,9 +289,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   };
 
   if (warp >= 12) {
-    // ---------------- int8: codes to bf16 slots ----------------
+    // ---------------- int8: codes to f16 slots ----------------
     if constexpr (I8) {
-      regs_dec<S::REGS_CONVERT>();
       constexpr int NL = D / 16;  // 16-byte loads of a lane: 32 rows of a warp
       const int w = warp - 12;
       const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
@@ -260,22 +334,30 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
                                                      c * 16);
         }
       };
-      auto convert = [&](int it, const uint4 (&buf)[NL]) -> bool {
+      // scale: of this lane's row of the warp's 32, as f16 (values only)
+      auto convert = [&](int it, const uint4 (&buf)[NL], uint32_t scale) -> bool {
         const int slot = it % S::NSLOT;
         if (it >= S::NSLOT && !__all_sync(0xffffffffu, wait(&ctrl->empty[slot], ((it / S::NSLOT) + 1) & 1, 362)))
           return false;
         uint8_t* dst = sm_slots + slot * S::TILE;
+        const bool scaled = it & 1;
 #pragma unroll
         for (int u = 0; u < NL; ++u) {
           int row, c;
           place(u, row, c);
+          const uint32_t sc = scaled ? __shfl_sync(0xffffffffu, scale, row) : 0u;
           row += 32 * w;
           uint8_t* at = dst + (c >> 2) * HALF + row * 128;
-          const uint4 x = buf[u];
-          *reinterpret_cast<uint4*>(at + (((2 * (c & 3)) ^ (row & 7)) << 4)) =
-              make_uint4(codes_bf2(x.x), codes_bf2(x.x >> 8), codes_bf2(x.y), codes_bf2(x.y >> 8));
-          *reinterpret_cast<uint4*>(at + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) =
-              make_uint4(codes_bf2(x.z), codes_bf2(x.z >> 8), codes_bf2(x.w), codes_bf2(x.w >> 8));
+          const uint32_t x[4] = {buf[u].x, buf[u].y, buf[u].z, buf[u].w};
+          uint32_t y[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[2 * e] = codes_f2(x[e]), y[2 * e + 1] = codes_f2(x[e] >> 8);
+          if (scaled) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = h2_mul(y[e], sc);
+          }
+          *reinterpret_cast<uint4*>(at + (((2 * (c & 3)) ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(at + (((2 * (c & 3) + 1) ^ (row & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
         }
         return true;
       };
@@ -284,6 +366,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctrl->full[it % S::NSLOT]);
       };
+      const float v_up = __uint_as_float(pow2_field(ctrl->v_top, 7) << 23);
       uint4 bk[NL], bv[NL];
       look_up(0);
       load(0, p.kv.k, bk);
@@ -297,83 +380,75 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
           vs = p.kv.vs[row];
         }
         load(j, p.kv.v, bv);
-        if (!convert(2 * j, bk)) break;
-        float* sc = sm_scale + (j % S::RING) * 256 + 32 * w + lane;
-        sc[0] = ks;
-        sc[128] = vs;
-        arrive(2 * j);
         look_up(j + 1);
+        if (!convert(2 * j, bk, 0)) break;
+        sm_scale[(j % S::RING) * 128 + 32 * w + lane] = ks;
+        arrive(2 * j);
         load(j + 1, p.kv.k, bk);
-        if (!convert(2 * j + 1, bv)) break;
+        if (!convert(2 * j + 1, bv, f16x2_of(vs * v_up, vs * v_up))) break;
         arrive(2 * j + 1);
       }
     }
   } else if (warp >= 8) {
-    regs_dec<S::REGS_MMA>();
-    if (warp == 8 && lane == 0 && ntile > 0) {
-      // ---------------- MMA issuer ----------------
-      constexpr uint32_t idesc_s = idesc_bf16_f32(128, PCH_KB);
-      constexpr uint32_t idesc_o = idesc_bf16_f32(128, D) | (1u << 16);  // V: dims contiguous
-      const uint32_t q0 = smem_u32(sm_q), s0 = smem_u32(sm_slots);
-      auto qk = [&](int t, int j) {
-        const uint32_t a = q0 + t * S::TILE, b = s0 + ((2 * j) % S::NSLOT) * S::TILE;
+    const int t = warp == 8 ? 0 : 1, nt = t ? n1 : n0;
+    if ((warp == 8 && nstep > 0) || (warp == 10 && n1 > 0)) {
+      // ---------------- MMA issuers ----------------
+      constexpr uint32_t f16_types = (1u << 7) | (1u << 10);  // set: bf16, clear: f16
+      constexpr uint32_t idesc_s = idesc_bf16_f32(128, PCH_STEP) & (I8 ? ~f16_types : ~0u);
+      constexpr uint32_t idesc_o = (idesc_bf16_f32(128, D) & (I8 ? ~f16_types : ~0u)) | (1u << 16);  // V: dims contiguous
+      // descriptors of the first product: the others differ in the address field (16-byte units)
+      const uint64_t dq = smem_desc_sw128(smem_u32(sm_q) + t * S::TILE, 16, 1024),
+                     dk = smem_desc_sw128(smem_u32(sm_slots), 16, 1024), dv = smem_desc_sw128(smem_u32(sm_slots), HALF, 1024);
+      auto qk = [&](int slot, int h) {
+        const uint64_t b = dk + slot * (S::TILE >> 4) + h * (PCH_STEP * 128 >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * HALF + (k & 3) * 32;
-          mma_f16_ss(tbase + t * 128, smem_desc_sw128(a + off, 16, 1024), smem_desc_sw128(b + off, 16, 1024), idesc_s, k > 0);
+          const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32) >> 4;
+          mma_f16_ss(tbase + t * 128 + h * 64, dq + off, b + off, idesc_s, k > 0);
         }
+        tc_commit(&ctrl->s_full[t][h]);
       };
-      auto pv = [&](int t, int j) {
-        const uint32_t b = s0 + ((2 * j + 1) % S::NSLOT) * S::TILE;
+      auto pv = [&](int slot, int h, bool first) {
+        const uint64_t b = dv + slot * (S::TILE >> 4) + h * (PCH_STEP * 128 >> 4);
+        const uint32_t a = tbase + t * 128 + h * 64, d = tbase + 256 + t * D;
 #pragma unroll
-        for (int k = 0; k < PCH_KB / 16; ++k)
-          mma_f16_ts(tbase + 256 + t * D, tbase + t * 128 + k * 8, smem_desc_sw128(b + k * 2048, HALF, 1024), idesc_o,
-                     (j | k) > 0);
+        for (int k = 0; k < PCH_STEP / 16; ++k) mma_f16_ts(d, a + k * 8, b + k * (16 * 128 >> 4), idesc_o, k > 0 || !first);
+        tc_commit(&ctrl->o_done[t][h]);
       };
-      auto filled = [&](int it, int site) {
-        const bool ok = wait(&ctrl->full[it % S::NSLOT], (it / S::NSLOT) & 1, site);
+      auto arrived = [&](uint64_t* bar, uint32_t parity, int site) {
+        const bool ok = __all_sync(0xffffffffu, wait(bar, parity, site));
         tc_fence_after();
         return ok;
       };
+      auto filled = [&](int it, int site) { return arrived(&ctrl->full[it % S::NSLOT], (it / S::NSLOT) & 1, site); };
+      // Each issuer releases every slot, those past its own tile's keys too.
       bool ok = filled(0, 363);
-      if (ok) {
-        if (n0 > 0) {
-          qk(0, 0);
-          tc_commit(&ctrl->s_full[0]);
-        }
-        if (n1 > 0) {
-          qk(1, 0);
-          tc_commit(&ctrl->s_full[1]);
-        }
+      if (ok && elect_one()) {
+        if (nt > 0) qk(0, 0);
+        if (nt > 1) qk(0, 1);
         tc_commit(&ctrl->empty[0]);
       }
-      for (int j = 0; ok && j < ntile; ++j) {
-        ok = filled(2 * j + 1, 364);
-        bool next = false;  // K of tile j + 1 seen
-        for (int t = 0; ok && t < 2; ++t) {
-          const int nt = t ? n1 : n0;
-          if (j < nt) {
-            ok = wait(&ctrl->p_ready[t], j & 1, 365);
-            if (!ok) break;
-            tc_fence_after();
-            pv(t, j);
-          }
-          if (t == (n1 > 0)) tc_commit(&ctrl->empty[(2 * j + 1) % S::NSLOT]);  // V read by its last tile
-          if (j + 1 < nt) {
-            if (!next) ok = filled(2 * j + 2, 366);
-            if (!ok) break;
-            next = true;
-            qk(t, j + 1);
-            tc_commit(&ctrl->s_full[t]);
-          } else if (j + 1 == nt) {
-            tc_commit(&ctrl->o_full[t]);
-          }
+      __syncwarp();
+      for (int i = 0; ok && i < nstep; ++i) {
+        const int j = i >> 1, h = i & 1;
+        const int vs = (2 * j + 1) % S::NSLOT, ks = (2 * j + 2) % S::NSLOT;  // slots of V, and of the next K
+        if (h == 0) {
+          ok = filled(2 * j + 1, 364);
+          if (ok && i + 2 < nstep) ok = filled(2 * j + 2, 366);
         }
-        if (next) tc_commit(&ctrl->empty[(2 * j + 2) % S::NSLOT]);
+        if (ok && i < nt) ok = arrived(&ctrl->p_ready[t][h], j & 1, 365);
+        if (ok && elect_one()) {
+          if (i < nt) pv(vs, h, i == 0);
+          if (i + 2 < nt) qk(ks, h);
+          if (h == 1 || i + 1 == nstep) tc_commit(&ctrl->empty[vs]);
+          if (i + 2 < nstep && (h == 1 || i + 3 == nstep)) tc_commit(&ctrl->empty[ks]);
+        }
+        __syncwarp();
       }
       if (!ok) {  // let the MMAs in flight end before tensor memory is freed
-        tc_commit(&ctrl->drain);
-        mbar_wait(&ctrl->drain, 0, 367);
+        if (elect_one()) tc_commit(&ctrl->drain[t]);
+        __syncwarp();
+        mbar_wait(&ctrl->drain[t], 0, 367);
       }
     } else if (!I8 && warp == 9) {
       // ---------------- bf16: TMA loads ----------------
@@ -434,7 +509,6 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     }
   } else {
     // ---------------- softmax: a thread owns a row ----------------
-    regs_inc<S::REGS_SOFTMAX>();
     const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
     const int nt = t ? n1 : n0;
     const bool live = r < blk.nrows;
@@ -443,54 +517,64 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     const int lim = live ? blk.past + tok + 1 : INT_MAX;
     const int lim_min = __reduce_min_sync(0xffffffffu, lim);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tbase + lanes + t * 128, to = tbase + lanes + 256 + t * D;
-    const uint64_t scale2 = f2_splat(p.scale_log2);
+    const uint32_t to = tbase + lanes + 256 + t * D;
+    const float scale = I8 ? p.scale_log2 * sm_fac[r] : p.scale_log2;
+    const uint64_t scale2 = f2_splat(scale);
     float m = -INFINITY;
     uint64_t l2[2] = {0, 0};
     bool ok = true;
-    for (int j = 0; j < nt; ++j) {
-      ok = wait(&ctrl->s_full[t], j & 1, 371);
+    for (int i = 0; i < nt; ++i) {
+      const int j = i >> 1, h = i & 1;
+      ok = wait(&ctrl->s_full[t][h], j & 1, 371);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
       if (warp_live) {
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s + 32 * c);
+        const uint32_t ts = tbase + lanes + t * 128 + h * 64;
+        uint32_t s[PCH_STEP];
+        tmem_ld32(ts, s);
+        tmem_ld32(ts + 32, s + 32);
         tmem_wait_ld();
-        const float* sc = sm_scale + (j % S::RING) * 256;
         if (I8) {
+          const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(sm_scale + (j % S::RING) * 128 + h * 64);
 #pragma unroll
-          for (int c = 0; c < 128; c += 4) {
-            const float4 k = *reinterpret_cast<const float4*>(sc + c);
-            s[c] = __float_as_uint(__uint_as_float(s[c]) * k.x);
-            s[c + 1] = __float_as_uint(__uint_as_float(s[c + 1]) * k.y);
-            s[c + 2] = __float_as_uint(__uint_as_float(s[c + 2]) * k.z);
-            s[c + 3] = __float_as_uint(__uint_as_float(s[c + 3]) * k.w);
+          for (int c = 0; c < PCH_STEP / 4; ++c) {
+            const ulonglong2 k = sc[c];
+            f2_split(f2_mul(f2_make(s[4 * c], s[4 * c + 1]), k.x), s[4 * c], s[4 * c + 1]);
+            f2_split(f2_mul(f2_make(s[4 * c + 2], s[4 * c + 3]), k.y), s[4 * c + 2], s[4 * c + 3]);
           }
         }
-        const int base = k0 + j * PCH_KB;
-        if (base + PCH_KB > min(lim_min, k1)) {
+        const int base = k0 + i * PCH_STEP;
+        if (base + PCH_STEP > min(lim_min, k1)) {
           const int see = min(lim, k1) - base;
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
+          for (int c = 0; c < PCH_STEP; ++c)
             if (c >= see) s[c] = 0xff800000u;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-        if (j == 0) {
+        for (int c = 0; c < PCH_STEP; c += 2)
+          mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
+        if (i == 0) {
           m = top;
-        } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+        } else if (__any_sync(0xffffffffu, top > m + PCH_GROWTH)) {
           const float mn = fmaxf(m, top);
           const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
           m = mn;
           const uint64_t f2 = f2_splat(f);
           l2[0] = f2_mul(l2[0], f2);
           l2[1] = f2_mul(l2[1], f2);
+          // O holds all steps so far once the product of step i - 1 is in (that of step i - 3, one
+          // phase earlier on this barrier, is: S of step i - 1 came after it)
+          ok = wait(&ctrl->o_done[t][h ^ 1], ((i - 1) >> 1) & 1, 374);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D; c += 32) {
             uint32_t o[32];
@@ -501,23 +585,23 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
             tmem_st32(to + c, o);
           }
         }
-        const uint64_t ref2 = f2_splat(m == -INFINITY ? 0.f : -m);
+        const uint64_t ref2 = f2_splat(m == -INFINITY ? 0.f : S::LIFT - m);
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) {
+        for (int c = 0; c < PCH_STEP; c += 32) {
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            uint32_t a, b;
-            f2_split(f2_fma(f2_make(s[c + 2 * e], s[c + 2 * e + 1]), scale2, ref2), a, b);
-            float x = ex2(__uint_as_float(a)), y = ex2(__uint_as_float(b));
-            l2[e & 1] = f2_add(l2[e & 1], f2_make(__float_as_uint(x), __float_as_uint(y)));
-            if (I8) {
-              const float2 v = *reinterpret_cast<const float2*>(sc + 128 + c + 2 * e);
-              // a masked key's scale may be anything
-              x = x == 0.f ? 0.f : x * v.x;
-              y = y == 0.f ? 0.f : y * v.y;
+            const uint64_t z = f2_fma(f2_make(s[c + 2 * e], s[c + 2 * e + 1]), scale2, ref2);
+            float x, y;
+            if (e % 4 == 3) {
+              ex2_poly2(z, x, y);
+            } else {
+              uint32_t a, b;
+              f2_split(z, a, b);
+              x = ex2(__uint_as_float(a)), y = ex2(__uint_as_float(b));
             }
-            pw[e] = bf2_of(x, y);
+            l2[e & 1] = f2_add(l2[e & 1], f2_make(__float_as_uint(x), __float_as_uint(y)));
+            pw[e] = I8 ? f16x2_of(x, y) : bf2_of(x, y);
           }
           tmem_st16(ts + c / 2, pw);
         }
@@ -525,9 +609,9 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->p_ready[t]);
+      if (lane == 0) mbar_arrive(&ctrl->p_ready[t][h]);
     }
-    if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait(&ctrl->o_full[t], 0, 372));
+    if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait(&ctrl->o_done[t][(nt - 1) & 1], ((nt - 1) >> 1) & 1, 372));
     if (ok && warp_live) {
       tc_fence_after();
       uint32_t a, b, c2, d2;
@@ -536,7 +620,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       const float l = (__uint_as_float(a) + __uint_as_float(b)) + (__uint_as_float(c2) + __uint_as_float(d2));
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       const size_t pr = (((size_t)sp * p.blocks + bx) * p.kv.n_kv + g) * PCH_R + r;
-      if (live && nparts > 1) p.part_ml[pr] = make_float2(m, l);
+      if (live && nparts > 1) p.part_ml[pr] = make_float2(m - S::LIFT, l);
+      const float vf = I8 ? __uint_as_float((254u - pow2_field(ctrl->v_top, 7)) << 23) : 1.f;  // the values' power of two
       uint16_t* dst = p.out + ((size_t)(blk.tok0 + tok) * p.n_heads + g * p.G + row - tok * p.G) * D;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
@@ -557,6 +642,10 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
           }
         }
         if (!live) continue;
+        if (I8) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * vf);
+        }
         if (nparts > 1) {
 #pragma unroll
           for (int e = 0; e < 32; e += 4)

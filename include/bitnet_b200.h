@@ -292,8 +292,8 @@ int bitnet_attention_prefill_varlen(const void* q, const void* k_cache, const vo
  * `pos` of sequence b is row pos % page_size of page
  * block_table[b * max_pages + pos / page_size].  BITNET_KV_INT8: a code's value
  * is code * scale, one fp32 scale per row of a KV head, [num_pages][n_kv_heads][page_size].
- * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; page pools 16-byte
- * aligned; num_pages * n_kv_heads * page_size < 2^31.
+ * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; pools and scales 16-byte
+ * aligned, scales not negative; num_pages * n_kv_heads * page_size < 2^31.
  *
  * Common arguments: block_table int32 [B][max_pages] (only entries that a
  * sequence's length reaches are read); cu_seqlens int32 [B + 1], the packed row

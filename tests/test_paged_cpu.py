@@ -45,6 +45,7 @@ COMMON = [({"B": 0}, -1), ({"max_pages": 0}, -1), ({"block_table": None}, -1), (
 COMMON_KV = [({"k_pages": None}, -1), ({"v_pages": None}, -1), ({"k_pages": 8}, -2), ({"num_pages": 0}, -1),
              ({"page_size": 8}, -1), ({"page_size": 48}, -1), ({"page_size": 512}, -1), ({"n_kv_heads": 0}, -1),
              ({"head_dim": 32}, -1), ({"head_dim": 96}, -1), ({"kv_type": 2}, -1), ({"kv_type": 1}, -1),
+             ({"kv_type": 1, "k_scale": 16, "v_scale": 8}, -2), ({"kv_type": 1, "k_scale": 4, "v_scale": 16}, -2),
              ({"num_pages": 1 << 26}, -1)]
 OWN = {
     "bitnet_paged_append": [({"cu_seqlens": None}, -1), ({"kv_lens": None}, -1), ({"qkv": None}, -1),

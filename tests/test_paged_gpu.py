@@ -12,9 +12,11 @@ Tolerances, derived from the arithmetic:
   exp2 of it, its sum and the rescaling add less than 2^-14.  A weight is off by
   half a step of its type: 2^-8 as one bf16 (more than 8 rows of a KV head), else
   2^-11 as f16 (int8 caches) or 2^-16 as a bf16 pair, so the bound is
-  2^-8 |o| + (2^-11 + weight) A.  f16 has a smallest step too, 2^-24: a weight
-  w_j = p_j vs_j is off by up to half of it at a scale where the largest is at
-  least 2^7, by 2^-32 max w, which its code c_j multiplies: + 2^-32 max w sum |c_j|.
+  2^-8 |o| + (2^-11 + weight) A.  (int8 and more than 8 rows: f16 weights and f16
+  values code * scale, three half steps of 2^-11, which is below 2^-8.)
+  f16 has a smallest step too, 2^-24: a weight w_j (p_j, or p_j vs_j with up to 8
+  rows) is off by up to half of it at a scale where the largest is at least 2^7, by
+  2^-32 max w, which its value v_j (or code c_j) multiplies: + 2^-32 max w sum |v_j|.
   (Where one key has nearly all the weight and its code is 0, that is all there is.)"""
 
 import pytest
@@ -271,9 +273,9 @@ def _attend_case(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, max_q=None, max_k
             want, spread = p @ vv[:, h // grp], p @ vv[:, h // grp].abs()
             err = (got[int(cu[b]):int(cu[b + 1]), h] - want).abs()
             room = want.abs() * 2.0 ** -8 + (2.0 ** -11 + weight) * spread
-            if dtype == I8 and m * grp <= 8 and k > 0:
-                codes = vv[:, h // grp].abs() / _scales(c, table, b, k)[:, h // grp, None]
-                room = room + 2.0 ** -32 * (p * _scales(c, table, b, k)[:, h // grp]).amax(-1, keepdim=True) * codes.sum(0)
+            if dtype == I8 and k > 0:
+                vs = _scales(c, table, b, k)[:, h // grp] if m * grp <= 8 else torch.ones(k)
+                room = room + 2.0 ** -32 * (p * vs).amax(-1, keepdim=True) * (vv[:, h // grp].abs() / vs[:, None]).sum(0)
             worst = float((err - room).max())
             assert worst <= 0, f"sequence {b} head {h}: {worst} over the bound"
 
