@@ -1312,6 +1312,16 @@ int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspa
   if (pl.chunk.blocks > 0) {
     using S = PchShape<D, I8>;
     auto k = paged_chunk_kernel<D, I8>;
+    if (I8) {  // the warpgroups' register shares are out of the launch's: fewer would wait for good
+      static std::atomic<int> regs{0};
+      if (regs.load() == 0) {
+        cudaFuncAttributes fa;
+        const cudaError_t e = cudaFuncGetAttributes(&fa, k);
+        if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes");
+        regs.store(fa.numRegs);
+      }
+      if (regs.load() != 128) return cuda_fail(cudaErrorInvalidConfiguration, "paged_chunk_kernel registers");
+    }
     if (int e = ensure_smem(k, &g_smem_pch[idx])) return e;
     CUtensorMap mk, mv;
     memset(&mk, 0, sizeof(mk));

@@ -44,11 +44,12 @@ struct PagedBlock {
   int kend;    // keys that the block's last row sees, not below 0
 };
 
-// Rows row0 .. of sequence b in a block of up to R rows.  False when the sequence
-// has no new token, or when its lengths do not hold.
+// Rows row0 .. of sequence b, which has n new tokens from packed row lo on and kv
+// keys, in a block of up to R rows.  False when there are none, or when the
+// lengths do not hold.
 template <int R>
-__device__ __forceinline__ bool paged_block_of(const PagedAttnParams& p, int b, int row0, int lane, PagedBlock& o) {
-  const int lo = p.cu[b], n = p.cu[b + 1] - lo, kv = p.kv_lens[b];
+__device__ __forceinline__ bool paged_block_of(const PagedAttnParams& p, int b, int lo, int n, int kv, int row0, int lane,
+                                               PagedBlock& o) {
   if (n == 0) return false;
   if (n < 0 || n > p.max_q || lo < 0 || lo > p.tokens - n || kv < 0 || kv > p.max_kv) {
     if (lane == 0) record_error(DEV_ERR_BOUNDS, 350);
@@ -69,9 +70,9 @@ __device__ __forceinline__ bool paged_block_of(const PagedAttnParams& p, int b, 
 template <int R>
 __device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
   const int b = bx / p.per, row0 = (bx - b * p.per) * R;
-  const long long rows = (long long)(p.cu[b + 1] - p.cu[b]) * p.G;
-  if (rows > p.most && (long long)p.max_q * p.G > p.most) return false;
-  return paged_block_of<R>(p, b, row0, lane, o);
+  const int lo = p.cu[b], n = p.cu[b + 1] - lo;
+  if ((long long)n * p.G > p.most && (long long)p.max_q * p.G > p.most) return false;
+  return paged_block_of<R>(p, b, lo, n, p.kv_lens[b], row0, lane, o);
 }
 
 // The R-row blocks of all sequences of more than p.small rows, numbered so that
@@ -84,12 +85,14 @@ __device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int
 template <int R>
 __device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
   if (p.B <= 32) {
-    int rows = 0, past = 0;
+    int at = 0, len = 0, kv = 0;
     if (lane < p.B) {
-      const int n = min(max(p.cu[lane + 1] - p.cu[lane], 0), p.max_q);
-      past = min(p.kv_lens[lane], p.max_kv) - n;
-      rows = n * p.G > p.small ? n * p.G : 0;
+      at = p.cu[lane];
+      len = p.cu[lane + 1] - at;
+      kv = p.kv_lens[lane];
     }
+    const int n = min(max(len, 0), p.max_q), past = min(kv, p.max_kv) - n;
+    const int rows = n * p.G > p.small ? n * p.G : 0;
     const int nb = (rows + R - 1) / R;
     // this sequence's blocks of at least t tiles: those whose last row's token is y or later
     auto count = [&](int t) {
@@ -118,7 +121,8 @@ __device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int
     const int src = __ffs(over) - 1;
     rank -= __shfl_sync(0xffffffffu, sum - here, src);
     const int last = __shfl_sync(0xffffffffu, nb - 1 - above, src);
-    return paged_block_of<R>(p, src, (last - rank) * R, lane, o);
+    return paged_block_of<R>(p, src, __shfl_sync(0xffffffffu, at, src), __shfl_sync(0xffffffffu, len, src),
+                             __shfl_sync(0xffffffffu, kv, src), (last - rank) * R, lane, o);
   }
   bx = p.blocks - 1 - bx;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -133,8 +137,9 @@ __device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int
     }
     const unsigned above = __ballot_sync(0xffffffffu, sum > bx);
     if (above) {
-      const int src = __ffs(above) - 1;
-      return paged_block_of<R>(p, b0 + src, (bx - __shfl_sync(0xffffffffu, sum - nb, src)) * R, lane, o);
+      const int src = __ffs(above) - 1, b = b0 + src;
+      return paged_block_of<R>(p, b, p.cu[b], p.cu[b + 1] - p.cu[b], p.kv_lens[b],
+                               (bx - __shfl_sync(0xffffffffu, sum - nb, src)) * R, lane, o);
     }
     bx -= __shfl_sync(0xffffffffu, sum, 31);
   }

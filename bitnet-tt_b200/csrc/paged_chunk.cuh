@@ -16,11 +16,11 @@
 // Roles, one warp each unless said otherwise:
 //   warps 0-3, 4-7   softmax of tile 0 and of tile 1: a thread owns a row (a lane of
 //                    tensor memory), so maxima and sums need no shuffles
-//   warps 8, 10      issue the MMAs of tile 0 and of tile 1: O_t of a step, then S_t of the step
+//   warps 8, 9       issue the MMAs of tile 0 and of tile 1: O_t of a step, then S_t of the step
 //                    after next.  Two, because the tensor cores queue few MMAs: a look at a
 //                    barrier costs the issuing warp about 100 cycles even when it is complete,
 //                    and with one warp those were gaps (980 cycles a tile and step for 640 of work)
-//   warp 9 (bf16)    loads K and V tiles by TMA, a box per page, into a ring of slots
+//   warp 10 (bf16)   loads K and V tiles by TMA, a box per page, into a ring of slots
 //   warps 12-15 (int8)  load codes and write them to the slots as f16
 // The softmax's maximum is lazy: O and the sum are rescaled only when a row's
 // maximum grew by more than 2^8, so weights reach at most 2^8 and the pass over
@@ -52,7 +52,7 @@ constexpr float PCH_GROWTH = 8.f;
 
 template <int D, bool I8>
 struct PchShape {
-  static constexpr int THREADS = I8 ? 512 : 384;
+  static constexpr int THREADS = I8 ? 512 : 352;
   static constexpr int TILE = 128 * D * 2;          // bytes of Q_t, K or V as bf16
   static constexpr int NSLOT = D == 64 ? 8 : (I8 ? 4 : 5);
   // int8: the keys' scales [RING tiles][128], then the rows' factors [256].  When the codes of
@@ -62,6 +62,9 @@ struct PchShape {
   static constexpr int EXTRA = I8 ? RING * 512 + 1024 : 0;
   // Weights are exp2(x - m + LIFT): with f16's range the smallest step is below 2^-31 of the largest.
   static constexpr float LIFT = I8 ? 7.f : 0.f;
+  // int8: registers a thread of the softmax, MMA and converting warpgroups, out of the launch's 128
+  static constexpr int REGS_SOFTMAX = 168, REGS_MMA = 56, REGS_CONVERT = 120;
+  static_assert(256 * REGS_SOFTMAX + 128 * REGS_MMA + 128 * REGS_CONVERT <= 512 * 128, "within the launch's");
   static constexpr int CTRL = 512;
   static constexpr int SMEM = 2 * TILE + NSLOT * TILE + EXTRA + CTRL;
 };
@@ -121,13 +124,21 @@ __device__ __forceinline__ uint32_t pow2_field(uint32_t bits, int k) { return 25
 struct PchCtrl {
   uint64_t full[PCH_MAX_SLOTS], empty[PCH_MAX_SLOTS];
   uint64_t s_full[2][2], p_ready[2][2];  // [row tile][step % 2]
-  uint64_t o_done[2][2], drain[2], tail; // o_done: O_t holds the step
+  uint64_t o_done[2][2], drain[2], tail, q_full, v_full;  // o_done: O_t holds the step
   uint32_t tmem;
   int abort_flag;
-  uint32_t v_top;  // int8: the largest value scale of the part, by its bits
+  uint32_t v_top[8];  // int8: the largest value scale of the part, by its bits, as each softmax warp saw it
 };
 static_assert(sizeof(PchCtrl) <= 512, "control block");
 
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
@@ -173,6 +184,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
+__device__ __forceinline__ uint32_t pch_v_top(const PchCtrl* c) {
+  uint32_t t = c->v_top[0];
+  for (int i = 1; i < 8; ++i) t = max(t, c->v_top[i]);
+  return t;
+}
+
 template <int D, bool I8>
 __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     paged_chunk_kernel(const PagedAttnParams p, const __grid_constant__ CUtensorMap map_k,
@@ -187,26 +204,11 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   PchCtrl* ctrl = reinterpret_cast<PchCtrl*>(sm_slots + S::NSLOT * S::TILE + S::EXTRA);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_trigger();
-  pdl_wait();
-  // the blocks with the most keys first
-  PagedBlock blk;
-  const int bx = p.blocks - 1 - (int)blockIdx.x;
-  if (!paged_block_search<PCH_R>(p, bx, lane, blk)) return;
-  const int g = blockIdx.y, sp = blockIdx.z;
-  const int nparts = paged_parts(p, blk.kend);
-  if (sp >= nparts) return;
-  const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);
-  // 64-key steps of the two row tiles (the second sees at least the first's keys)
-  const int end0 = min(k1, max(0, blk.past + (blk.row0 + min(blk.nrows, 128) - 1) / p.G + 1));
-  const int n0 = max(0, (end0 - k0 + PCH_STEP - 1) / PCH_STEP);
-  const int n1 = blk.nrows > 128 ? max(0, (k1 - k0 + PCH_STEP - 1) / PCH_STEP) : 0;
-  const int nstep = max(n0, n1), ntile = (nstep + 1) / 2;
-
   volatile int* abort_flag = &ctrl->abort_flag;
   if (tid == 0) {
     for (int s = 0; s < S::NSLOT; ++s) {
       mbar_init(&ctrl->full[s], I8 ? 4 : 1);
-      mbar_init(&ctrl->empty[s], n1 > 0 ? 2 : 1);
+      mbar_init(&ctrl->empty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
       for (int h = 0; h < 2; ++h) {
@@ -217,63 +219,34 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       mbar_init(&ctrl->drain[t], 1);
     }
     mbar_init(&ctrl->tail, 1);
+    mbar_init(&ctrl->q_full, 8);
+    mbar_init(&ctrl->v_full, 8);
     ctrl->abort_flag = 0;
-    ctrl->v_top = 0;
     fence_mbar_init();
   }
+  pdl_wait();
+  // Only now: the kernel before this one may need tensor memory to end.
   if (warp == 8) {
     tmem_alloc(&ctrl->tmem, 512);
     tmem_relinquish();
   }
-  if (I8) __syncthreads();
-  // Q, 16 bytes at a time, into the swizzled tiles (rows past the block: zeros)
-  for (int i = tid; i < 2 * 128 * (D / 8); i += S::THREADS) {
-    const int r = i / (D / 8), c = i % (D / 8);
-    if (r >= 128 && blk.nrows <= 128) break;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (r < blk.nrows) {
-      const int row = blk.row0 + r, tok = row / p.G;
-      w = *reinterpret_cast<const uint4*>(p.q + (size_t)(blk.tok0 + tok) * p.ld_q +
-                                          (size_t)(g * p.G + row - tok * p.G) * D + c * 8);
-    }
-    if (I8) {  // D / 8 neighbouring lanes hold a row: its largest value goes to 2^13 .. 2^14
-      float x[8];
-      unpack_bf8(w, x);
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = D / 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const uint32_t field = pow2_field(top, 13);
-      const float f = __uint_as_float(field << 23);
-      w = make_uint4(f16x2_of(x[0] * f, x[2] * f), f16x2_of(x[1] * f, x[3] * f), f16x2_of(x[4] * f, x[6] * f),
-                     f16x2_of(x[5] * f, x[7] * f));
-      if (c == 0) sm_fac[r] = __uint_as_float((254u - field) << 23);
-    }
-    const int rr = r & 127;
-    *reinterpret_cast<uint4*>(sm_q + (r >> 7) * S::TILE + (c >> 3) * HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = w;
-  }
-  if (I8) {  // the largest value scale of the part's rows, four rows (of one page) a load
-    const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
-    float top = 0.f;
-#pragma unroll 4
-    for (int key = k0 + 4 * tid; key < k1; key += 4 * S::THREADS) {
-      const int page = table[key >> p.kv.page_shift];
-      if (page < 0 || page >= p.kv.num_pages) continue;  // reported by the loads below
-      const float4 v = *reinterpret_cast<const float4*>(
-          p.kv.vs + paged_row(p.kv, page, g, key & ((1 << p.kv.page_shift) - 1)));
-      top = fmaxf(top, v.x);
-      if (key + 1 < k1) top = fmaxf(top, v.y);
-      if (key + 2 < k1) top = fmaxf(top, v.z);
-      if (key + 3 < k1) top = fmaxf(top, v.w);
-    }
-    const uint32_t t = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-    if (lane == 0) atomicMax(&ctrl->v_top, t);
-  }
-  fence_proxy_async_smem();
+  const int bx = blockIdx.x, g = blockIdx.y, sp = blockIdx.z;
+  PagedBlock blk;
+  const bool found = paged_block_search<PCH_R>(p, bx, lane, blk);
+  const int nparts = found ? paged_parts(p, blk.kend) : 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (sp >= nparts) {
+    if (warp == 8) tmem_dealloc(0, 512);
+    return;
+  }
+  const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);
+  // 64-key steps of the two row tiles (the second sees at least the first's keys)
+  const int end0 = min(k1, max(0, blk.past + (blk.row0 + min(blk.nrows, 128) - 1) / p.G + 1));
+  const int n0 = max(0, (end0 - k0 + PCH_STEP - 1) / PCH_STEP);
+  const int n1 = blk.nrows > 128 ? max(0, (k1 - k0 + PCH_STEP - 1) / PCH_STEP) : 0;
+  const int nstep = max(n0, n1), ntile = (nstep + 1) / 2;
   // All 512 columns are this CTA's, so they start at 0: a constant, as the MMAs' operands
   // should be (below).
   constexpr uint32_t tbase = 0;
@@ -288,9 +261,10 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     return true;
   };
 
-  if (warp >= 12) {
+  if (I8 && warp >= 12) {
     // ---------------- int8: codes to f16 slots ----------------
     if constexpr (I8) {
+      regs_dec<S::REGS_CONVERT>();
       constexpr int NL = D / 16;  // 16-byte loads of a lane: 32 rows of a warp
       const int w = warp - 12;
       const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
@@ -366,7 +340,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctrl->full[it % S::NSLOT]);
       };
-      const float v_up = __uint_as_float(pow2_field(ctrl->v_top, 7) << 23);
+      float v_up = 0.f;
       uint4 bk[NL], bv[NL];
       look_up(0);
       load(0, p.kv.k, bk);
@@ -385,13 +359,18 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         sm_scale[(j % S::RING) * 128 + 32 * w + lane] = ks;
         arrive(2 * j);
         load(j + 1, p.kv.k, bk);
+        if (j == 0) {
+          if (!__all_sync(0xffffffffu, wait(&ctrl->v_full, 0, 376))) break;
+          v_up = __uint_as_float(pow2_field(pch_v_top(ctrl), 7) << 23);
+        }
         if (!convert(2 * j + 1, bv, f16x2_of(vs * v_up, vs * v_up))) break;
         arrive(2 * j + 1);
       }
     }
   } else if (warp >= 8) {
+    if constexpr (I8) regs_dec<S::REGS_MMA>();
     const int t = warp == 8 ? 0 : 1, nt = t ? n1 : n0;
-    if ((warp == 8 && nstep > 0) || (warp == 10 && n1 > 0)) {
+    if (warp < 10 && nstep > 0) {
       // ---------------- MMA issuers ----------------
       constexpr uint32_t f16_types = (1u << 7) | (1u << 10);  // set: bf16, clear: f16
       constexpr uint32_t idesc_s = idesc_bf16_f32(128, PCH_STEP) & (I8 ? ~f16_types : ~0u);
@@ -422,7 +401,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       };
       auto filled = [&](int it, int site) { return arrived(&ctrl->full[it % S::NSLOT], (it / S::NSLOT) & 1, site); };
       // Each issuer releases every slot, those past its own tile's keys too.
-      bool ok = filled(0, 363);
+      bool ok = filled(0, 363) && arrived(&ctrl->q_full, 0, 375);
       if (ok && elect_one()) {
         if (nt > 0) qk(0, 0);
         if (nt > 1) qk(0, 1);
@@ -450,7 +429,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         __syncwarp();
         mbar_wait(&ctrl->drain[t], 0, 367);
       }
-    } else if (!I8 && warp == 9) {
+    } else if (!I8 && warp == 10) {
       // ---------------- bf16: TMA loads ----------------
       const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
       const int box = min(1 << p.kv.page_shift, PCH_KB);  // rows of a box: the map's
@@ -508,7 +487,68 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       }
     }
   } else {
-    // ---------------- softmax: a thread owns a row ----------------
+    // ---------------- softmax: a thread owns a row (and the eight warps load Q first) ----------------
+    if constexpr (I8) regs_inc<S::REGS_SOFTMAX>();
+    // Q, 16 bytes at a time, into the swizzled tiles (rows past the block: zeros)
+    constexpr int NQ = D / 16;  // loads in flight
+#pragma unroll 1
+    for (int half = 0; half < (blk.nrows > 128 ? 2 : 1); ++half) {
+      uint4 w[NQ];
+#pragma unroll
+      for (int u = 0; u < NQ; ++u) {
+        const int i = tid + 256 * (half * NQ + u), r = i / (D / 8), c = i % (D / 8);
+        w[u] = make_uint4(0, 0, 0, 0);
+        if (r < blk.nrows) {
+          const int row = blk.row0 + r, tok = row / p.G;
+          w[u] = *reinterpret_cast<const uint4*>(p.q + (size_t)(blk.tok0 + tok) * p.ld_q +
+                                                 (size_t)(g * p.G + row - tok * p.G) * D + c * 8);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NQ; ++u) {
+        const int i = tid + 256 * (half * NQ + u), r = i / (D / 8), c = i % (D / 8), rr = r & 127;
+        if (I8) {  // D / 8 neighbouring lanes hold a row: its largest value goes to 2^13 .. 2^14
+          float x[8];
+          unpack_bf8(w[u], x);
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+#pragma unroll
+          for (int o = D / 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const uint32_t field = pow2_field(top, 13);
+          const float f = __uint_as_float(field << 23);
+          w[u] = make_uint4(f16x2_of(x[0] * f, x[2] * f), f16x2_of(x[1] * f, x[3] * f), f16x2_of(x[4] * f, x[6] * f),
+                            f16x2_of(x[5] * f, x[7] * f));
+          if (c == 0) sm_fac[r] = __uint_as_float((254u - field) << 23);
+        }
+        *reinterpret_cast<uint4*>(sm_q + (r >> 7) * S::TILE + (c >> 3) * HALF + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = w[u];
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctrl->q_full);
+    if (I8) {  // the largest value scale of the part's rows, four rows (of one page) a load
+      const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
+      float top = 0.f;
+#pragma unroll 4
+      for (int key = k0 + 4 * tid; key < k1; key += 1024) {
+        const int page = table[key >> p.kv.page_shift];
+        if (page < 0 || page >= p.kv.num_pages) continue;  // reported by the loads of the rows
+        const float4 v = *reinterpret_cast<const float4*>(
+            p.kv.vs + paged_row(p.kv, page, g, key & ((1 << p.kv.page_shift) - 1)));
+        top = fmaxf(top, v.x);
+        if (key + 1 < k1) top = fmaxf(top, v.y);
+        if (key + 2 < k1) top = fmaxf(top, v.z);
+        if (key + 3 < k1) top = fmaxf(top, v.w);
+      }
+      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+      if (lane == 0) {
+        ctrl->v_top[warp] = most;
+        mbar_arrive(&ctrl->v_full);
+      }
+      // sm_fac is read across warps
+      named_bar_sync(1, 256);
+    }
     const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane;
     const int nt = t ? n1 : n0;
     const bool live = r < blk.nrows;
@@ -621,7 +661,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       const size_t pr = (((size_t)sp * p.blocks + bx) * p.kv.n_kv + g) * PCH_R + r;
       if (live && nparts > 1) p.part_ml[pr] = make_float2(m - S::LIFT, l);
-      const float vf = I8 ? __uint_as_float((254u - pow2_field(ctrl->v_top, 7)) << 23) : 1.f;  // the values' power of two
+      if (I8) wait(&ctrl->v_full, 0, 377);  // complete: every warp arrived before the barrier above
+      const float vf = I8 ? __uint_as_float((254u - pow2_field(pch_v_top(ctrl), 7)) << 23) : 1.f;  // the values' power of two
       uint16_t* dst = p.out + ((size_t)(blk.tok0 + tok) * p.n_heads + g * p.G + row - tok * p.G) * D;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
