@@ -1295,12 +1295,11 @@ int launch_paged_join(const PagedAttnParams& p, bitnet_stream_t st) {
 }
 
 template <int D, bool I8, int H>
-int launch_paged_rows(PagedAttnParams p, bitnet_stream_t st) {
+int launch_paged_rows(const PagedAttnParams& p, bitnet_stream_t st) {
   using S = PraShape<D, I8, H>;
   auto k = paged_rows_kernel<D, I8, H>;
   if (int e = ensure_smem(k, &g_smem_pra[((D == 128) * 2 + I8) * 2 + H - 1])) return e;
-  if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(PRA_THREADS), S::SMEM, st, 1, p)) return e;
-  return launch_paged_join<D, S::R, 4>(p, st);
+  return launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(PRA_THREADS), S::SMEM, st, 1, p);
 }
 
 template <int D, bool I8>
@@ -1332,12 +1331,17 @@ int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspa
     }
     paged_apply(&p, pl.chunk, workspace);
     if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(S::THREADS), S::SMEM, st, 1, p, mk, mv)) return e;
-    if (int e = launch_paged_join<D, PCH_R, 1>(p, st)) return e;
   }
+  PagedAttnParams pr = p;
   if (pl.rows.blocks > 0) {
-    paged_apply(&p, pl.rows, workspace);
-    return pl.r == 8 ? launch_paged_rows<D, I8, 1>(p, st) : launch_paged_rows<D, I8, 2>(p, st);
+    paged_apply(&pr, pl.rows, workspace);
+    pr.beside = pl.chunk.blocks > 0;
+    if (int e = pl.r == 8 ? launch_paged_rows<D, I8, 1>(pr, st) : launch_paged_rows<D, I8, 2>(pr, st)) return e;
   }
+  if (pl.chunk.blocks > 0)
+    if (int e = launch_paged_join<D, PCH_R, 1>(p, st)) return e;
+  if (pl.rows.blocks > 0)
+    return pl.r == 8 ? launch_paged_join<D, 8, 4>(pr, st) : launch_paged_join<D, 16, 4>(pr, st);
   return BITNET_OK;
 }
 

@@ -31,6 +31,7 @@ struct PagedAttnParams {
   int blocks;          // grid.x: row blocks, an upper bound
   int small;           // chunk kernel: sequences of up to this many rows are not its own
   int most, per;       // rows kernel: rows of its longest sequences, and blocks of each
+  int beside;          // rows kernel: launched after the chunk kernel, to run beside it
   float2* part_ml;     // [nsplit][blocks][n_kv][R] (maximum, sum)
   float* part_o;       // [nsplit][blocks][n_kv][R][D], unnormalised
   uint16_t* out;       // [tokens][n_heads * D]
@@ -80,49 +81,72 @@ __device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int
 // not end last); whole warp.  Blocks are ranked by their 128-key tiles: the rank
 // of block bx is found by bisection over the number of tiles, counting the blocks
 // with at least that many by arithmetic (a sequence's later blocks see more).
-// Equal ranks are in the order of sequences.  Up to 32 sequences; beyond that the
+// Equal ranks are in the order of sequences.  Up to 128 sequences; beyond that the
 // blocks are in the order of sequences alone, the last first.
 template <int R>
 __device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
-  if (p.B <= 32) {
-    int at = 0, len = 0, kv = 0;
-    if (lane < p.B) {
-      at = p.cu[lane];
-      len = p.cu[lane + 1] - at;
-      kv = p.kv_lens[lane];
+  constexpr int C = 4;  // sequences of a lane
+  if (p.B <= 32 * C) {
+    int at[C], len[C], kv[C], rows[C], past[C], nb = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int b = 32 * c + lane;
+      at[c] = len[c] = kv[c] = rows[c] = past[c] = 0;
+      if (b < p.B) {
+        at[c] = p.cu[b];
+        len[c] = p.cu[b + 1] - at[c];
+        kv[c] = p.kv_lens[b];
+        const int n = min(max(len[c], 0), p.max_q);
+        past[c] = min(kv[c], p.max_kv) - n;
+        rows[c] = n * p.G > p.small ? n * p.G : 0;
+        nb += (rows[c] + R - 1) / R;
+      }
     }
-    const int n = min(max(len, 0), p.max_q), past = min(kv, p.max_kv) - n;
-    const int rows = n * p.G > p.small ? n * p.G : 0;
-    const int nb = (rows + R - 1) / R;
-    // this sequence's blocks of at least t tiles: those whose last row's token is y or later
-    auto count = [&](int t) {
-      const long long y = (long long)(t - 1) * 128 - past;
-      if (t <= 0 || y <= 0 || nb == 0) return nb;
+    // the blocks of at least t tiles of sequence c: those whose last row's token is y or later
+    auto count = [&](int c, int t) {
+      const int all = (rows[c] + R - 1) / R;
+      const long long y = (long long)(t - 1) * 128 - past[c];
+      if (t <= 0 || y <= 0 || all == 0) return all;
       const long long first = y * p.G;  // the first row of token y
-      return first >= rows ? 0 : nb - (int)(first / R);
+      return first >= rows[c] ? 0 : all - (int)(first / R);
+    };
+    auto total = [&](int t) {
+      int n = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (32 * c < p.B) n += count(c, t);
+      return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
     };
     if (bx >= (int)__reduce_add_sync(0xffffffffu, (unsigned)nb)) return false;
     int lo = 0, hi = (p.max_kv + 127) / 128 + 1;  // more than bx blocks have lo tiles, not more have hi
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if ((int)__reduce_add_sync(0xffffffffu, (unsigned)count(mid)) > bx) lo = mid;
+      if (total(mid) > bx) lo = mid;
       else hi = mid;
     }
     // among the blocks of exactly lo tiles
-    const int above = count(lo + 1), here = count(lo) - above;
-    int rank = bx - (int)__reduce_add_sync(0xffffffffu, (unsigned)above), sum = here;
+    int rank = bx - total(lo + 1);
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += v;
+    for (int c = 0; c < C; ++c) {
+      if (32 * c >= p.B) break;
+      const int above = count(c, lo + 1), here = count(c, lo) - above;
+      int sum = here;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += v;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, sum > rank);
+      if (over) {
+        const int src = __ffs(over) - 1;
+        rank -= __shfl_sync(0xffffffffu, sum - here, src);
+        const int last = __shfl_sync(0xffffffffu, (rows[c] + R - 1) / R - 1 - above, src);
+        return paged_block_of<R>(p, 32 * c + src, __shfl_sync(0xffffffffu, at[c], src), __shfl_sync(0xffffffffu, len[c], src),
+                                 __shfl_sync(0xffffffffu, kv[c], src), (last - rank) * R, lane, o);
+      }
+      rank -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    const unsigned over = __ballot_sync(0xffffffffu, sum > rank);
-    if (!over) return false;
-    const int src = __ffs(over) - 1;
-    rank -= __shfl_sync(0xffffffffu, sum - here, src);
-    const int last = __shfl_sync(0xffffffffu, nb - 1 - above, src);
-    return paged_block_of<R>(p, src, __shfl_sync(0xffffffffu, at, src), __shfl_sync(0xffffffffu, len, src),
-                             __shfl_sync(0xffffffffu, kv, src), (last - rank) * R, lane, o);
+    return false;
   }
   bx = p.blocks - 1 - bx;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -272,12 +296,19 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
   extern __shared__ __align__(128) uint8_t smem_pra[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
-  pdl_wait();
-  PagedBlock blk;
-  if (!paged_block_direct<S::R>(p, blockIdx.x, lane, blk)) return;
   const int g = blockIdx.y, sp = blockIdx.z;
-  const int nparts = paged_parts(p, blk.kend);
-  if (sp >= nparts) return;
+  // Beside the chunk kernel there is nothing to wait for: its CTAs allow this launch only after
+  // their own wait for what came before.  The last CTA waits for the chunk kernel before it ends,
+  // so that what follows this kernel follows both.
+  if (!p.beside) pdl_wait();
+  const bool closes = p.beside && blockIdx.x == gridDim.x - 1 && g == (int)gridDim.y - 1 && sp == (int)gridDim.z - 1;
+  PagedBlock blk;
+  const bool found = paged_block_direct<S::R>(p, blockIdx.x, lane, blk);
+  const int nparts = found ? paged_parts(p, blk.kend) : 0;
+  if (sp >= nparts) {
+    if (closes) pdl_wait();
+    return;
+  }
   const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);  // this part's keys
   const int ntiles = max(0, (k1 - k0 + KT - 1) / KT);
   const int ntw = ntiles > warp ? (ntiles - warp + PRA_WARPS - 1) / PRA_WARPS : 0;
@@ -644,6 +675,7 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
       *reinterpret_cast<float4*>(p.part_o + (pb * S::R + r) * D + d) = num;
     }
   }
+  if (closes) pdl_wait();
 }
 
 // ---------------------------------------------------------------------------

@@ -203,7 +203,6 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   float* sm_fac = sm_scale + S::RING * 128;
   PchCtrl* ctrl = reinterpret_cast<PchCtrl*>(sm_slots + S::NSLOT * S::TILE + S::EXTRA);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_trigger();
   volatile int* abort_flag = &ctrl->abort_flag;
   if (tid == 0) {
     for (int s = 0; s < S::NSLOT; ++s) {
@@ -225,6 +224,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     fence_mbar_init();
   }
   pdl_wait();
+  pdl_trigger();  // after the wait: the rows kernel may then start without one of its own
   // Only now: the kernel before this one may need tensor memory to end.
   if (warp == 8) {
     tmem_alloc(&ctrl->tmem, 512);
