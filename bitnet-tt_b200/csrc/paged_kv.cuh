@@ -59,6 +59,21 @@ __device__ __forceinline__ uint4 pack_bf8(const float (&x)[8]) {
   return make_uint4(bf2_of(x[0], x[1]), bf2_of(x[2], x[3]), bf2_of(x[4], x[5]), bf2_of(x[6], x[7]));
 }
 
+// Four codes of a word as fp32 values, and four fp32 values of at most 127.49 as
+// codes (half to even), without the conversion unit, which handles 16 values a
+// cycle and SM: fp32 0x4B0000uu is 2^23 + u, and v + 1.5 * 2^23 holds rint(v) in its
+// low byte.
+__device__ __forceinline__ void codes_to_f32(uint32_t w, float* x) {
+  w ^= 0x80808080u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = __fsub_rn(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 + e)), 8388736.f);
+}
+__device__ __forceinline__ uint32_t codes_of_f32(float a, float b, float c, float d) {
+  const uint32_t m0 = __float_as_uint(__fadd_rn(a, 12582912.f)), m1 = __float_as_uint(__fadd_rn(b, 12582912.f));
+  const uint32_t m2 = __float_as_uint(__fadd_rn(c, 12582912.f)), m3 = __float_as_uint(__fadd_rn(d, 12582912.f));
+  return __byte_perm(__byte_perm(m0, m1, 0x0040), __byte_perm(m2, m3, 0x0040), 0x5410);
+}
+
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
@@ -78,7 +93,9 @@ __device__ __forceinline__ uint4 pack_bf8(const float (&x)[8]) {
 // Bound: memory.  D/16 lanes take one head of one token, each the two 16-byte
 // chunks that hold eight pairs (or two chunks of the dims that only move), so a
 // rotation needs no shuffle and reads each table entry once; the row's maximum
-// is a short shuffle tree.  Two heads a lane are loaded before the first is worked on.
+// is a short shuffle tree.  In bf16 two heads a lane are loaded before the first is
+// worked on (one in int8, whose work needs the registers).  B200: 32 x 512 tokens,
+// 20 + 2 x 5 heads of 128, 47.3 us, 5.3 TB/s.
 struct PagedAppendParams {
   PagedKV kv;
   const int32_t* cu;       // [B + 1] token offsets
@@ -116,10 +133,10 @@ __device__ __forceinline__ void append_chunks(int l, int rot, bool interleaved, 
 }
 
 template <int D, bool I8, bool F32>
-__global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAppendParams p) {
+__global__ void __launch_bounds__(PKV_THREADS, 4) paged_append_kernel(const PagedAppendParams p) {
   constexpr int LPH = D / 16;                 // lanes of one head
   constexpr int GROUPS = PKV_THREADS / LPH;   // heads at once
-  constexpr int U = 2;                        // heads of a lane in flight
+  constexpr int U = I8 ? 1 : 3;                        // heads of a lane in flight
   __shared__ int s_pos[8], s_page[8];
   pdl_trigger();
   pdl_wait();
@@ -204,7 +221,7 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAp
       const int g = is_q ? 0 : (is_v ? hh - p.n_heads - p.kv.n_kv : hh - p.n_heads);
       const size_t row = live ? paged_row(p.kv, s_page[t], g, pos & ((1 << p.kv.page_shift) - 1)) : 0;
       uint8_t* pool = is_v ? p.kv.v : p.kv.k;
-      if (I8) {
+      if (I8 && __any_sync(0xffffffffu, live && !is_q)) {
         uint32_t top = 0;  // the largest |x| by its bits: a NaN or an infinity wins
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -214,14 +231,15 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAp
         if (live && !is_q) {
           const bool finite = top < 0x7f800000u;
           const float amax = fmaxf(__uint_as_float(top), 1e-5f), inv = __fdiv_rn(127.f, amax);
-          uint32_t q[4] = {0, 0, 0, 0};
+          uint32_t q[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int a = finite ? __float2int_rn(__fmul_rn(x[e], inv)) : 0;
-            const int b = finite ? __float2int_rn(__fmul_rn(y[e], inv)) : 0;
-            q[e >> 2] |= (uint32_t)(a & 0xff) << (8 * (e & 3));
-            q[2 + (e >> 2)] |= (uint32_t)(b & 0xff) << (8 * (e & 3));
+          for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], inv), y[e] = __fmul_rn(y[e], inv);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            q[e] = codes_of_f32(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+            q[2 + e] = codes_of_f32(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
           }
+          if (!finite) q[0] = q[1] = q[2] = q[3] = 0;
           *reinterpret_cast<uint2*>(pool + row * D + c0 * 8) = make_uint2(q[0], q[1]);
           *reinterpret_cast<uint2*>(pool + row * D + c1 * 8) = make_uint2(q[2], q[3]);
           if (tid % LPH == 0)
@@ -243,7 +261,10 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_append_kernel(const PagedAp
 // Row r of sequence b's packed rows (cu[b] .. cu[b + 1] - 1) is cache row
 // starts[b] + r - cu[b]; k_out / v_out are bf16 [rows][n_kv][D].  int8: the value
 // bf16(code * scale), rounded once.  Bound: memory, one pass; a lane moves 16 bytes
-// of a row, four rows' worth in flight.
+// of two rows at a time, neighbours in a page side by side.  Eight rows a CTA and
+// six CTAs an SM: the look-ups before the first load hide behind other CTAs (16
+// rows and four loads in flight took 31.5 us where this takes 29.0, 4.6 TB/s, for 16
+// ragged int8 contexts of up to 4096 rows).
 struct PagedReadParams {
   PagedKV kv;
   const int32_t* cu;
@@ -252,13 +273,13 @@ struct PagedReadParams {
   uint16_t* k_out;
   uint16_t* v_out;
 };
-constexpr int PKV_READ_ROWS = 16;
+constexpr int PKV_READ_ROWS = 8;
 
 template <int D, bool I8>
-__global__ void __launch_bounds__(PKV_THREADS) paged_read_kernel(const PagedReadParams p) {
+__global__ void __launch_bounds__(PKV_THREADS, 7) paged_read_kernel(const PagedReadParams p) {
   constexpr int LPH = D / (I8 ? 16 : 8);  // lanes of a row, 16 bytes each
   constexpr int GROUPS = PKV_THREADS / LPH;
-  constexpr int U = 4;
+  constexpr int U = 2;
   __shared__ int s_slot[PKV_READ_ROWS], s_page[PKV_READ_ROWS];
   pdl_trigger();
   pdl_wait();
@@ -297,7 +318,7 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_read_kernel(const PagedRead
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int it = it0 + u * GROUPS;
-      const int t = it < items ? it / per_row : 0, h = it - t * per_row;
+      const int h = it < items ? it / nrow : 0, t = it - h * nrow;  // neighbours in a page side by side
       dst[u] = nullptr;
       if (it < items && s_page[t] >= 0) {
         const bool is_v = h >= p.kv.n_kv;
@@ -316,8 +337,10 @@ __global__ void __launch_bounds__(PKV_THREADS) paged_read_kernel(const PagedRead
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float x[8];
+          codes_to_f32(c[2 * h], x);
+          codes_to_f32(c[2 * h + 1], x + 4);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = __fmul_rn((float)(int8_t)(c[2 * h + (e >> 2)] >> (8 * (e & 3))), sc[u]);
+          for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], sc[u]);
           *reinterpret_cast<uint4*>(dst[u] + l * 16 + h * 8) = pack_bf8(x);
         }
       } else {
