@@ -180,7 +180,7 @@ _SIGNATURES = {
                  _c_void_p, _c_void_p]),
     "bitnet_paged_append": (
         _c_int, [ctypes.POINTER(PagedKV), _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
-                 _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p]),
+                 _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_void_p]),
     "bitnet_paged_read": (
         _c_int, [ctypes.POINTER(PagedKV), _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p,
                  _c_void_p]),
@@ -545,13 +545,13 @@ def attention_prefill_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
 # looked up once.  index: the device of the cache, which must be current.
 def paged_append(kv: PagedKV, index: int, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
                  qkv: torch.Tensor, n_heads: int, rope_cos: torch.Tensor, rope_sin: torch.Tensor, q_out: torch.Tensor,
-                 interleaved: bool = False) -> None:
+                 interleaved: bool = False, stepwise: bool = False) -> None:
     b, max_pages = block_table.shape
     rope_len, half = rope_cos.shape
     st = (_lib or load()).bitnet_paged_append(
         kv, block_table.data_ptr(), b, max_pages, cu_seqlens.data_ptr(), kv_lens.data_ptr(), qkv.data_ptr(),
         qkv.stride(0), qkv.shape[0], n_heads, rope_cos.data_ptr(), rope_sin.data_ptr(), rope_len, 2 * half,
-        rope_cos.dtype is torch.float32, interleaved, q_out.data_ptr(), raw_stream(index))
+        rope_cos.dtype is torch.float32, interleaved, stepwise, q_out.data_ptr(), raw_stream(index))
     if st:
         check(st, "bitnet_paged_append")
 

@@ -16,6 +16,7 @@ import torch
 
 from .. import _lib
 from .bitlinear import Linear, RMSNorm, quantize_and_transpose_weight, quantize_ternary
+from .paged_kv import PagedBatch, PagedKVCache
 
 
 def _permute_halfsplit_to_adjacent(weight_t: np.ndarray, num_heads: int, head_dim: int) -> np.ndarray:
@@ -133,5 +134,18 @@ class MultiHeadAttention:
         qkv = self.qkv_proj(hidden_states, norm_weight=norm_weight, norm_epsilon=norm_epsilon)
         attn = torch.empty((qkv.shape[0], self.num_heads * self.head_dim), dtype=torch.bfloat16, device=qkv.device)
         self.decode_attention(qkv, positions, rope[0], rope[1], cache, attn)
+        return self.o_proj(attn, norm_weight=self.attn_sub_norm.weight, norm_epsilon=self.attn_sub_norm.eps,
+                           residual=residual)
+
+    def forward_paged(self, hidden_states: torch.Tensor, batch: PagedBatch, rope: tuple[torch.Tensor, torch.Tensor],
+                      cache: PagedKVCache, norm_weight: torch.Tensor | None = None, norm_epsilon: float = 1e-5,
+                      residual: torch.Tensor | None = None) -> torch.Tensor:
+        """Forward of [tokens, hidden], any number of new tokens per sequence, over a
+        paged cache (head_dim 64 or 128, bf16 or int8 pages).  bf16 rows are those of
+        the contiguous cache, bit for bit."""
+        qkv = self.qkv_proj(hidden_states, norm_weight=norm_weight, norm_epsilon=norm_epsilon)
+        q = cache.append(qkv, batch.cu_seqlens, batch.kv_lens, batch.block_table, rope[0], rope[1], stepwise=True)
+        attn = cache.attend(q, batch.cu_seqlens, batch.kv_lens, batch.block_table, batch.max_seqlen, batch.max_kv_len,
+                            self.scale)
         return self.o_proj(attn, norm_weight=self.attn_sub_norm.weight, norm_epsilon=self.attn_sub_norm.eps,
                            residual=residual)

@@ -20,12 +20,36 @@ lengths live on the device, where a bad one is recorded
 from __future__ import annotations
 
 import functools
+from dataclasses import dataclass
 
 import torch
 
 from .. import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+@dataclass
+class PagedBatch:
+    """The new tokens of one forward pass over paged caches: one per sequence of a
+    decode step, any number elsewhere."""
+
+    cu_seqlens: torch.Tensor   # int32 [B + 1]
+    kv_lens: torch.Tensor      # int32 [B], the new tokens included
+    block_table: torch.Tensor  # int32 [B, max_pages]
+    max_seqlen: int
+    max_kv_len: int
+
+    @classmethod
+    def of(cls, new_tokens: list[int], kv_lens: list[int], pages: list[list[int]], device) -> "PagedBatch":
+        """From host lists: new tokens, keys after them, and pages of every sequence."""
+        width = max(1, max(len(x) for x in pages))
+        table = torch.full((len(pages), width), -1, dtype=torch.int32)
+        for b, x in enumerate(pages):
+            table[b, : len(x)] = torch.tensor(x, dtype=torch.int32)
+        cu = torch.tensor([0, *new_tokens], dtype=torch.int32).cumsum(0, dtype=torch.int32)
+        return cls(cu.to(device), torch.tensor(kv_lens, dtype=torch.int32).to(device), table.to(device),
+                   max(new_tokens), max(kv_lens))
 
 
 def _want(ok: bool, what: str) -> None:
@@ -125,12 +149,14 @@ class PagedKVCache:
     # ---- calls -------------------------------------------------------------
     def append(self, qkv: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
                rope_cos: torch.Tensor, rope_sin: torch.Tensor, q_out: torch.Tensor | None = None,
-               interleaved: bool = False) -> torch.Tensor:
+               interleaved: bool = False, stepwise: bool = False) -> torch.Tensor:
         """Rotates the new tokens' queries and keys (qkv rows [tokens, (n_heads +
         2 n_kv) * head_dim], which may be strided), writes keys and values to their
         pages and returns the queries [tokens, n_heads * head_dim].  Token i of n
         stands at position kv_lens[b] - n + i.  rope tables: bf16 or fp32 [positions,
-        rotary_dim / 2]; rotary_dim may be less than head_dim."""
+        rotary_dim / 2]; rotary_dim may be less than head_dim.  The rotation is
+        rounded once; stepwise rounds its products and sums to bf16 too, as the bf16
+        model code and the contiguous cache's kernels do."""
         n = kv_lens.numel()
         if not (self._index_ok(block_table) and self._index_ok(cu_seqlens) and self._index_ok(kv_lens)
                 and block_table.dim() == 2 and block_table.shape[0] == n and cu_seqlens.numel() == n + 1 and n):
@@ -145,7 +171,8 @@ class PagedKVCache:
                 and rope_sin.get_device() == self._index and rope_cos.is_contiguous() and rope_sin.is_contiguous()):
             raise ValueError("rope tables must be two equal contiguous bf16 or fp32 [positions, rotary_dim / 2]")
         q_out = self._out(q_out, (tokens, heads * self.head_dim), "q_out")
-        self._launch(_lib.paged_append, block_table, cu_seqlens, kv_lens, qkv, heads, rope_cos, rope_sin, q_out, interleaved)
+        self._launch(_lib.paged_append, block_table, cu_seqlens, kv_lens, qkv, heads, rope_cos, rope_sin, q_out, interleaved,
+                     stepwise)
         return q_out
 
     def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,

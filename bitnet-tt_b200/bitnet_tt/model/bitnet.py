@@ -14,6 +14,7 @@ from .. import _lib
 from ..config import BitNetConfig
 from ..layers.bitlinear import RMSNorm
 from ..layers.embedding import Embedding
+from ..layers.paged_kv import PagedBatch, PagedKVCache
 from .transformer import TransformerBlock
 
 
@@ -63,6 +64,33 @@ class BitNetModel:
         logits = (torch.empty((b, self.config.vocab_size), dtype=torch.bfloat16, device=self.device)
                   if return_logits else None)
         self.lm_head_argmax(normed, ws, nxt, logits)
+        return nxt, logits
+
+    # ---- forward over paged caches -------------------------------------------
+    def paged_caches(self, num_pages: int, page_size: int = 64, dtype: torch.dtype = torch.bfloat16) -> list[PagedKVCache]:
+        """One cache per layer; a block table's page ids hold for all of them."""
+        c = self.config
+        return [PagedKVCache(num_pages, page_size, c.num_key_value_heads, c.head_dim, self.device, dtype)
+                for _ in range(c.num_layers)]
+
+    def forward_paged(self, ids: torch.Tensor, batch: PagedBatch, rope, caches: list[PagedKVCache],
+                      return_logits: bool = False):
+        """All new tokens (packed int32 ids) through every layer: a decode step, a
+        chunk of a prompt, drafted tokens, or a mix.  Returns (the token that follows
+        each sequence's last one, the logits there | None); a sequence without new
+        tokens repeats the row before it."""
+        h = self.embed_tokens(ids)
+        for layer, cache in zip(self.layers, caches):
+            h = layer.forward_paged(h, batch, rope, cache)
+        normed = self.norm(h.index_select(0, (batch.cu_seqlens[1:] - 1).clamp(min=0)))
+        b, cfg = normed.shape[0], self.config
+        nxt = torch.empty(b, dtype=torch.int32, device=self.device)
+        logits = torch.empty((b, cfg.vocab_size), dtype=torch.bfloat16, device=self.device) if return_logits else None
+        for i in range(0, b, 256):  # the lm_head kernel takes 256 rows
+            rows = normed[i:i + 256]
+            ws = torch.empty(_lib.argmax_workspace_bytes(rows.shape[0], cfg.hidden_size, cfg.vocab_size),
+                             dtype=torch.uint8, device=self.device)
+            self.lm_head_argmax(rows, ws, nxt[i:i + 256], None if logits is None else logits[i:i + 256])
         return nxt, logits
 
 

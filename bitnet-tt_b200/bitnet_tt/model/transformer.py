@@ -14,6 +14,7 @@ from ..config import BitNetConfig
 from ..layers.attention import KVCache, MultiHeadAttention
 from ..layers.bitlinear import RMSNorm
 from ..layers.ffn import FeedForward
+from ..layers.paged_kv import PagedBatch, PagedKVCache
 
 
 class TransformerBlock:
@@ -46,4 +47,11 @@ class TransformerBlock:
         eps = self.config.rms_norm_eps
         h = self.self_attn(hidden, positions, rope, cache, norm_weight=self.input_layernorm.weight,
                            norm_epsilon=eps, residual=hidden)
+        return self.mlp(h, norm_weight=self.post_attention_layernorm.weight, norm_epsilon=eps, residual=h)
+
+    def forward_paged(self, hidden: torch.Tensor, batch: PagedBatch, rope, cache: PagedKVCache) -> torch.Tensor:
+        """Eager forward of the new tokens' rows [tokens, hidden] over a paged cache."""
+        eps = self.config.rms_norm_eps
+        h = self.self_attn.forward_paged(hidden, batch, rope, cache, norm_weight=self.input_layernorm.weight,
+                                         norm_epsilon=eps, residual=hidden)
         return self.mlp(h, norm_weight=self.post_attention_layernorm.weight, norm_epsilon=eps, residual=h)

@@ -1352,7 +1352,8 @@ extern "C" {
 int bitnet_paged_append(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
                         const int32_t* cu_seqlens, const int32_t* kv_lens, const void* qkv, int ld_qkv,
                         int total_tokens, int n_heads, const void* rope_cos, const void* rope_sin, int rope_len,
-                        int rotary_dim, int rope_f32, int interleaved, void* q_out, bitnet_stream_t stream) {
+                        int rotary_dim, int rope_f32, int interleaved, int stepwise, void* q_out,
+                        bitnet_stream_t stream) {
   PagedAppendParams p;
   memset(&p, 0, sizeof(p));
   if (int e = paged_kv_args(kv, block_table, B, max_pages, &p.kv)) return e;
@@ -1382,6 +1383,7 @@ int bitnet_paged_append(const bitnet_paged_kv_t* kv, const int32_t* block_table,
   p.rope_len = rope_len;
   p.rot = rotary_dim;
   p.interleaved = interleaved != 0;
+  p.stepwise = stepwise != 0;
   p.q_out = (uint16_t*)q_out;
   // a token a CTA until the GPU is full, so that a decode batch is one round of loads deep
   p.tok_per_cta = std::min(8, std::max(1, total_tokens / (d->sms * 4)));

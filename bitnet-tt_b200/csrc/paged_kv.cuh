@@ -82,10 +82,10 @@ __device__ __forceinline__ uint32_t codes_of_f32(float a, float b, float c, floa
 //     a' = a cos[pos][j] - b sin[pos][j],   b' = b cos[pos][j] + a sin[pos][j]
 // in fp32, each product and sum rounded on its own (so an int8 code is a
 // function of the inputs alone, not of how the compiler fuses), and the dims
-// from rot on copied.  A value is rounded once, to bf16 or to its int8 code: the
-// contiguous cache's kernels round after every product and sum as the bf16
-// model code does, which costs up to three roundings a value and, with an int8
-// cache, a fourth.
+// from rot on copied.  A value is rounded once, to bf16 or to its int8 code; with
+// `stepwise` every product and sum is rounded to bf16 as well, which is what the
+// bf16 model code and the contiguous cache's kernels do: the rows are then those
+// kernels' bit for bit.
 //     int8: top = max(max_d |row|, 1e-5), scale = top / 127, code = rint(row * (127 / top)),
 // the floor of the framework's activation quantiser.  A row with an infinity or
 // a NaN gets the scale NaN (its values read back as NaN).
@@ -105,7 +105,7 @@ struct PagedAppendParams {
   int ld_qkv, n_heads;
   const void* cos;         // [rope_len][rot / 2], bf16 or fp32
   const void* sin;
-  int rope_len, rot, interleaved;
+  int rope_len, rot, interleaved, stepwise;
   uint16_t* q_out;         // [tokens][n_heads * D]
   int tok_per_cta;         // 1 .. 8
 };
@@ -123,6 +123,18 @@ __device__ __forceinline__ void rope_entries8(const void* t, size_t i, float (&x
   }
 }
 
+// One rotated pair.
+__device__ __forceinline__ void rotate_pair(float& a, float& b, float c, float s, bool stepwise) {
+  const float ac = __fmul_rn(a, c), bs = __fmul_rn(-b, s), bc = __fmul_rn(b, c), as = __fmul_rn(a, s);
+  if (stepwise) {
+    a = round_bf16(__fadd_rn(round_bf16(ac), round_bf16(bs)));
+    b = round_bf16(__fadd_rn(round_bf16(bc), round_bf16(as)));
+  } else {
+    a = __fadd_rn(ac, bs);
+    b = __fadd_rn(bc, as);
+  }
+}
+
 // The chunks (of 8 dims) that lane l of a head takes: c0 and c1 hold the pairs
 // (d, d + rot / 2) of half layouts; adjacent pairs lie within a chunk.
 __device__ __forceinline__ void append_chunks(int l, int rot, bool interleaved, int& c0, int& c1, bool& turns) {
@@ -133,10 +145,10 @@ __device__ __forceinline__ void append_chunks(int l, int rot, bool interleaved, 
 }
 
 template <int D, bool I8, bool F32>
-__global__ void __launch_bounds__(PKV_THREADS, 4) paged_append_kernel(const PagedAppendParams p) {
+__global__ void __launch_bounds__(PKV_THREADS, 5) paged_append_kernel(const PagedAppendParams p) {
   constexpr int LPH = D / 16;                 // lanes of one head
   constexpr int GROUPS = PKV_THREADS / LPH;   // heads at once
-  constexpr int U = I8 ? 1 : 3;                        // heads of a lane in flight
+  constexpr int U = I8 ? 1 : 2;               // heads of a lane in flight
   __shared__ int s_pos[8], s_page[8];
   pdl_trigger();
   pdl_wait();
@@ -203,19 +215,12 @@ __global__ void __launch_bounds__(PKV_THREADS, 4) paged_append_kernel(const Page
         if (p.interleaved) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float a = x[2 * e], b = x[2 * e + 1], a2 = y[2 * e], b2 = y[2 * e + 1];
-            x[2 * e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
-            x[2 * e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
-            y[2 * e] = __fsub_rn(__fmul_rn(a2, c[4 + e]), __fmul_rn(b2, s[4 + e]));
-            y[2 * e + 1] = __fadd_rn(__fmul_rn(b2, c[4 + e]), __fmul_rn(a2, s[4 + e]));
+            rotate_pair(x[2 * e], x[2 * e + 1], c[e], s[e], p.stepwise);
+            rotate_pair(y[2 * e], y[2 * e + 1], c[4 + e], s[4 + e], p.stepwise);
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float a = x[e], b = y[e];
-            x[e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
-            y[e] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
-          }
+          for (int e = 0; e < 8; ++e) rotate_pair(x[e], y[e], c[e], s[e], p.stepwise);
         }
       }
       const int g = is_q ? 0 : (is_v ? hh - p.n_heads - p.kv.n_kv : hh - p.n_heads);
@@ -276,7 +281,7 @@ struct PagedReadParams {
 constexpr int PKV_READ_ROWS = 8;
 
 template <int D, bool I8>
-__global__ void __launch_bounds__(PKV_THREADS, 7) paged_read_kernel(const PagedReadParams p) {
+__global__ void __launch_bounds__(PKV_THREADS, 6) paged_read_kernel(const PagedReadParams p) {
   constexpr int LPH = D / (I8 ? 16 : 8);  // lanes of a row, 16 bytes each
   constexpr int GROUPS = PKV_THREADS / LPH;
   constexpr int U = 2;

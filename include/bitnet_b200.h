@@ -323,15 +323,17 @@ typedef struct {
  * fp32 if rope_f32, else bf16.  rotary_dim (a multiple of 16, at most head_dim):
  * the head's first dims, which are rotated; the rest is copied.  Pairs are dims
  * (j, j + rotary_dim / 2), or (2j, 2j + 1) if interleaved.  The rotation is in
- * fp32 and rounded once; bitnet_rope_append_prefill rounds after each product
- * and sum, so their last bits differ.  int8: top = max(max |row|, 1e-5),
+ * fp32 and its result rounded once; with stepwise, products and sums are rounded
+ * to bf16 too, as the bf16 model code and bitnet_rope_append_prefill do (the rows
+ * are then bit-identical to that entry point's).  int8: top = max(max |row|, 1e-5),
  * scale = top / 127, code = rint(row * (127 / top)); a row that holds an infinity
  * or a NaN gets the scale NaN.  qkv, q_out, rope_cos and rope_sin 16-byte
  * aligned, ld_qkv a multiple of 8. */
 int bitnet_paged_append(const bitnet_paged_kv_t* kv, const int32_t* block_table, int B, int max_pages,
                         const int32_t* cu_seqlens, const int32_t* kv_lens, const void* qkv, int ld_qkv,
                         int total_tokens, int n_heads, const void* rope_cos, const void* rope_sin, int rope_len,
-                        int rotary_dim, int rope_f32, int interleaved, void* q_out, bitnet_stream_t stream);
+                        int rotary_dim, int rope_f32, int interleaved, int stepwise, void* q_out,
+                        bitnet_stream_t stream);
 /* Reads rows back: sequence b's packed rows cu_rows[b] .. cu_rows[b + 1] - 1 of
  * k_out / v_out (bf16 [total_rows][n_kv_heads][head_dim], 16-byte aligned) are its
  * cache rows from starts[b] (int32 [B], NULL: 0) on; int8 as bf16(code * scale). */

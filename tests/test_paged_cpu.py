@@ -25,7 +25,7 @@ def _call(name, over_kv=None, **over):
     args = {
         "bitnet_paged_append": dict(kv=_lib.PagedKV(*kv.values()), block_table=a, B=2, max_pages=4, cu_seqlens=a,
                                     kv_lens=a, qkv=a, ld_qkv=512, total_tokens=3, n_heads=4, rope_cos=a, rope_sin=a,
-                                    rope_len=64, rotary_dim=64, rope_f32=0, interleaved=0, q_out=a, stream=None),
+                                    rope_len=64, rotary_dim=64, rope_f32=0, interleaved=0, stepwise=0, q_out=a, stream=None),
         "bitnet_paged_read": dict(kv=_lib.PagedKV(*kv.values()), block_table=a, B=2, max_pages=4, starts=None, cu_rows=a,
                                   total_rows=5, k_out=a, v_out=a, stream=None),
         "bitnet_paged_attention": dict(kv=_lib.PagedKV(*kv.values()), block_table=a, B=2, max_pages=4, cu_seqlens=a,

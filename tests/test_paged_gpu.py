@@ -161,6 +161,27 @@ def test_append_strided_rows_and_rows_behind_the_last_sequence(cuda, dtype):
     _append_case(cuda, [3, 4], [19, 4], 4, 2, 64, 16, dtype, 64, False, torch.float32, seed=5, pad=24, extra=3)
 
 
+def test_append_stepwise_rows_are_the_contiguous_caches(cuda):
+    """stepwise: the rows and queries of bitnet_rope_append_prefill, bit for bit."""
+    from bitnet_tt import _lib
+    from bitnet_tt.utils.rope import half_split_tables
+
+    b, n, hq, hk, d = 3, 21, 8, 2, 128
+    qkv = torch.randn((b * n, (hq + 2 * hk) * d), generator=torch.Generator().manual_seed(6)).to(BF16).to(cuda)
+    cos, sin = (t.to(cuda) for t in half_split_tables(d, 32, 500000.0))
+    kc, vc = (torch.zeros((b, hk, 32, d), dtype=BF16, device=cuda) for _ in range(2))
+    q = torch.empty((b * n, hq * d), dtype=BF16, device=cuda)
+    _lib.rope_append_prefill(qkv, b, n, hq, hk, cos, sin, q, kc, vc)
+    table, pages = _pages([n] * b, 16, 1)
+    c = _cache(cuda, pages, 16, hk, d, BF16)
+    args = (_cu([n] * b).to(cuda), torch.full((b,), n, dtype=torch.int32, device=cuda), table.to(cuda), cos, sin)
+    assert torch.equal(c.append(qkv, *args, stepwise=True), q)
+    k, v = c.read(args[2], None, args[0], b * n)
+    _ok()
+    assert torch.equal(k.view(b, n, hk, d), kc[:, :, :n].transpose(1, 2))
+    assert torch.equal(v.view(b, n, hk, d), vc[:, :, :n].transpose(1, 2))
+
+
 def test_append_many_sequences_and_tokens(cuda):
     # more than one round of the sequence search, several tokens a CTA
     qs = [(i * 7) % 5 for i in range(1100)]
@@ -500,3 +521,160 @@ def test_offsets_beyond_32_bits(cuda):
     last = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
     assert torch.equal(c.attend(q[-1:], last, lens, table, 1, 600), small.attend(q[-1:], last, lens, at, 1, 600))
     _ok()
+
+
+# ---------------------------------------------------------------------------
+# the operators together: a model over paged caches
+# ---------------------------------------------------------------------------
+def _model(cuda, **kw):
+    from bitnet_tt.config import BitNetConfig
+    from bitnet_tt.model import create_model
+    from bitnet_tt.utils.weights import load_weights_to_model, synthetic_state_dict
+
+    cfg = BitNetConfig(**(dict(hidden_size=512, num_layers=3, num_attention_heads=4, num_key_value_heads=2,
+                               intermediate_size=1024, vocab_size=1000, max_position_embeddings=256) | kw))
+    lazy = synthetic_state_dict(cfg, 5)
+    sd = {k: lazy[k].numpy() for k in lazy}
+    m = create_model(cfg, cuda)
+    load_weights_to_model(m, sd)
+    return m, cfg, sd
+
+
+# head dimensions 128, and 64 (the mini model, 256 / 4), which the contiguous path does not take
+MODELS = [dict(), dict(hidden_size=256, intermediate_size=512)]
+
+
+@pytest.mark.parametrize("kw", MODELS)
+@pytest.mark.parametrize("cuts", [[], [10, 11, 40], [1, 2, 3, 70]])
+def test_paged_layers_match_the_oracle(cuda, kw, cuts):
+    """On identical inputs the K and V rows are the oracle's bit for bit and the
+    layer's outputs within 4e-2 of it (norms), whether a prompt is read at once or in
+    chunks (cut at these tokens).
+
+    4e-2, and not the contiguous path's 2e-2: one bf16 weight is off by 2^-9 (rms of a
+    half step), so the attention's output by e = 2^-9 beside its own rounding.  The
+    int8 quantiser behind it has steps of q = amax / 127, about 3 / 127 of the rms:
+    a share e / q of the codes flips by one step, an error of q sqrt(e / q) = sqrt(e q)
+    = 6.8e-3 after o_proj.  The same quantiser before gate and up makes that
+    sqrt(6.8e-3 q) = 1.3e-2, ReLU^2 times up at most three times as much: 3.8e-2 of the
+    feed-forward's share of the output, which is less than all of it."""
+    import numpy as np
+
+    from bitnet_tt.layers import PagedBatch
+    from bitnet_tt.utils.rope import half_split_tables
+    from oracle.model import OracleBitNet
+
+    m, cfg, sd = _model(cuda, **kw)
+    o = OracleBitNet(cfg, sd, max_len=128)
+    lens = [90, 33]
+    prompts = [np.random.default_rng(n).integers(0, cfg.vocab_size, size=n) for n in lens]
+    rope = tuple(t.to(cuda) for t in half_split_tables(cfg.head_dim, 128, cfg.rope_theta))
+    pages = [[5, 0, 3, 7, 2, 1], [4, 6, 8]]
+    caches = m.paged_caches(9, 16)
+    hs = [o.embed[torch.from_numpy(p)] for p in prompts]
+    for i, layer in enumerate(m.layers):
+        ref, rows = [], []
+        for h in hs:
+            cache = o.new_cache(1, 128)[0]
+            ref.append(o.layer_prefill(i, h, 1, h.shape[0], cache))
+            rows.append(cache)
+        got = [[], []]
+        for lo, hi in zip([0] + cuts, cuts + [max(lens)]):
+            new = [max(0, min(hi, n) - lo) for n in lens]
+            batch = PagedBatch.of(new, [min(hi, n) for n in lens], pages, cuda)
+            x = torch.cat([h[lo:lo + k] for h, k in zip(hs, new)]).to(BF16).to(cuda)
+            y = layer.forward_paged(x, batch, rope, caches[i]).float().cpu()
+            for b, part in enumerate(y.split(new)):
+                got[b].append(part)
+        k, v = caches[i].read(batch.block_table, None, _cu(lens).to(cuda), sum(lens))
+        _ok()
+        for b, n in enumerate(lens):
+            out = torch.cat(got[b])
+            assert float((out - ref[b]).norm() / ref[b].norm()) < 4e-2
+            at = slice(sum(lens[:b]), sum(lens[:b]) + n)
+            for mine, want in ((k, rows[b][0]), (v, rows[b][1])):
+                assert torch.equal(mine[at].float().cpu(), want[0, :, :n].transpose(0, 1))
+        hs = ref
+
+
+@pytest.mark.parametrize("kw", MODELS)
+@pytest.mark.parametrize("chunk", [8192, 13])  # whole prompts, and chunks of them beside decoding sequences
+def test_paged_generation_follows_the_oracle(cuda, kw, chunk):
+    """Greedy tokens are the oracle's on the same history, but where its logits are
+    too close to tell (tests/parity_rules.py)."""
+    import numpy as np
+
+    from bitnet_tt.inference import PagedGenerator
+    from oracle.model import OracleBitNet
+    from parity_rules import within_logit_tol
+
+    m, cfg, sd = _model(cuda, **kw)
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, cfg.vocab_size, size=n).tolist() for n in (1, 37, 16, 90)]
+    gen = PagedGenerator(m, num_pages=24, page_size=16, chunk_tokens=chunk)
+    tokens = gen.generate(prompts, 6)
+    _ok()
+    assert sorted(gen.free_pages) == list(range(24)) and not gen.sequences
+    o = OracleBitNet(cfg, sd, max_len=128)
+    for p, mine in zip(prompts, tokens):
+        caches = o.new_cache(1)
+        _, logits = o.prefill(np.asarray(p).reshape(1, -1), caches)
+        for i, t in enumerate(mine):
+            fine, why = within_logit_tol(logits[0], t)
+            assert fine, why
+            _, logits = o.step(torch.tensor([t]), torch.tensor([len(p) + i], dtype=torch.int32), caches)
+
+
+def test_paged_generation_int8_extended_and_interleaved(cuda):
+    """An int8 cache: a second turn read in one chunk, and two sequences that grow
+    beside each other, give what one pass over the same tokens gives."""
+    import numpy as np
+
+    from bitnet_tt.inference import PagedGenerator
+
+    m, cfg, _ = _model(cuda)
+    rng = np.random.default_rng(4)
+    a, b, c = (rng.integers(0, cfg.vocab_size, size=n).tolist() for n in (40, 25, 60))
+    gen = PagedGenerator(m, num_pages=24, page_size=16, cache_dtype=I8)
+    one = gen.add(a)
+    for _ in range(3):
+        gen.step()
+    two = gen.add(c)
+    gen.extend(one, b)  # behind the token that is pending
+    gen.step(keep_logits=True)
+    got = gen.last_logits.float().cpu()
+    told = gen.sequences[one].generated
+    fresh = PagedGenerator(m, num_pages=24, page_size=16, cache_dtype=I8)
+    fresh.add(a + told[:3] + b)
+    fresh.add(c)
+    fresh.step(keep_logits=True)
+    want = fresh.last_logits.float().cpu()
+    _ok()
+    # The hidden states of the two runs differ by bf16 roundings, which the activation
+    # quantiser turns into code flips: 2e-2 to 4.5e-2 between this model's contiguous
+    # path and the oracle (no reading of bf16 arithmetic is the right one).
+    assert float((got - want).norm() / want.norm()) < 0.1
+    assert gen.sequences[one].length == len(a) + 3 + len(b) and gen.sequences[two].length == len(c)
+    out = PagedGenerator(m, num_pages=8, page_size=16, cache_dtype=I8).generate([a, b], 5)
+    assert [len(o) for o in out] == [5, 5]
+
+
+def test_paged_generator_refusals(cuda):
+    from bitnet_tt.inference import PagedGenerator
+
+    m, cfg, _ = _model(cuda)
+    gen = PagedGenerator(m, num_pages=2, page_size=16, max_seq_len=64)
+    for bad in ([], [cfg.vocab_size], [-1], [0] * 65):
+        with pytest.raises(ValueError):
+            gen.add(bad)
+    with pytest.raises(ValueError):
+        gen.generate([[1, 2]], 64)
+    s = gen.add(list(range(40)))  # three pages; the pool has two
+    assert gen.step() == {} and gen.sequences[s].length == 32
+    with pytest.raises(RuntimeError, match="no pages"):
+        gen.step()
+    with pytest.raises(ValueError):
+        gen.extend(s, [1] * 30)
+    gen.release(s)
+    assert gen.step() == {}
+    assert len(gen.generate([[1, 2, 3], [4]], 3)[1]) == 3
