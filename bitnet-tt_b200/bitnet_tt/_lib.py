@@ -541,27 +541,27 @@ def attention_prefill_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
 
 # The paged cache's calls are short on the GPU (a decode step's append takes 3 us),
 # so these wrappers keep the host's share small: the caller (layers/paged_kv.py)
-# checks its tensors, the stream comes as the raw handle, and the library is
-# looked up once.  index: the device of the cache, which must be current.
-def paged_append(kv: PagedKV, index: int, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
-                 qkv: torch.Tensor, n_heads: int, rope_cos: torch.Tensor, rope_sin: torch.Tensor, q_out: torch.Tensor,
-                 interleaved: bool = False, stepwise: bool = False) -> None:
-    b, max_pages = block_table.shape
+# checks its tensors and passes their sizes, the stream comes as the raw handle, and
+# the library is looked up once.  index: the device of the cache, which must be
+# current; b, max_pages: the block table's shape.
+def paged_append(kv: PagedKV, index: int, block_table: torch.Tensor, b: int, max_pages: int, cu_seqlens: torch.Tensor,
+                 kv_lens: torch.Tensor, qkv: torch.Tensor, tokens: int, n_heads: int, rope_cos: torch.Tensor,
+                 rope_sin: torch.Tensor, rope_f32: bool, q_out: torch.Tensor, interleaved: bool = False,
+                 stepwise: bool = False) -> None:
     rope_len, half = rope_cos.shape
     st = (_lib or load()).bitnet_paged_append(
         kv, block_table.data_ptr(), b, max_pages, cu_seqlens.data_ptr(), kv_lens.data_ptr(), qkv.data_ptr(),
-        qkv.stride(0), qkv.shape[0], n_heads, rope_cos.data_ptr(), rope_sin.data_ptr(), rope_len, 2 * half,
-        rope_cos.dtype is torch.float32, interleaved, stepwise, q_out.data_ptr(), raw_stream(index))
+        qkv.stride(0), tokens, n_heads, rope_cos.data_ptr(), rope_sin.data_ptr(), rope_len, 2 * half, rope_f32,
+        interleaved, stepwise, q_out.data_ptr(), raw_stream(index))
     if st:
         check(st, "bitnet_paged_append")
 
 
-def paged_read(kv: PagedKV, index: int, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor,
-               k_out: torch.Tensor, v_out: torch.Tensor) -> None:
-    b, max_pages = block_table.shape
+def paged_read(kv: PagedKV, index: int, block_table: torch.Tensor, b: int, max_pages: int, starts: torch.Tensor | None,
+               cu_rows: torch.Tensor, rows: int, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
     st = (_lib or load()).bitnet_paged_read(
         kv, block_table.data_ptr(), b, max_pages, None if starts is None else starts.data_ptr(), cu_rows.data_ptr(),
-        k_out.shape[0], k_out.data_ptr(), v_out.data_ptr(), raw_stream(index))
+        rows, k_out.data_ptr(), v_out.data_ptr(), raw_stream(index))
     if st:
         check(st, "bitnet_paged_read")
 
@@ -572,13 +572,12 @@ def paged_attention_workspace_bytes(b: int, total_tokens: int, max_seqlen: int, 
                                                              head_dim))
 
 
-def paged_attention(kv: PagedKV, index: int, block_table: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
-                    q: torch.Tensor, max_seqlen: int, max_kv_len: int, n_heads: int, scale: float,
-                    workspace: torch.Tensor | None, out: torch.Tensor) -> None:
-    b, max_pages = block_table.shape
+def paged_attention(kv: PagedKV, index: int, block_table: torch.Tensor, b: int, max_pages: int, cu_seqlens: torch.Tensor,
+                    kv_lens: torch.Tensor, q: torch.Tensor, tokens: int, max_seqlen: int, max_kv_len: int, n_heads: int,
+                    scale: float, workspace: torch.Tensor | None, out: torch.Tensor) -> None:
     ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
     st = (_lib or load()).bitnet_paged_attention(
         kv, block_table.data_ptr(), b, max_pages, cu_seqlens.data_ptr(), kv_lens.data_ptr(), q.data_ptr(), q.stride(0),
-        q.shape[0], max_seqlen, max_kv_len, n_heads, scale, ws, ws_bytes, out.data_ptr(), raw_stream(index))
+        tokens, max_seqlen, max_kv_len, n_heads, scale, ws, ws_bytes, out.data_ptr(), raw_stream(index))
     if st:
         check(st, "bitnet_paged_attention")

@@ -29,6 +29,17 @@ from .. import _lib
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
 
+class _Current:
+    def __enter__(self) -> None:
+        pass
+
+    def __exit__(self, *_exc) -> None:
+        pass
+
+
+_CURRENT = _Current()
+
+
 @dataclass
 class PagedBatch:
     """The new tokens of one forward pass over paged caches: one per sequence of a
@@ -98,6 +109,8 @@ class PagedKVCache:
         self.device = k.device
         self._index = k.get_device()
         self.dtype = k.dtype
+        self._bf16 = k.new_empty(0, dtype=torch.bfloat16)
+        self._scale = k.shape[3] ** -0.5
         self._kv = _lib.PagedKV(_lib.ptr(k), _lib.ptr(v), _lib.ptr(ks), _lib.ptr(vs), *k.shape[0:1], k.shape[2],
                                 k.shape[1], k.shape[3], _lib.KV_INT8 if k.dtype == torch.int8 else _lib.KV_BF16)
 
@@ -133,18 +146,14 @@ class PagedKVCache:
 
     def _out(self, t: torch.Tensor | None, shape: tuple, name: str) -> torch.Tensor:
         if t is None:
-            return torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            return self._bf16.new_empty(shape)
         if t.dtype is not torch.bfloat16 or t.get_device() != self._index or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous bfloat16 {shape} on {self.device}")
         return t
 
-    def _launch(self, call, *args) -> None:
-        """call(*args) with the cache's device current."""
-        if torch._C._cuda_getDevice() == self._index:
-            call(self._kv, self._index, *args)
-        else:
-            with torch.cuda.device(self._index):
-                call(self._kv, self._index, *args)
+    def _on_device(self):
+        """The cache's device as the current one (nothing to do when it is)."""
+        return _CURRENT if torch._C._cuda_getDevice() == self._index else torch.cuda.device(self._index)
 
     # ---- calls -------------------------------------------------------------
     def append(self, qkv: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
@@ -157,9 +166,9 @@ class PagedKVCache:
         rotary_dim / 2]; rotary_dim may be less than head_dim.  The rotation is
         rounded once; stepwise rounds its products and sums to bf16 too, as the bf16
         model code and the contiguous cache's kernels do."""
-        n = kv_lens.numel()
+        n, table = kv_lens.numel(), block_table.shape
         if not (self._index_ok(block_table) and self._index_ok(cu_seqlens) and self._index_ok(kv_lens)
-                and block_table.dim() == 2 and block_table.shape[0] == n and cu_seqlens.numel() == n + 1 and n):
+                and len(table) == 2 and table[0] == n and table[1] and cu_seqlens.numel() == n + 1 and n):
             self._refuse_index(block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens)
         if not self._rows_ok(qkv):
             raise ValueError(f"qkv must be bfloat16 rows [tokens, features] on {self.device}")
@@ -171,8 +180,9 @@ class PagedKVCache:
                 and rope_sin.get_device() == self._index and rope_cos.is_contiguous() and rope_sin.is_contiguous()):
             raise ValueError("rope tables must be two equal contiguous bf16 or fp32 [positions, rotary_dim / 2]")
         q_out = self._out(q_out, (tokens, heads * self.head_dim), "q_out")
-        self._launch(_lib.paged_append, block_table, cu_seqlens, kv_lens, qkv, heads, rope_cos, rope_sin, q_out, interleaved,
-                     stepwise)
+        with self._on_device():
+            _lib.paged_append(self._kv, self._index, block_table, n, table[1], cu_seqlens, kv_lens, qkv, tokens, heads,
+                              rope_cos, rope_sin, tab is torch.float32, q_out, interleaved, stepwise)
         return q_out
 
     def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
@@ -183,9 +193,9 @@ class PagedKVCache:
         bound the new tokens and the keys of every sequence.  scale: 1 /
         sqrt(head_dim) by default.  workspace (attention_workspace): taken from the
         allocator if not given."""
-        n = kv_lens.numel()
+        n, table = kv_lens.numel(), block_table.shape
         if not (self._index_ok(block_table) and self._index_ok(cu_seqlens) and self._index_ok(kv_lens)
-                and block_table.dim() == 2 and block_table.shape[0] == n and cu_seqlens.numel() == n + 1 and n):
+                and len(table) == 2 and table[0] == n and table[1] and cu_seqlens.numel() == n + 1 and n):
             self._refuse_index(block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens)
         if not self._rows_ok(q):
             raise ValueError(f"q must be bfloat16 rows [tokens, features] on {self.device}")
@@ -196,8 +206,9 @@ class PagedKVCache:
             workspace = self.attention_workspace(n, tokens, max_seqlen, max_kv_len, heads)
         elif workspace.get_device() != self._index or not workspace.is_contiguous():
             raise ValueError(f"workspace must be a contiguous tensor on {self.device}")
-        self._launch(_lib.paged_attention, block_table, cu_seqlens, kv_lens, q, max_seqlen, max_kv_len, heads,
-                     self.head_dim ** -0.5 if scale is None else scale, workspace, out)
+        with self._on_device():
+            _lib.paged_attention(self._kv, self._index, block_table, n, table[1], cu_seqlens, kv_lens, q, tokens, max_seqlen,
+                                 max_kv_len, heads, self._scale if scale is None else scale, workspace, out)
         return out
 
     def attention_workspace(self, batch: int, total_tokens: int, max_seqlen: int, max_kv_len: int,
@@ -206,23 +217,24 @@ class PagedKVCache:
         that may overlap need one each."""
         n = _workspace_bytes(self._index, batch, total_tokens, max_seqlen, max_kv_len, num_heads, self.num_kv_heads,
                              self.head_dim)
-        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        return self._bf16.new_empty(n // 2) if n else None
 
     def read(self, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor, total_rows: int,
              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows starts[b] .. starts[b] + cu_rows[b + 1] - cu_rows[b] - 1 of every
         sequence (starts None: from row 0) as packed bf16 keys and values
         [total_rows, n_kv, head_dim]."""
-        n = cu_rows.numel() - 1
-        if not (self._index_ok(block_table) and self._index_ok(cu_rows) and block_table.dim() == 2
-                and block_table.shape[0] == n and n
+        n, table = cu_rows.numel() - 1, block_table.shape
+        if not (self._index_ok(block_table) and self._index_ok(cu_rows) and len(table) == 2 and table[0] == n and table[1]
+                and n
                 and (starts is None or (self._index_ok(starts) and starts.numel() == n))):
             self._refuse_index(block_table, cu_rows=cu_rows, **({} if starts is None else {"starts": starts}))
         if total_rows < 0:
             raise ValueError("total_rows is negative")
         shape = (total_rows, self.num_kv_heads, self.head_dim)
         k_out, v_out = self._out(k_out, shape, "k_out"), self._out(v_out, shape, "v_out")
-        self._launch(_lib.paged_read, block_table, starts, cu_rows, k_out, v_out)
+        with self._on_device():
+            _lib.paged_read(self._kv, self._index, block_table, n, table[1], starts, cu_rows, total_rows, k_out, v_out)
         return k_out, v_out
 
 
