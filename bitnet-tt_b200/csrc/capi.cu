@@ -1263,16 +1263,17 @@ int encode_tiled(EncodeTiled* out) {
   return BITNET_OK;
 }
 
-// A bf16 pool as rows of head_dim; a box is 64 dims of the rows of a page (at most
-// a key tile), swizzled as the MMA reads them.
-int paged_map(CUtensorMap* m, const PagedKV& kv, const void* pool, int D) {
+// A pool as rows of head_dim; a box holds the rows of a page (at most a key tile):
+// 64 dims of them in bf16, swizzled as the MMA reads them, or all codes, as they are.
+int paged_map(CUtensorMap* m, const PagedKV& kv, const void* pool, int D, bool i8) {
   EncodeTiled enc;
   if (int e = encode_tiled(&enc)) return e;
   const cuuint64_t dims[2] = {(cuuint64_t)D, ((cuuint64_t)kv.num_pages * kv.n_kv) << kv.page_shift};
-  const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)std::min(1 << kv.page_shift, PCH_KB)}, elem[2] = {1, 1};
-  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pool), dims, strides, box, elem,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const cuuint64_t strides[1] = {(cuuint64_t)(i8 ? D : D * 2)};
+  const cuuint32_t box[2] = {(cuuint32_t)(i8 ? D : 64), (cuuint32_t)std::min(1 << kv.page_shift, PCH_KB)}, elem[2] = {1, 1};
+  const CUresult r = enc(m, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                         const_cast<void*>(pool), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         i8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return BITNET_OK;
   snprintf(g_cuda_msg, sizeof(g_cuda_msg), "cuTensorMapEncodeTiled: error %d", (int)r);
@@ -1323,12 +1324,8 @@ int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspa
     }
     if (int e = ensure_smem(k, &g_smem_pch[idx])) return e;
     CUtensorMap mk, mv;
-    memset(&mk, 0, sizeof(mk));
-    memset(&mv, 0, sizeof(mv));
-    if (!I8) {
-      if (int e = paged_map(&mk, p.kv, p.kv.k, D)) return e;
-      if (int e = paged_map(&mv, p.kv, p.kv.v, D)) return e;
-    }
+    if (int e = paged_map(&mk, p.kv, p.kv.k, D, I8)) return e;
+    if (int e = paged_map(&mv, p.kv, p.kv.v, D, I8)) return e;
     paged_apply(&p, pl.chunk, workspace);
     if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(S::THREADS), S::SMEM, st, 1, p, mk, mv)) return e;
   }

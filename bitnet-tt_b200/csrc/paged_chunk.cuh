@@ -20,8 +20,9 @@
 //                    after next.  Two, because the tensor cores queue few MMAs: a look at a
 //                    barrier costs the issuing warp about 100 cycles even when it is complete,
 //                    and with one warp those were gaps (980 cycles a tile and step for 640 of work)
-//   warp 10 (bf16)   loads K and V tiles by TMA, a box per page, into a ring of slots
-//   warps 12-15 (int8)  load codes and write them to the slots as f16
+//   warp 10          loads K and V tiles by TMA, a box per page, into a ring of slots (int8: of
+//                    raw tiles)
+//   warps 12-15 (int8)  write the raw tiles' codes to the slots as f16
 // The softmax's maximum is lazy: O and the sum are rescaled only when a row's
 // maximum grew by more than 2^8, so weights reach at most 2^8 and the pass over
 // O is rare (it waits for the products in flight).  P is rounded to bf16 (half a step: 2^-8 of a weight), the output's
@@ -60,13 +61,17 @@ struct PchShape {
   // softmaxes of that tile.
   static constexpr int RING = NSLOT / 2 + 1;
   static constexpr int EXTRA = I8 ? RING * 512 + 1024 : 0;
+  // int8: raw tiles in flight.  (Loaded through the converting warps' registers, one tile ahead,
+  // the loads' latency was what a step cost: 913 us where this takes 851, two 4096-token chunks over
+  // 16384 keys.)
+  static constexpr int NRAW = I8 ? (D == 64 ? 4 : 2) : 0, RAW = 128 * D;
   // Weights are exp2(x - m + LIFT): with f16's range the smallest step is below 2^-31 of the largest.
   static constexpr float LIFT = I8 ? 7.f : 0.f;
   // int8: registers a thread of the softmax, MMA and converting warpgroups, out of the launch's 128
-  static constexpr int REGS_SOFTMAX = 168, REGS_MMA = 56, REGS_CONVERT = 120;
+  static constexpr int REGS_SOFTMAX = 176, REGS_MMA = 56, REGS_CONVERT = 104;
   static_assert(256 * REGS_SOFTMAX + 128 * REGS_MMA + 128 * REGS_CONVERT <= 512 * 128, "within the launch's");
   static constexpr int CTRL = 512;
-  static constexpr int SMEM = 2 * TILE + NSLOT * TILE + EXTRA + CTRL;
+  static constexpr int SMEM = 2 * TILE + NSLOT * TILE + NRAW * RAW + EXTRA + CTRL;
 };
 
 // One lane of a converged warp.  The MMAs and their commits are issued under it:
@@ -123,6 +128,7 @@ __device__ __forceinline__ uint32_t pow2_field(uint32_t bits, int k) { return 25
 
 struct PchCtrl {
   uint64_t full[PCH_MAX_SLOTS], empty[PCH_MAX_SLOTS];
+  uint64_t raw_full[4], raw_empty[4];
   uint64_t s_full[2][2], p_ready[2][2];  // [row tile][step % 2]
   uint64_t o_done[2][2], drain[2], tail, q_full, v_full;  // o_done: O_t holds the step
   uint32_t tmem;
@@ -199,15 +205,20 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem_pch[];
   uint8_t* sm_q = smem_pch;
   uint8_t* sm_slots = sm_q + 2 * S::TILE;
-  float* sm_scale = reinterpret_cast<float*>(sm_slots + S::NSLOT * S::TILE);
+  uint8_t* sm_raw = sm_slots + S::NSLOT * S::TILE;
+  float* sm_scale = reinterpret_cast<float*>(sm_raw + S::NRAW * S::RAW);
   float* sm_fac = sm_scale + S::RING * 128;
-  PchCtrl* ctrl = reinterpret_cast<PchCtrl*>(sm_slots + S::NSLOT * S::TILE + S::EXTRA);
+  PchCtrl* ctrl = reinterpret_cast<PchCtrl*>(sm_raw + S::NRAW * S::RAW + S::EXTRA);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &ctrl->abort_flag;
   if (tid == 0) {
     for (int s = 0; s < S::NSLOT; ++s) {
       mbar_init(&ctrl->full[s], I8 ? 4 : 1);
       mbar_init(&ctrl->empty[s], 2);
+    }
+    for (int s = 0; s < S::NRAW; ++s) {
+      mbar_init(&ctrl->raw_full[s], 1);
+      mbar_init(&ctrl->raw_empty[s], 4);
     }
     for (int t = 0; t < 2; ++t) {
       for (int h = 0; h < 2; ++h) {
@@ -269,48 +280,46 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       const int w = warp - 12;
       const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
       const int slot_mask = (1 << p.kv.page_shift) - 1;
-      int pg[2] = {0, 0};  // pages of the warp's rows 0-15 and 16-31 in the tile being loaded
-      auto look_up = [&](int j) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = k0 + j * PCH_KB + 32 * w + 16 * h;
-          int page = 0;
-          if (j < ntile && key < k1) {
-            page = table[key >> p.kv.page_shift];
-            if (page < 0 || page >= p.kv.num_pages) {
-              record_error(DEV_ERR_BOUNDS, 361);
-              page = 0;
-            }
+      // this lane's row of a tile: the page, then the scales (0 past the part's keys)
+      auto key_of = [&](int j) { return k0 + j * PCH_KB + 32 * w + lane; };
+      auto page_of = [&](int j) {
+        if (j >= ntile || key_of(j) >= k1) return -1;
+        const int page = table[key_of(j) >> p.kv.page_shift];
+        return page < p.kv.num_pages ? page : -1;  // a bad one is reported by the loader
+      };
+      auto scales_of = [&](int j, int page, float& ks, float& vs) {
+        ks = vs = 0.f;
+        if (page >= 0) {
+          const size_t row = paged_row(p.kv, page, g, key_of(j) & slot_mask);
+          ks = p.kv.ks[row];
+          vs = p.kv.vs[row];
+        }
+      };
+      // Raw tile `it` to its slot; scale: of this lane's row of the warp's 32, as f16 (values only).
+      // Row and 16-byte chunk of piece u are such that eight lanes read 128 bytes of different
+      // banks and write eight different chunks.
+      auto convert = [&](int it, uint32_t scale) -> bool {
+        const int slot = it % S::NSLOT, stage = it % S::NRAW;
+        bool ok = wait(&ctrl->raw_full[stage], (it / S::NRAW) & 1, 378);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        uint4 buf[NL];
+        auto place = [&](int u, int& row, int& c) {
+          if (D == 128) {
+            c = lane & 7;
+            row = 2 * ((u >> 1) * 4 + (lane >> 3)) + (((lane >> 2) & 1) ^ (u & 1));
+          } else {
+            c = lane & 3;
+            row = u * 8 + (lane >> 2);
           }
-          pg[h] = page;
-        }
-      };
-      // row (of the warp's 32) and 16-byte chunk of load u: eight lanes read 128
-      // contiguous bytes' worth of banks and write eight different chunks
-      auto place = [&](int u, int& row, int& c) {
-        if (D == 128) {
-          c = lane & 7;
-          row = 2 * ((u >> 1) * 4 + (lane >> 3)) + (((lane >> 2) & 1) ^ (u & 1));
-        } else {
-          c = lane & 3;
-          row = u * 8 + (lane >> 2);
-        }
-      };
-      auto load = [&](int j, const uint8_t* pool, uint4 (&buf)[NL]) {
+        };
 #pragma unroll
         for (int u = 0; u < NL; ++u) {
           int row, c;
           place(u, row, c);
-          const int key = k0 + j * PCH_KB + 32 * w + row;
-          buf[u] = make_uint4(0, 0, 0, 0);
-          if (j < ntile && key < k1)
-            buf[u] = *reinterpret_cast<const uint4*>(pool + paged_row(p.kv, row < 16 ? pg[0] : pg[1], g, key & slot_mask) * D +
-                                                     c * 16);
+          buf[u] = *reinterpret_cast<const uint4*>(sm_raw + stage * S::RAW + (32 * w + row) * D + c * 16);
         }
-      };
-      // scale: of this lane's row of the warp's 32, as f16 (values only)
-      auto convert = [&](int it, const uint4 (&buf)[NL], uint32_t scale) -> bool {
-        const int slot = it % S::NSLOT;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctrl->raw_empty[stage]);
         if (it >= S::NSLOT && !__all_sync(0xffffffffu, wait(&ctrl->empty[slot], ((it / S::NSLOT) + 1) & 1, 362)))
           return false;
         uint8_t* dst = sm_slots + slot * S::TILE;
@@ -340,31 +349,23 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&ctrl->full[it % S::NSLOT]);
       };
-      float v_up = 0.f;
-      uint4 bk[NL], bv[NL];
-      look_up(0);
-      load(0, p.kv.k, bk);
+      float v_up = 0.f, ks, vs;
+      scales_of(0, page_of(0), ks, vs);
+      int page = page_of(1);
       for (int j = 0; j < ntile; ++j) {
-        // this lane's row: its scales (0 past the part's keys)
-        const int key = k0 + j * PCH_KB + 32 * w + lane;
-        float ks = 0.f, vs = 0.f;
-        if (key < k1) {
-          const size_t row = paged_row(p.kv, lane < 16 ? pg[0] : pg[1], g, key & slot_mask);
-          ks = p.kv.ks[row];
-          vs = p.kv.vs[row];
-        }
-        load(j, p.kv.v, bv);
-        look_up(j + 1);
-        if (!convert(2 * j, bk, 0)) break;
+        float ks1, vs1;
+        scales_of(j + 1, page, ks1, vs1);  // the next tile's, on the way while this one is converted
+        page = page_of(j + 2);
+        if (!convert(2 * j, 0)) break;
         sm_scale[(j % S::RING) * 128 + 32 * w + lane] = ks;
         arrive(2 * j);
-        load(j + 1, p.kv.k, bk);
         if (j == 0) {
           if (!__all_sync(0xffffffffu, wait(&ctrl->v_full, 0, 376))) break;
           v_up = __uint_as_float(pow2_field(pch_v_top(ctrl), 7) << 23);
         }
-        if (!convert(2 * j + 1, bv, f16x2_of(vs * v_up, vs * v_up))) break;
+        if (!convert(2 * j + 1, f16x2_of(vs * v_up, vs * v_up))) break;
         arrive(2 * j + 1);
+        ks = ks1, vs = vs1;
       }
     }
   } else if (warp >= 8) {
@@ -429,8 +430,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         __syncwarp();
         mbar_wait(&ctrl->drain[t], 0, 367);
       }
-    } else if (!I8 && warp == 10) {
-      // ---------------- bf16: TMA loads ----------------
+    } else if (warp == 10) {
+      // ---------------- TMA loads ----------------
       const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
       const int box = min(1 << p.kv.page_shift, PCH_KB);  // rows of a box: the map's
       const int slot_mask = (1 << p.kv.page_shift) - 1;
@@ -449,41 +450,59 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
           }
           y = (int)paged_row(p.kv, page, g, key & slot_mask);
         }
-        for (int v = 0; v < 2; ++v) {
-          const int it = 2 * j + v, slot = it % S::NSLOT;
-          if (it >= S::NSLOT) ok = __all_sync(0xffffffffu, wait(&ctrl->empty[slot], ((it / S::NSLOT) + 1) & 1, 368));
-          if (!ok) break;
-          const bool tail = v == 1 && base + PCH_KB > k1;
-          uint64_t* bar = tail ? &ctrl->tail : &ctrl->full[slot];
-          if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(nbox * box * D * 2));
-          __syncwarp();
-          const uint32_t dst = smem_u32(sm_slots + slot * S::TILE) + lane * box * 128;
-          if (lane < nbox) {
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h) tma_load_2d(dst + h * HALF, v ? &map_v : &map_k, h * 64, y, bar);
-          }
-          issued = it + 1;
-          if (tail) {
-            tail_issued = true;
-            // Whatever stands behind the last key must not meet a weight of 0: zeros.
-            ok = __all_sync(0xffffffffu, wait(&ctrl->tail, 0, 369));
+        for (int v = 0; ok && v < 2; ++v) {
+          const int it = 2 * j + v;
+          if constexpr (I8) {
+            // rows past the last key hold any codes: finite, and their scales are taken as 0
+            const int stage = it % S::NRAW;
+            if (it >= S::NRAW) ok = __all_sync(0xffffffffu, wait(&ctrl->raw_empty[stage], ((it / S::NRAW) + 1) & 1, 379));
             if (!ok) break;
-            const int live = k1 - base;
-            for (int i = lane; i < (128 - live) * (D / 8); i += 32) {
-              const int row = live + i / (D / 8), c = i % (D / 8);
-              *reinterpret_cast<uint4*>(sm_slots + slot * S::TILE + (c >> 3) * HALF + row * 128 + ((c & 7) << 4)) =
-                  make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
+            if (lane == 0) mbar_arrive_expect_tx(&ctrl->raw_full[stage], (uint32_t)(nbox * box * D));
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ctrl->full[slot]);
+            if (lane < nbox)
+              tma_load_2d(smem_u32(sm_raw + stage * S::RAW) + lane * box * D, v ? &map_v : &map_k, 0, y, &ctrl->raw_full[stage]);
+            issued = it + 1;
+          } else {
+            const int slot = it % S::NSLOT;
+            if (it >= S::NSLOT) ok = __all_sync(0xffffffffu, wait(&ctrl->empty[slot], ((it / S::NSLOT) + 1) & 1, 368));
+            if (!ok) break;
+            const bool tail = v == 1 && base + PCH_KB > k1;
+            uint64_t* bar = tail ? &ctrl->tail : &ctrl->full[slot];
+            if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(nbox * box * D * 2));
+            __syncwarp();
+            const uint32_t dst = smem_u32(sm_slots + slot * S::TILE) + lane * box * 128;
+            if (lane < nbox) {
+#pragma unroll
+              for (int h = 0; h < D / 64; ++h) tma_load_2d(dst + h * HALF, v ? &map_v : &map_k, h * 64, y, bar);
+            }
+            issued = it + 1;
+            if (tail) {
+              tail_issued = true;
+              // Whatever stands behind the last key must not meet a weight of 0: zeros.
+              ok = __all_sync(0xffffffffu, wait(&ctrl->tail, 0, 369));
+              if (!ok) break;
+              const int live = k1 - base;
+              for (int i = lane; i < (128 - live) * (D / 8); i += 32) {
+                const int row = live + i / (D / 8), c = i % (D / 8);
+                *reinterpret_cast<uint4*>(sm_slots + slot * S::TILE + (c >> 3) * HALF + row * 128 + ((c & 7) << 4)) =
+                    make_uint4(0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&ctrl->full[slot]);
+            }
           }
         }
       }
       if (*abort_flag) {  // copies in flight land before the CTA gives its memory back
-        if (tail_issued) mbar_wait(&ctrl->tail, 0, 370);
-        for (int it = max(0, issued - S::NSLOT); it < issued - (tail_issued ? 1 : 0); ++it)
-          mbar_wait(&ctrl->full[it % S::NSLOT], (it / S::NSLOT) & 1, 370);
+        if constexpr (I8) {
+          for (int it = max(0, issued - S::NRAW); it < issued; ++it)
+            mbar_wait(&ctrl->raw_full[it % S::NRAW], (it / S::NRAW) & 1, 380);
+        } else {
+          if (tail_issued) mbar_wait(&ctrl->tail, 0, 370);
+          for (int it = max(0, issued - S::NSLOT); it < issued - (tail_issued ? 1 : 0); ++it)
+            mbar_wait(&ctrl->full[it % S::NSLOT], (it / S::NSLOT) & 1, 370);
+        }
       }
     }
   } else {
