@@ -27,6 +27,7 @@ import torch
 from .. import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
+_INT_MAX = 0x7fffffff
 
 
 class _Current:
@@ -201,6 +202,8 @@ class PagedKVCache:
             raise ValueError(f"q must be bfloat16 rows [tokens, features] on {self.device}")
         tokens, features = q.shape
         heads = self._heads(features, 0, "q")
+        if max_seqlen > _INT_MAX or max_kv_len > _INT_MAX:
+            raise ValueError("max_seqlen and max_kv_len are 32-bit bounds")
         out = self._out(out, (tokens, features), "out")
         if workspace is None:
             workspace = self.attention_workspace(n, tokens, max_seqlen, max_kv_len, heads)
@@ -229,8 +232,8 @@ class PagedKVCache:
                 and n
                 and (starts is None or (self._index_ok(starts) and starts.numel() == n))):
             self._refuse_index(block_table, cu_rows=cu_rows, **({} if starts is None else {"starts": starts}))
-        if total_rows < 0:
-            raise ValueError("total_rows is negative")
+        if not 0 <= total_rows <= _INT_MAX:
+            raise ValueError("total_rows is out of range")
         shape = (total_rows, self.num_kv_heads, self.head_dim)
         k_out, v_out = self._out(k_out, shape, "k_out"), self._out(v_out, shape, "v_out")
         with self._on_device():

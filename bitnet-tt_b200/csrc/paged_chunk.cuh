@@ -581,7 +581,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     const int lim_min = __reduce_min_sync(0xffffffffu, lim);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t to = tbase + lanes + 256 + t * D;
-    const float scale = I8 ? p.scale_log2 * sm_fac[r] : p.scale_log2;
+    // not 0, which a hidden key's -infinity must not meet
+    const float scale = fmaxf(I8 ? p.scale_log2 * sm_fac[r] : p.scale_log2, 1e-37f);
     const uint64_t scale2 = f2_splat(scale);
     float m = -INFINITY;
     uint64_t l2[2] = {0, 0};

@@ -313,6 +313,13 @@ def test_attend_one_token(cuda, heads, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("heads", [(40, 1, 64), (64, 1, 128), (128, 2, 64)])
+def test_attend_wide_groups(cuda, heads, dtype):
+    # one token of a group is more rows than the small kernel takes
+    _attend_case(cuda, [1, 2, 0, 5], [300, 2, 9, 129], *heads, 16, dtype, seed=heads[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 def test_attend_page_sizes(cuda, page, dtype):
     _attend_case(cuda, [1, 2, 3, 0, 40], [300, 255, 256, 77, 513], 8, 2, 128, page, dtype, seed=page)
@@ -359,6 +366,22 @@ def test_attend_many_sequences(cuda):
     kv = [(37 * i) % 190 + q + 1 for i, q in enumerate(qs)]
     _attend_case(cuda, qs, kv, 4, 2, 64, 16, BF16, seed=2)
     _attend_case(cuda, [min(q, 1) for q in qs], kv, 4, 2, 64, 16, I8, seed=2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_attend_chunks_among_hundreds_of_decoding_sequences(cuda, dtype):
+    # more sequences than the longest-first order covers; short ones on the small kernel
+    qs = [1] * 150
+    for i in (0, 77, 149):
+        qs[i] = 40 + i
+    kv = [(29 * i) % 140 + q + 1 for i, q in enumerate(qs)]
+    _attend_case(cuda, qs, kv, 4, 2, 64, 16, dtype, seed=6)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_attend_both_kernels_with_split_contexts(cuda, dtype):
+    # one chunk and 15 decoding sequences, few enough that both kernels split the keys
+    _attend_case(cuda, [64] + [1] * 15, [6000] + [100 * i + 1 for i in range(15)], 4, 1, 64, 64, dtype, seed=7)
 
 
 def test_attend_sequences_may_share_pages(cuda):
@@ -441,6 +464,9 @@ def test_library_refusals_reach_the_caller(cuda):
     with pytest.raises(RuntimeError, match="aligned"):
         odd = torch.zeros(4 * 64 + 8, dtype=BF16, device=cuda)[1:257].view(1, 256)
         c.attend(odd, cu, lens, table, 1, 4)
+    for bounds in ((1 << 32, 4), (1, (1 << 32) + 4)):
+        with pytest.raises(ValueError):
+            c.attend(q, cu, lens, table, *bounds)
     assert c.attend(q[:0], torch.zeros(2, **i32), lens, table, 1, 4).shape == (0, 256)
     assert c.read(table, None, torch.zeros(2, **i32), 0)[0].shape == (0, 2, 64)
     _ok()
@@ -495,6 +521,39 @@ def test_append_then_attend_captured_and_replayed_on_another_stream(cuda, dtype)
         assert torch.equal(out, w)
     assert torch.equal(eager.key_pages, graph.key_pages) and torch.equal(eager.value_pages, graph.value_pages)
     _ok()
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+def test_two_streams_at_once_and_without_dependent_launch(cuda, dtype):
+    """Mixed calls (both kernels and the joins) on two streams, and the same without
+    programmatic dependent launch, give the bits of one call alone."""
+    from bitnet_tt import _lib
+
+    qs, kv = [64] + [1] * 15, [3000] + [200 * i + 1 for i in range(15)]
+    table, n = _pages(kv, 64)
+    c = _cache(cuda, n, 64, 2, 128, dtype, 3)
+    cu, lens, table = _cu(qs).to(cuda), torch.tensor(kv, dtype=torch.int32, device=cuda), table.to(cuda)
+    qq = [torch.randn((sum(qs), 8 * 128), generator=torch.Generator().manual_seed(i)).to(BF16).to(cuda) for i in range(2)]
+    want = [c.attend(q, cu, lens, table, 64, 3000).clone() for q in qq]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.zeros_like(w) for _ in range(8)] for w in want]
+    for r in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                c.attend(qq[i], cu, lens, table, 64, 3000, out=outs[i][r])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in outs[i]:
+            assert torch.equal(o, want[i])
+    _lib.set_pdl(False)
+    try:
+        got = c.attend(qq[0], cu, lens, table, 64, 3000)
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_pdl(True)
+    _ok()
+    assert torch.equal(got, want[0])
 
 
 def test_offsets_beyond_32_bits(cuda):
