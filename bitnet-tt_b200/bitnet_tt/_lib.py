@@ -9,6 +9,7 @@ path has no fallback: if the library cannot be loaded, the first call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -200,6 +201,7 @@ _SIGNATURES = {
 }
 
 _lib = None
+_paged = None
 _lock = threading.Lock()
 
 
@@ -252,11 +254,6 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def stream_handle(stream: torch.cuda.Stream | None = None) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
-
-
-def raw_stream(index: int) -> int:
-    """The current stream of device `index` as a handle, without a Stream object."""
-    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def last_device_status() -> tuple[int, int]:
@@ -539,45 +536,23 @@ def attention_prefill_varlen(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                                                  ptr(out), stream_handle()), "bitnet_attention_prefill_varlen")
 
 
-# The paged cache's calls are short on the GPU (a decode step's append takes 3 us),
-# so these wrappers keep the host's share small: the caller (layers/paged_kv.py)
-# checks its tensors and passes their sizes, the stream comes as the raw handle, and
-# the library is looked up once.  index: the device of the cache, which must be
-# current; b, max_pages: the block table's shape.
-def paged_append(kv: PagedKV, index: int, block_table: torch.Tensor, b: int, max_pages: int, cu_seqlens: torch.Tensor,
-                 kv_lens: torch.Tensor, qkv: torch.Tensor, tokens: int, n_heads: int, rope_cos: torch.Tensor,
-                 rope_sin: torch.Tensor, rope_f32: bool, q_out: torch.Tensor, interleaved: bool = False,
-                 stepwise: bool = False) -> None:
-    rope_len, half = rope_cos.shape
-    st = (_lib or load()).bitnet_paged_append(
-        kv, block_table.data_ptr(), b, max_pages, cu_seqlens.data_ptr(), kv_lens.data_ptr(), qkv.data_ptr(),
-        qkv.stride(0), tokens, n_heads, rope_cos.data_ptr(), rope_sin.data_ptr(), rope_len, 2 * half, rope_f32,
-        interleaved, stepwise, q_out.data_ptr(), raw_stream(index))
-    if st:
-        check(st, "bitnet_paged_append")
-
-
-def paged_read(kv: PagedKV, index: int, block_table: torch.Tensor, b: int, max_pages: int, starts: torch.Tensor | None,
-               cu_rows: torch.Tensor, rows: int, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
-    st = (_lib or load()).bitnet_paged_read(
-        kv, block_table.data_ptr(), b, max_pages, None if starts is None else starts.data_ptr(), cu_rows.data_ptr(),
-        rows, k_out.data_ptr(), v_out.data_ptr(), raw_stream(index))
-    if st:
-        check(st, "bitnet_paged_read")
+def paged_module():
+    """The Python module of the paged cache's calls (csrc/paged_binding.cpp)."""
+    global _paged
+    if _paged is None:
+        load()
+        p = os.path.join(_PKG_DIR, "_paged.so")
+        if not os.path.exists(p):
+            raise RuntimeError(
+                f"{p} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+        spec = importlib.util.spec_from_file_location("bitnet_tt._paged", p)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        _paged = mod
+    return _paged
 
 
 def paged_attention_workspace_bytes(b: int, total_tokens: int, max_seqlen: int, max_kv_len: int, n_heads: int,
                                     n_kv: int, head_dim: int) -> int:
     return int(load().bitnet_paged_attention_workspace_bytes(b, total_tokens, max_seqlen, max_kv_len, n_heads, n_kv,
                                                              head_dim))
-
-
-def paged_attention(kv: PagedKV, index: int, block_table: torch.Tensor, b: int, max_pages: int, cu_seqlens: torch.Tensor,
-                    kv_lens: torch.Tensor, q: torch.Tensor, tokens: int, max_seqlen: int, max_kv_len: int, n_heads: int,
-                    scale: float, workspace: torch.Tensor | None, out: torch.Tensor) -> None:
-    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.nbytes)
-    st = (_lib or load()).bitnet_paged_attention(
-        kv, block_table.data_ptr(), b, max_pages, cu_seqlens.data_ptr(), kv_lens.data_ptr(), q.data_ptr(), q.stride(0),
-        tokens, max_seqlen, max_kv_len, n_heads, scale, ws, ws_bytes, out.data_ptr(), raw_stream(index))
-    if st:
-        check(st, "bitnet_paged_attention")

@@ -19,7 +19,6 @@ lengths live on the device, where a bad one is recorded
 
 from __future__ import annotations
 
-import functools
 from dataclasses import dataclass
 
 import torch
@@ -28,17 +27,6 @@ from .. import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 _INT_MAX = 0x7fffffff
-
-
-class _Current:
-    def __enter__(self) -> None:
-        pass
-
-    def __exit__(self, *_exc) -> None:
-        pass
-
-
-_CURRENT = _Current()
 
 
 @dataclass
@@ -110,51 +98,49 @@ class PagedKVCache:
         self.device = k.device
         self._index = k.get_device()
         self.dtype = k.dtype
-        self._bf16 = k.new_empty(0, dtype=torch.bfloat16)
         self._scale = k.shape[3] ** -0.5
-        self._kv = _lib.PagedKV(_lib.ptr(k), _lib.ptr(v), _lib.ptr(ks), _lib.ptr(vs), *k.shape[0:1], k.shape[2],
-                                k.shape[1], k.shape[3], _lib.KV_INT8 if k.dtype == torch.int8 else _lib.KV_BF16)
+        self._module = _lib.paged_module()
+        self._handle = self._module.cache(
+            *(_lib.ptr(t) or 0 for t in (k, v, ks, vs)), self.num_pages, self.page_size, self.num_kv_heads, self.head_dim,
+            _lib.KV_INT8 if k.dtype == torch.int8 else _lib.KV_BF16, self._index)
 
     def nbytes(self) -> int:
         ts = [t for t in (self.key_pages, self.value_pages, self.key_scale, self.value_scale) if t is not None]
         return sum(t.numel() * t.element_size() for t in ts)
 
-    # ---- checks ------------------------------------------------------------
-    # Each call tests everything in one expression; what is wrong is found out
-    # only when something is.
-    def _index_ok(self, t: torch.Tensor) -> bool:
-        return t.dtype is torch.int32 and t.get_device() == self._index and t.is_contiguous()
-
-    def _rows_ok(self, t: torch.Tensor) -> bool:
-        return t.dtype is torch.bfloat16 and t.get_device() == self._index and t.dim() == 2 and t.stride(1) == 1
-
+    # ---- what is wrong with a call's arguments -------------------------------
+    # The module tests all of them at once; these run when it says that something is
+    # wrong, to say what.
     def _refuse_index(self, block_table: torch.Tensor, **vectors: torch.Tensor) -> None:
         for name, t in {"block_table": block_table, **vectors}.items():
-            if not self._index_ok(t):
+            if t.dtype is not torch.int32 or t.get_device() != self._index or not t.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous int32 tensor on {self.device}")
         if block_table.dim() != 2 or min(block_table.shape) < 1:
             raise ValueError("block_table must be [sequences, pages]")
-        shapes = ", ".join(f"{n} {tuple(t.shape)}" for n, t in vectors.items())
-        raise ValueError(f"{shapes} do not belong to a block_table of {block_table.shape[0]} sequences")
+        b = block_table.shape[0]
+        for name, t in vectors.items():
+            if t.numel() != b + name.startswith("cu_"):
+                raise ValueError(f"{name} of shape {tuple(t.shape)} does not belong to a block_table of {b} sequences")
 
-    def _heads(self, features: int, shared: int, name: str) -> int:
-        heads, rest = divmod(features, self.head_dim)
+    def _refuse_rows(self, t: torch.Tensor, shared: int, name: str) -> int:
+        if t.dtype is not torch.bfloat16 or t.get_device() != self._index or t.dim() != 2 or t.stride(1) != 1:
+            raise ValueError(f"{name} must be bfloat16 rows [tokens, features] on {self.device}")
+        heads, rest = divmod(t.shape[1], self.head_dim)
         heads -= shared
         if rest or heads < 1 or heads % self.num_kv_heads:
-            raise ValueError(f"{name} of {features} features does not hold heads of {self.head_dim} for "
+            raise ValueError(f"{name} of {t.shape[1]} features does not hold heads of {self.head_dim} for "
                              f"{self.num_kv_heads} KV heads")
         return heads
 
-    def _out(self, t: torch.Tensor | None, shape: tuple, name: str) -> torch.Tensor:
-        if t is None:
-            return self._bf16.new_empty(shape)
-        if t.dtype is not torch.bfloat16 or t.get_device() != self._index or t.shape != shape or not t.is_contiguous():
+    def _refuse_out(self, t: torch.Tensor | None, shape: tuple, name: str) -> None:
+        if t is not None and (t.dtype is not torch.bfloat16 or t.get_device() != self._index or t.shape != shape
+                              or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous bfloat16 {shape} on {self.device}")
-        return t
 
-    def _on_device(self):
-        """The cache's device as the current one (nothing to do when it is)."""
-        return _CURRENT if torch._C._cuda_getDevice() == self._index else torch.cuda.device(self._index)
+    def _refuse_rest(self, status: int | None, what: str) -> None:
+        if status is not None:
+            _lib.check(status, what)
+        raise ValueError(f"{what}: an argument is not as documented")
 
     # ---- calls -------------------------------------------------------------
     def append(self, qkv: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
@@ -167,24 +153,18 @@ class PagedKVCache:
         rotary_dim / 2]; rotary_dim may be less than head_dim.  The rotation is
         rounded once; stepwise rounds its products and sums to bf16 too, as the bf16
         model code and the contiguous cache's kernels do."""
-        n, table = kv_lens.numel(), block_table.shape
-        if not (self._index_ok(block_table) and self._index_ok(cu_seqlens) and self._index_ok(kv_lens)
-                and len(table) == 2 and table[0] == n and table[1] and cu_seqlens.numel() == n + 1 and n):
+        r = self._module.append(self._handle, qkv, cu_seqlens, kv_lens, block_table, rope_cos, rope_sin, q_out,
+                                interleaved, stepwise)
+        if r is None or type(r) is int:
             self._refuse_index(block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens)
-        if not self._rows_ok(qkv):
-            raise ValueError(f"qkv must be bfloat16 rows [tokens, features] on {self.device}")
-        tokens, features = qkv.shape
-        heads = self._heads(features, 2 * self.num_kv_heads, "qkv")
-        tab = rope_cos.dtype
-        if not ((tab is torch.float32 or tab is torch.bfloat16) and rope_sin.dtype is tab and rope_cos.dim() == 2
-                and rope_cos.shape == rope_sin.shape and rope_cos.get_device() == self._index
-                and rope_sin.get_device() == self._index and rope_cos.is_contiguous() and rope_sin.is_contiguous()):
-            raise ValueError("rope tables must be two equal contiguous bf16 or fp32 [positions, rotary_dim / 2]")
-        q_out = self._out(q_out, (tokens, heads * self.head_dim), "q_out")
-        with self._on_device():
-            _lib.paged_append(self._kv, self._index, block_table, n, table[1], cu_seqlens, kv_lens, qkv, tokens, heads,
-                              rope_cos, rope_sin, tab is torch.float32, q_out, interleaved, stepwise)
-        return q_out
+            heads = self._refuse_rows(qkv, 2 * self.num_kv_heads, "qkv")
+            for t in (rope_cos, rope_sin):
+                if (t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != rope_cos.dtype or t.dim() != 2
+                        or t.shape != rope_cos.shape or t.get_device() != self._index or not t.is_contiguous()):
+                    raise ValueError("rope tables must be two equal contiguous bf16 or fp32 [positions, rotary_dim / 2]")
+            self._refuse_out(q_out, (qkv.shape[0], heads * self.head_dim), "q_out")
+            self._refuse_rest(r, "bitnet_paged_append")
+        return r
 
     def attend(self, q: torch.Tensor, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor,
                max_seqlen: int, max_kv_len: int, scale: float | None = None, out: torch.Tensor | None = None,
@@ -194,54 +174,40 @@ class PagedKVCache:
         bound the new tokens and the keys of every sequence.  scale: 1 /
         sqrt(head_dim) by default.  workspace (attention_workspace): taken from the
         allocator if not given."""
-        n, table = kv_lens.numel(), block_table.shape
-        if not (self._index_ok(block_table) and self._index_ok(cu_seqlens) and self._index_ok(kv_lens)
-                and len(table) == 2 and table[0] == n and table[1] and cu_seqlens.numel() == n + 1 and n):
+        r = self._module.attend(self._handle, q, cu_seqlens, kv_lens, block_table, max_seqlen, max_kv_len,
+                                self._scale if scale is None else scale, out, workspace)
+        if r is None or type(r) is int:
             self._refuse_index(block_table, cu_seqlens=cu_seqlens, kv_lens=kv_lens)
-        if not self._rows_ok(q):
-            raise ValueError(f"q must be bfloat16 rows [tokens, features] on {self.device}")
-        tokens, features = q.shape
-        heads = self._heads(features, 0, "q")
-        if max_seqlen > _INT_MAX or max_kv_len > _INT_MAX:
-            raise ValueError("max_seqlen and max_kv_len are 32-bit bounds")
-        out = self._out(out, (tokens, features), "out")
-        if workspace is None:
-            workspace = self.attention_workspace(n, tokens, max_seqlen, max_kv_len, heads)
-        elif workspace.get_device() != self._index or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be a contiguous tensor on {self.device}")
-        with self._on_device():
-            _lib.paged_attention(self._kv, self._index, block_table, n, table[1], cu_seqlens, kv_lens, q, tokens, max_seqlen,
-                                 max_kv_len, heads, self._scale if scale is None else scale, workspace, out)
-        return out
+            self._refuse_rows(q, 0, "q")
+            if max(max_seqlen, max_kv_len) > _INT_MAX or min(max_seqlen, max_kv_len) < -_INT_MAX:
+                raise ValueError("max_seqlen and max_kv_len are 32-bit bounds")
+            self._refuse_out(out, tuple(q.shape), "out")
+            if workspace is not None and (workspace.get_device() != self._index or not workspace.is_contiguous()):
+                raise ValueError(f"workspace must be a contiguous tensor on {self.device}")
+            self._refuse_rest(r, "bitnet_paged_attention")
+        return r
 
     def attention_workspace(self, batch: int, total_tokens: int, max_seqlen: int, max_kv_len: int,
                             num_heads: int) -> torch.Tensor | None:
         """Workspace of attend() for these bounds (None when it needs none).  Calls
         that may overlap need one each."""
-        n = _workspace_bytes(self._index, batch, total_tokens, max_seqlen, max_kv_len, num_heads, self.num_kv_heads,
-                             self.head_dim)
-        return self._bf16.new_empty(n // 2) if n else None
+        with torch.cuda.device(self._index):
+            n = _lib.paged_attention_workspace_bytes(batch, total_tokens, max_seqlen, max_kv_len, num_heads,
+                                                     self.num_kv_heads, self.head_dim)
+        return torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
 
     def read(self, block_table: torch.Tensor, starts: torch.Tensor | None, cu_rows: torch.Tensor, total_rows: int,
              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows starts[b] .. starts[b] + cu_rows[b + 1] - cu_rows[b] - 1 of every
         sequence (starts None: from row 0) as packed bf16 keys and values
         [total_rows, n_kv, head_dim]."""
-        n, table = cu_rows.numel() - 1, block_table.shape
-        if not (self._index_ok(block_table) and self._index_ok(cu_rows) and len(table) == 2 and table[0] == n and table[1]
-                and n
-                and (starts is None or (self._index_ok(starts) and starts.numel() == n))):
+        r = self._module.read(self._handle, block_table, starts, cu_rows, total_rows, k_out, v_out)
+        if r is None or type(r) is int:
             self._refuse_index(block_table, cu_rows=cu_rows, **({} if starts is None else {"starts": starts}))
-        if not 0 <= total_rows <= _INT_MAX:
-            raise ValueError("total_rows is out of range")
-        shape = (total_rows, self.num_kv_heads, self.head_dim)
-        k_out, v_out = self._out(k_out, shape, "k_out"), self._out(v_out, shape, "v_out")
-        with self._on_device():
-            _lib.paged_read(self._kv, self._index, block_table, n, table[1], starts, cu_rows, total_rows, k_out, v_out)
-        return k_out, v_out
-
-
-@functools.lru_cache(maxsize=1024)
-def _workspace_bytes(index: int, *sizes: int) -> int:
-    with torch.cuda.device(index):
-        return _lib.paged_attention_workspace_bytes(*sizes)
+            if not 0 <= total_rows <= _INT_MAX:
+                raise ValueError("total_rows is out of range")
+            shape = (total_rows, self.num_kv_heads, self.head_dim)
+            self._refuse_out(k_out, shape, "k_out")
+            self._refuse_out(v_out, shape, "v_out")
+            self._refuse_rest(r, "bitnet_paged_read")
+        return r

@@ -97,13 +97,12 @@ def test_workspace_size_follows_from_the_sizes_alone():
 
 @pytest.fixture
 def host_cache(monkeypatch):
-    """A cache over host tensors: its checks run, the library must not be reached."""
+    """A cache over host tensors: the module refuses them, and the checks say why.
+    Good arguments but for their device are the last check's."""
     from bitnet_tt import _lib
     from bitnet_tt.layers import PagedKVCache
 
     monkeypatch.setattr(_lib, "ptr", lambda t: None if t is None else t.data_ptr())
-    for f in ("paged_append", "paged_read", "paged_attention"):
-        monkeypatch.setattr(_lib, f, lambda *a, **k: pytest.fail("the call was not refused"))
     k = torch.zeros((8, 2, 16, 64), dtype=torch.bfloat16)
     return PagedKVCache.from_tensors(k, k.clone())
 
@@ -132,6 +131,26 @@ def test_cache_checks_its_pools():
         PagedKVCache(8, 16, 2, 64, "cpu", torch.float16)
 
 
+def test_host_tensors_are_refused(host_cache):
+    g = _good()
+    for call in (lambda: host_cache.append(g["qkv"], g["cu"], g["lens"], g["table"], g["cos"], g["sin"]),
+                 lambda: host_cache.attend(g["q"], g["cu"], g["lens"], g["table"], 2, 64),
+                 lambda: host_cache.read(g["table"], None, g["cu"], 5)):
+        with pytest.raises(ValueError, match="not as documented"):
+            call()
+    for call in (lambda: host_cache.attend(g["q"], g["cu"], g["lens"], g["table"], 2, "64"),
+                 lambda: host_cache.attend(g["q"], g["cu"], g["lens"], g["table"], 2, 64, scale="1")):
+        with pytest.raises((TypeError, ValueError)):
+            call()
+
+
+def _specific(call, **over):
+    """Refused with a reason of its own."""
+    with pytest.raises(ValueError) as e:
+        call(**over)
+    assert "not as documented" not in str(e.value), over
+
+
 def test_append_checks_its_arguments(host_cache):
     def call(**over):
         g = _good() | over
@@ -146,8 +165,7 @@ def test_append_checks_its_arguments(host_cache):
                  {"cos": z((64, 32), dtype=torch.float64), "sin": z((64, 32), dtype=torch.float64)},
                  {"cos": z((64, 16))}, {"sin": z((64, 32), dtype=torch.bfloat16)},
                  {"q_out": z((3, 256))}, {"q_out": z((4, 256), dtype=torch.bfloat16)}]:
-        with pytest.raises(ValueError):
-            call(**over)
+        _specific(call, **over)
 
 
 def test_attend_and_read_check_their_arguments(host_cache):
@@ -163,9 +181,7 @@ def test_attend_and_read_check_their_arguments(host_cache):
     for over in [{"q": z((3, 256))}, {"q": z((3, 192), dtype=torch.bfloat16)}, {"q": z((3, 100), dtype=torch.bfloat16)},
                  {"q": z(256, dtype=torch.bfloat16)}, {"cu": z(2, dtype=torch.int32)}, {"lens": z(2)},
                  {"out": z((3, 128), dtype=torch.bfloat16)}, {"out": z((3, 512), dtype=torch.bfloat16)[:, :256]}]:
-        with pytest.raises(ValueError):
-            attend(**over)
+        _specific(attend, **over)
     for over in [{"cu": z(4, dtype=torch.int32)}, {"starts": z(3, dtype=torch.int32)}, {"starts": z(2)}, {"total": -1},
                  {"k_out": z((5, 2, 128), dtype=torch.bfloat16)}, {"v_out": z((5, 2, 64))}]:
-        with pytest.raises(ValueError):
-            read(**over)
+        _specific(read, **over)
