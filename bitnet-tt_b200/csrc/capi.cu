@@ -1327,7 +1327,9 @@ int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspa
     if (int e = paged_map(&mk, p.kv, p.kv.k, D, I8)) return e;
     if (int e = paged_map(&mv, p.kv, p.kv.v, D, I8)) return e;
     paged_apply(&p, pl.chunk, workspace);
-    if (int e = launch(k, dim3(p.blocks, p.kv.n_kv, p.nsplit), dim3(S::THREADS), S::SMEM, st, 1, p, mk, mv)) return e;
+    const long long ctas = (long long)p.blocks * p.nsplit * p.kv.n_kv;
+    if (ctas > INT_MAX) return BITNET_ERR_INVALID_ARGUMENT;
+    if (int e = launch(k, dim3((unsigned)ctas), dim3(S::THREADS), S::SMEM, st, 1, p, mk, mv)) return e;
   }
   PagedAttnParams pr = p;
   if (pl.rows.blocks > 0) {

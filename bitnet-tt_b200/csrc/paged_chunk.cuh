@@ -236,22 +236,20 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   }
   pdl_wait();
   pdl_trigger();  // after the wait: the rows kernel may then start without one of its own
-  // Only now: the kernel before this one may need tensor memory to end.
+  // Blocks vary slowest: CTAs start in this order, and the longest blocks of all heads come first.
+  const int g = blockIdx.x % p.kv.n_kv, bs = blockIdx.x / p.kv.n_kv, bx = bs / p.nsplit, sp = bs - bx * p.nsplit;
+  PagedBlock blk;
+  if (!paged_block_search<PCH_R>(p, bx, lane, blk)) return;
+  const int nparts = paged_parts(p, blk.kend);
+  if (sp >= nparts) return;
+  // After pdl_wait: the kernel before this one may need tensor memory to end.
   if (warp == 8) {
     tmem_alloc(&ctrl->tmem, 512);
     tmem_relinquish();
   }
-  const int bx = blockIdx.x, g = blockIdx.y, sp = blockIdx.z;
-  PagedBlock blk;
-  const bool found = paged_block_search<PCH_R>(p, bx, lane, blk);
-  const int nparts = found ? paged_parts(p, blk.kend) : 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (sp >= nparts) {
-    if (warp == 8) tmem_dealloc(0, 512);
-    return;
-  }
   const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);
   // 64-key steps of the two row tiles (the second sees at least the first's keys)
   const int end0 = min(k1, max(0, blk.past + (blk.row0 + min(blk.nrows, 128) - 1) / p.G + 1));
