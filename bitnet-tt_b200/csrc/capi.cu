@@ -1174,7 +1174,7 @@ int launch_paged_append(const PagedAppendParams& p, bool f32, dim3 grid, bitnet_
 // launched) and parts of the keys, and where its partial results lie.
 struct PagedCut {
   int blocks, nsplit, span;
-  size_t ml, o;  // offsets in the workspace
+  size_t ml, o, found;  // offsets in the workspace
 };
 constexpr int PAGED_ROWS_MOST = 32;
 struct PagedPlan {
@@ -1219,7 +1219,8 @@ PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, 
     const size_t rows = c.nsplit > 1 ? (size_t)c.nsplit * c.blocks * n_kv * R : 0;
     c.ml = at;
     c.o = c.ml + rows * sizeof(float2);
-    at = c.o + rows * D * sizeof(float);
+    c.found = c.o + rows * D * sizeof(float);
+    at = c.found + (R == PCH_R && rows ? round_up(c.blocks * sizeof(PagedBlock), 16) : 0);
   };
   const long long rows = (long long)max_q * G;
   const int most_rows = PAGED_ROWS_MOST;
@@ -1286,6 +1287,7 @@ void paged_apply(PagedAttnParams* p, const PagedCut& c, void* workspace) {
   p->span = c.span;
   p->part_ml = (float2*)((uint8_t*)workspace + c.ml);
   p->part_o = (float*)((uint8_t*)workspace + c.o);
+  p->found = (PagedBlock*)((uint8_t*)workspace + c.found);
 }
 
 template <int D, int R, int W>
@@ -1337,8 +1339,9 @@ int launch_paged_attention(PagedAttnParams p, const PagedPlan& pl, void* workspa
     pr.beside = pl.chunk.blocks > 0;
     if (int e = pl.r == 8 ? launch_paged_rows<D, I8, 1>(pr, st) : launch_paged_rows<D, I8, 2>(pr, st)) return e;
   }
-  if (pl.chunk.blocks > 0)
-    if (int e = launch_paged_join<D, PCH_R, 1>(p, st)) return e;
+  if (pl.chunk.blocks > 0 && p.nsplit > 1)
+    if (int e = launch(paged_chunk_join_kernel<D, PCH_R>, dim3(p.blocks, p.kv.n_kv, PCH_R / (4 * PJC_N)), dim3(128), 0, st, 1, p))
+      return e;
   if (pl.rows.blocks > 0)
     return pl.r == 8 ? launch_paged_join<D, 8, 4>(pr, st) : launch_paged_join<D, 16, 4>(pr, st);
   return BITNET_OK;

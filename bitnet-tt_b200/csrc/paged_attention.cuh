@@ -19,6 +19,14 @@
 
 namespace bitnet {
 
+// One block of rows: rows row0 .. row0 + nrows - 1 of sequence b.
+struct PagedBlock {
+  int b, row0, nrows;
+  int tok0;    // the sequence's first packed token
+  int past;    // kv_len - n: keys before the new tokens (may be negative)
+  int kend;    // keys that the block's last row sees, not below 0
+};
+
 struct PagedAttnParams {
   PagedKV kv;
   const int32_t* cu;
@@ -34,15 +42,8 @@ struct PagedAttnParams {
   int beside;          // rows kernel: launched after the chunk kernel, to run beside it
   float2* part_ml;     // [nsplit][blocks][n_kv][R] (maximum, sum)
   float* part_o;       // [nsplit][blocks][n_kv][R][D], unnormalised
+  PagedBlock* found;   // chunk kernel with nsplit > 1: [blocks], nrows 0 where there is none
   uint16_t* out;       // [tokens][n_heads * D]
-};
-
-// One block of rows: rows row0 .. row0 + nrows - 1 of sequence b.
-struct PagedBlock {
-  int b, row0, nrows;
-  int tok0;    // the sequence's first packed token
-  int past;    // kv_len - n: keys before the new tokens (may be negative)
-  int kend;    // keys that the block's last row sees, not below 0
 };
 
 // Rows row0 .. of sequence b, which has n new tokens from packed row lo on and kv
@@ -681,10 +682,10 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
 // ---------------------------------------------------------------------------
 // joining the parts
 // ---------------------------------------------------------------------------
-// W warps a row, each the parts w, w + W, ...: they weigh the parts'
-// unnormalised outputs by exp2(m_part - max).  A block whose keys fit in one
-// part was written by its own CTA.  A few rows in many parts take W = 4, so that
-// the chain of loads is short; many rows in few parts W = 1.
+// Parts' unnormalised outputs are weighed by exp2(m_part - max).  A block whose
+// keys fit in one part was written by its own CTA.  The rows kernel's few rows in
+// many parts: W warps a row, each the parts w, w + W, ..., so that the chain of
+// loads is short.
 template <int D, int R, int W>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p) {
   constexpr int V = D / 32;
@@ -694,8 +695,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
   pdl_trigger();
   pdl_wait();
   PagedBlock blk;
-  if (!(R <= 16 ? paged_block_direct<R>(p, blockIdx.x, lane, blk) : paged_block_search<R>(p, blockIdx.x, lane, blk)))
-    return;
+  if (!paged_block_direct<R>(p, blockIdx.x, lane, blk)) return;
   const int nparts = paged_parts(p, blk.kend);
   if (nparts == 1) return;
   const size_t step = (size_t)p.blocks * p.kv.n_kv;
@@ -737,6 +737,77 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnParams p
       p.out + ((size_t)(blk.tok0 + tok) * p.n_heads + g * p.G + row - tok * p.G) * D + lane * V);
 #pragma unroll
   for (int e = 0; e < V / 2; ++e) dst[e] = bf2_of(num[2 * e] * inv, num[2 * e + 1] * inv);
+}
+
+template <int V>
+__device__ __forceinline__ void load_f(const float* src, float* x) {
+  if constexpr (V == 4) {
+    const float4 v = *reinterpret_cast<const float4*>(src);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const float2 v = *reinterpret_cast<const float2*>(src);
+    x[0] = v.x, x[1] = v.y;
+  }
+}
+
+// The chunk kernel's blocks of R rows in few parts: N rows a warp, whose loads do
+// not wait for one another.  The blocks are as the chunk kernel found them (a
+// search of its own in each of these short CTAs cost 80 us where the parts' bytes
+// take 20).
+constexpr int PJC_N = 4;
+template <int D, int R>
+__global__ void __launch_bounds__(128) paged_chunk_join_kernel(const PagedAttnParams p) {
+  constexpr int V = D / 32, N = PJC_N;
+  const int lane = threadIdx.x & 31, g = blockIdx.y;
+  const int r0 = (blockIdx.z * 4 + (threadIdx.x >> 5)) * N;
+  pdl_trigger();
+  pdl_wait();
+  const PagedBlock blk = p.found[blockIdx.x];
+  if (r0 >= blk.nrows) return;
+  const int nparts = paged_parts(p, blk.kend);
+  if (nparts == 1) return;
+  const size_t step = (size_t)p.blocks * p.kv.n_kv;
+  const size_t pb = (size_t)blockIdx.x * p.kv.n_kv + g;
+  float num[N][V], den[N], M[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    den[k] = 0.f;
+    M[k] = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < V; ++e) num[k][e] = 0.f;
+  }
+  // rows past the block's last read the last one's parts and are not stored
+  for (int s = lane; s < nparts; s += 32)
+#pragma unroll
+    for (int k = 0; k < N; ++k) M[k] = fmaxf(M[k], p.part_ml[(pb + s * step) * R + min(r0 + k, blk.nrows - 1)].x);
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M[k] = fmaxf(M[k], __shfl_xor_sync(0xffffffffu, M[k], o));
+#pragma unroll 2
+  for (int s = 0; s < nparts; ++s) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const size_t at = (pb + s * step) * R + min(r0 + k, blk.nrows - 1);
+      const float2 ml = p.part_ml[at];
+      float x[V];
+      load_f<V>(p.part_o + at * D + lane * V, x);
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - M[k]);
+      den[k] = fmaf(ml.y, f, den[k]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) num[k][e] = fmaf(x[e], f, num[k][e]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (r0 + k >= blk.nrows) break;
+    const float inv = M[k] == -INFINITY ? 0.f : 1.f / den[k];
+    const int row = blk.row0 + r0 + k, tok = row / p.G;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(
+        p.out + ((size_t)(blk.tok0 + tok) * p.n_heads + g * p.G + row - tok * p.G) * D + lane * V);
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) dst[e] = bf2_of(num[k][2 * e] * inv, num[k][2 * e + 1] * inv);
+  }
 }
 
 }  // namespace bitnet

@@ -239,7 +239,12 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   // Blocks vary slowest: CTAs start in this order, and the longest blocks of all heads come first.
   const int g = blockIdx.x % p.kv.n_kv, bs = blockIdx.x / p.kv.n_kv, bx = bs / p.nsplit, sp = bs - bx * p.nsplit;
   PagedBlock blk;
-  if (!paged_block_search<PCH_R>(p, bx, lane, blk)) return;
+  const bool found = paged_block_search<PCH_R>(p, bx, lane, blk);
+  if (p.nsplit > 1 && sp == 0 && g == 0 && tid == 0) {  // for the join
+    if (!found) blk.nrows = 0;
+    p.found[bx] = blk;
+  }
+  if (!found) return;
   const int nparts = paged_parts(p, blk.kend);
   if (sp >= nparts) return;
   // After pdl_wait: the kernel before this one may need tensor memory to end.
