@@ -84,71 +84,74 @@ __device__ __forceinline__ bool paged_block_direct(const PagedAttnParams& p, int
 // with at least that many by arithmetic (a sequence's later blocks see more).
 // Equal ranks are in the order of sequences.  Up to 128 sequences; beyond that the
 // blocks are in the order of sequences alone, the last first.
+// C: sequences of a lane; cold code, so the common case has its own shorter copy.
+template <int R, int C>
+__device__ __forceinline__ bool paged_block_ranked(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
+  int at[C], len[C], kv[C], rows[C], past[C], nb = 0;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int b = 32 * c + lane;
+    at[c] = len[c] = kv[c] = rows[c] = past[c] = 0;
+    if (b < p.B) {
+      at[c] = p.cu[b];
+      len[c] = p.cu[b + 1] - at[c];
+      kv[c] = p.kv_lens[b];
+      const int n = min(max(len[c], 0), p.max_q);
+      past[c] = min(kv[c], p.max_kv) - n;
+      rows[c] = n * p.G > p.small ? n * p.G : 0;
+      nb += (rows[c] + R - 1) / R;
+    }
+  }
+  // the blocks of at least t tiles of sequence c: those whose last row's token is y or later
+  auto count = [&](int c, int t) {
+    const int all = (rows[c] + R - 1) / R;
+    const long long y = (long long)(t - 1) * 128 - past[c];
+    if (t <= 0 || y <= 0 || all == 0) return all;
+    const long long first = y * p.G;  // the first row of token y
+    return first >= rows[c] ? 0 : all - (int)(first / R);
+  };
+  auto total = [&](int t) {
+    int n = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (32 * c < p.B) n += count(c, t);
+    return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+  };
+  if (bx >= (int)__reduce_add_sync(0xffffffffu, (unsigned)nb)) return false;
+  int lo = 0, hi = (p.max_kv + 127) / 128 + 1;  // more than bx blocks have lo tiles, not more have hi
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (total(mid) > bx) lo = mid;
+    else hi = mid;
+  }
+  // among the blocks of exactly lo tiles
+  int rank = bx - total(lo + 1);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (32 * c >= p.B) break;
+    const int above = count(c, lo + 1), here = count(c, lo) - above;
+    int sum = here;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, sum > rank);
+    if (over) {
+      const int src = __ffs(over) - 1;
+      rank -= __shfl_sync(0xffffffffu, sum - here, src);
+      const int last = __shfl_sync(0xffffffffu, (rows[c] + R - 1) / R - 1 - above, src);
+      return paged_block_of<R>(p, 32 * c + src, __shfl_sync(0xffffffffu, at[c], src), __shfl_sync(0xffffffffu, len[c], src),
+                               __shfl_sync(0xffffffffu, kv[c], src), (last - rank) * R, lane, o);
+    }
+    rank -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
 template <int R>
 __device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int bx, int lane, PagedBlock& o) {
-  constexpr int C = 4;  // sequences of a lane
-  if (p.B <= 32 * C) {
-    int at[C], len[C], kv[C], rows[C], past[C], nb = 0;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int b = 32 * c + lane;
-      at[c] = len[c] = kv[c] = rows[c] = past[c] = 0;
-      if (b < p.B) {
-        at[c] = p.cu[b];
-        len[c] = p.cu[b + 1] - at[c];
-        kv[c] = p.kv_lens[b];
-        const int n = min(max(len[c], 0), p.max_q);
-        past[c] = min(kv[c], p.max_kv) - n;
-        rows[c] = n * p.G > p.small ? n * p.G : 0;
-        nb += (rows[c] + R - 1) / R;
-      }
-    }
-    // the blocks of at least t tiles of sequence c: those whose last row's token is y or later
-    auto count = [&](int c, int t) {
-      const int all = (rows[c] + R - 1) / R;
-      const long long y = (long long)(t - 1) * 128 - past[c];
-      if (t <= 0 || y <= 0 || all == 0) return all;
-      const long long first = y * p.G;  // the first row of token y
-      return first >= rows[c] ? 0 : all - (int)(first / R);
-    };
-    auto total = [&](int t) {
-      int n = 0;
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        if (32 * c < p.B) n += count(c, t);
-      return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
-    };
-    if (bx >= (int)__reduce_add_sync(0xffffffffu, (unsigned)nb)) return false;
-    int lo = 0, hi = (p.max_kv + 127) / 128 + 1;  // more than bx blocks have lo tiles, not more have hi
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (total(mid) > bx) lo = mid;
-      else hi = mid;
-    }
-    // among the blocks of exactly lo tiles
-    int rank = bx - total(lo + 1);
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      if (32 * c >= p.B) break;
-      const int above = count(c, lo + 1), here = count(c, lo) - above;
-      int sum = here;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += v;
-      }
-      const unsigned over = __ballot_sync(0xffffffffu, sum > rank);
-      if (over) {
-        const int src = __ffs(over) - 1;
-        rank -= __shfl_sync(0xffffffffu, sum - here, src);
-        const int last = __shfl_sync(0xffffffffu, (rows[c] + R - 1) / R - 1 - above, src);
-        return paged_block_of<R>(p, 32 * c + src, __shfl_sync(0xffffffffu, at[c], src), __shfl_sync(0xffffffffu, len[c], src),
-                                 __shfl_sync(0xffffffffu, kv[c], src), (last - rank) * R, lane, o);
-      }
-      rank -= __shfl_sync(0xffffffffu, sum, 31);
-    }
-    return false;
-  }
+  if (p.B <= 32) return paged_block_ranked<R, 1>(p, bx, lane, o);
+  if (p.B <= 128) return paged_block_ranked<R, 4>(p, bx, lane, o);
   bx = p.blocks - 1 - bx;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int i = b0 + lane;

@@ -133,7 +133,8 @@ struct PchCtrl {
   uint64_t o_done[2][2], drain[2], tail, q_full, v_full;  // o_done: O_t holds the step
   uint32_t tmem;
   int abort_flag;
-  uint32_t v_top[8];  // int8: the largest value scale of the part, by its bits, as each softmax warp saw it
+  uint32_t v_top[4];  // int8: the largest value scale of the part, by its bits, as each converting warp saw it
+  PagedBlock block;   // nrows 0: none
 };
 static_assert(sizeof(PchCtrl) <= 512, "control block");
 
@@ -192,7 +193,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
 }
 __device__ __forceinline__ uint32_t pch_v_top(const PchCtrl* c) {
   uint32_t t = c->v_top[0];
-  for (int i = 1; i < 8; ++i) t = max(t, c->v_top[i]);
+  for (int i = 1; i < 4; ++i) t = max(t, c->v_top[i]);
   return t;
 }
 
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     }
     mbar_init(&ctrl->tail, 1);
     mbar_init(&ctrl->q_full, 8);
-    mbar_init(&ctrl->v_full, 8);
+    mbar_init(&ctrl->v_full, 4);
     ctrl->abort_flag = 0;
     fence_mbar_init();
   }
@@ -238,23 +239,27 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   pdl_trigger();  // after the wait: the rows kernel may then start without one of its own
   // Blocks vary slowest: CTAs start in this order, and the longest blocks of all heads come first.
   const int g = blockIdx.x % p.kv.n_kv, bs = blockIdx.x / p.kv.n_kv, bx = bs / p.nsplit, sp = bs - bx * p.nsplit;
-  PagedBlock blk;
-  const bool found = paged_block_search<PCH_R>(p, bx, lane, blk);
-  if (p.nsplit > 1 && sp == 0 && g == 0 && tid == 0) {  // for the join
-    if (!found) blk.nrows = 0;
-    p.found[bx] = blk;
-  }
-  if (!found) return;
-  const int nparts = paged_parts(p, blk.kend);
-  if (sp >= nparts) return;
-  // After pdl_wait: the kernel before this one may need tensor memory to end.
+  // One warp searches: the code is cold, and all warps at it took longer than one and the exchange.
+  // Tensor memory after pdl_wait: the kernel before this one may need it to end.
   if (warp == 8) {
-    tmem_alloc(&ctrl->tmem, 512);
-    tmem_relinquish();
+    PagedBlock found;
+    if (!paged_block_search<PCH_R>(p, bx, lane, found)) found.nrows = 0;
+    if (lane == 0) {
+      ctrl->block = found;
+      if (p.nsplit > 1 && sp == 0 && g == 0) p.found[bx] = found;  // for the join
+    }
+    if (found.nrows > 0 && sp < paged_parts(p, found.kend)) {
+      tmem_alloc(&ctrl->tmem, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const PagedBlock blk = ctrl->block;
+  if (blk.nrows == 0) return;
+  const int nparts = paged_parts(p, blk.kend);
+  if (sp >= nparts) return;
   const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);
   // 64-key steps of the two row tiles (the second sees at least the first's keys)
   const int end0 = min(k1, max(0, blk.past + (blk.row0 + min(blk.nrows, 128) - 1) / p.G + 1));
@@ -362,7 +367,23 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         if (!convert(2 * j, 0)) break;
         sm_scale[(j % S::RING) * 128 + 32 * w + lane] = ks;
         arrive(2 * j);
-        if (j == 0) {
+        if (j == 0) {  // the largest value scale of the part's rows, four rows (of one page) a load
+          float top = 0.f;
+#pragma unroll 4
+          for (int key = k0 + 4 * (32 * w + lane); key < k1; key += 512) {
+            const int at = table[key >> p.kv.page_shift];
+            if (at < 0 || at >= p.kv.num_pages) continue;  // reported by the loader
+            const float4 v = *reinterpret_cast<const float4*>(p.kv.vs + paged_row(p.kv, at, g, key & slot_mask));
+            top = fmaxf(top, v.x);
+            if (key + 1 < k1) top = fmaxf(top, v.y);
+            if (key + 2 < k1) top = fmaxf(top, v.z);
+            if (key + 3 < k1) top = fmaxf(top, v.w);
+          }
+          const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+          if (lane == 0) {
+            ctrl->v_top[w] = most;
+            mbar_arrive(&ctrl->v_full);
+          }
           if (!__all_sync(0xffffffffu, wait(&ctrl->v_full, 0, 376))) break;
           v_up = __uint_as_float(pow2_field(pch_v_top(ctrl), 7) << 23);
         }
@@ -553,25 +574,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&ctrl->q_full);
-    if (I8) {  // the largest value scale of the part's rows, four rows (of one page) a load
-      const int32_t* table = p.kv.table + (size_t)blk.b * p.kv.max_pages;
-      float top = 0.f;
-#pragma unroll 4
-      for (int key = k0 + 4 * tid; key < k1; key += 1024) {
-        const int page = table[key >> p.kv.page_shift];
-        if (page < 0 || page >= p.kv.num_pages) continue;  // reported by the loads of the rows
-        const float4 v = *reinterpret_cast<const float4*>(
-            p.kv.vs + paged_row(p.kv, page, g, key & ((1 << p.kv.page_shift) - 1)));
-        top = fmaxf(top, v.x);
-        if (key + 1 < k1) top = fmaxf(top, v.y);
-        if (key + 2 < k1) top = fmaxf(top, v.z);
-        if (key + 3 < k1) top = fmaxf(top, v.w);
-      }
-      const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-      if (lane == 0) {
-        ctrl->v_top[warp] = most;
-        mbar_arrive(&ctrl->v_full);
-      }
+    if (I8) {
       // sm_fac is read across warps
       named_bar_sync(1, 256);
     }
@@ -688,8 +691,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       const size_t pr = (((size_t)sp * p.blocks + bx) * p.kv.n_kv + g) * PCH_R + r;
       if (live && nparts > 1) p.part_ml[pr] = make_float2(m - S::LIFT, l);
-      if (I8) wait(&ctrl->v_full, 0, 377);  // complete: every warp arrived before the barrier above
-      const float vf = I8 ? __uint_as_float((254u - pow2_field(pch_v_top(ctrl), 7)) << 23) : 1.f;  // the values' power of two
+      if (I8 && nt > 0) wait(&ctrl->v_full, 0, 377);  // complete: the values were converted after it
+      const float vf = I8 && nt > 0 ? __uint_as_float((254u - pow2_field(pch_v_top(ctrl), 7)) << 23) : 1.f;  // the values' power of two
       uint16_t* dst = p.out + ((size_t)(blk.tok0 + tok) * p.n_heads + g * p.G + row - tok * p.G) * D;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {

@@ -538,6 +538,7 @@ def test_two_streams_at_once_and_without_dependent_launch(cuda, dtype):
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
     outs = [[torch.zeros_like(w) for _ in range(8)] for w in want]
+    torch.cuda.synchronize()  # the zeros are the default stream's
     for r in range(8):
         for i, st in enumerate(streams):
             with torch.cuda.stream(st):
