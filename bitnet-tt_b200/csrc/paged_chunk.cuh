@@ -10,7 +10,11 @@
 // the next step is there when the softmax of one is done, and neither waits for
 // the other: with one S of 128 keys a tile, the products that follow a softmax and
 // the signals between them (about 1300 cycles) stood in every step's chain, and
-// two 4096-token chunks over 16384 keys took 690 us.  The price is that 64-key
+// two 4096-token chunks over 16384 keys took 690 us (576 now, 1190 TFLOP/s; int8
+// 802).  What bounds a step now (1670 cycles, int8 2150) is a tile's softmax chain
+// beside the MMAs: 190 until it sees the scores, 230 to load them, 330 for the
+// maximum, 790 for exponentials, sums and P; the MMAs alone take 1280 and the
+// softmax of both tiles alone 1000.  The price of short steps is that 64-key
 // score products read Q twice as often: 48 cycles each (shared memory's rate)
 // instead of half of 64.
 // Roles, one warp each unless said otherwise:
