@@ -14,6 +14,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
@@ -111,14 +112,12 @@ int heads_of(int64_t features, int shared, const Cache& c) {
   return n >= 1 && n % c.kv.n_kv_heads == 0 ? (int)n : 0;
 }
 
+// C++ exceptions as torch's own calls raise them (an allocation that fails: torch.OutOfMemoryError).
 template <typename F>
 PyObject* guarded(F f) {
-  try {
-    return f();
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  HANDLE_TH_ERRORS
+  return f();
+  END_HANDLE_TH_ERRORS
 }
 template <typename F>
 PyObject* launched(PyObject* result, F call) {

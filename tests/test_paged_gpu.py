@@ -738,3 +738,24 @@ def test_paged_generator_refusals(cuda):
     gen.release(s)
     assert gen.step() == {}
     assert len(gen.generate([[1, 2, 3], [4]], 3)[1]) == 3
+
+
+def test_allocation_that_fails_is_torchs_error(cuda):
+    """The calls' own outputs come from torch's allocator and fail as its do; the
+    cache works on."""
+    c = _cache(cuda, 4, 16, 2, 64, BF16, 1)
+    tokens = 1 << 19
+    q = torch.zeros((1, 2 * 64), dtype=BF16, device=cuda).expand(tokens, -1)  # the output: 128 MiB
+    table, n = _pages([16], 16)
+    args = (_cu([0]).to(cuda), torch.tensor([16], dtype=torch.int32, device=cuda), table.to(cuda))
+    torch.cuda.empty_cache()
+    used = torch.cuda.memory_reserved(cuda)
+    torch.cuda.set_per_process_memory_fraction((used + (64 << 20)) / torch.cuda.get_device_properties(cuda).total_memory, cuda)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            c.attend(q, *args, 1, 16)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0, cuda)
+    assert c.attend(q[:16].contiguous(), *args, 1, 16).shape == (16, 128)  # rows a stride of 0 apart are refused
+    torch.cuda.synchronize()
+    _ok()
