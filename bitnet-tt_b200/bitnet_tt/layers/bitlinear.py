@@ -10,32 +10,16 @@ Mirrors the reference's src/bitnet_tt/layers/bitlinear.py:
     (reference bitlinear.py:356-461).
 Only the packed_ternary weight dtype exists here: the weights live in the 2-bit
 device layout and __call__ runs the fused RMSNorm + int8 quant + ternary
-contraction + scale kernels (bitnet_act_quant + bitnet_bitlinear_q).
+contraction + scale kernels (bitnet_bitlinear).
 """
 
 from __future__ import annotations
-
-import threading
 
 import numpy as np
 import torch
 
 from .. import _lib
 from ..utils.quantization import weight_quant_ternary
-
-_WS_LOCK = threading.Lock()
-_WORKSPACES: dict[tuple, _lib.ActBuffers] = {}
-
-
-def _workspace(m: int, k: int, device: torch.device) -> _lib.ActBuffers:
-    """Activation buffers shared by eager Linear calls (keyed by shape and device)."""
-    key = (device.index, m, k)
-    with _WS_LOCK:
-        ws = _WORKSPACES.get(key)
-        if ws is None:
-            ws = _lib.ActBuffers(m, k, device)
-            _WORKSPACES[key] = ws
-    return ws
 
 
 def quantize_ternary(weight) -> tuple[torch.Tensor, float]:
@@ -158,13 +142,14 @@ class Linear:
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.in_features).to(torch.bfloat16).contiguous()
         m = x2.shape[0]
-        ws = _workspace(m, self.in_features, x2.device)
+        # From the stream-ordered allocator, call by call: buffers shared between calls would be written by
+        # two streams at once, and token counts that vary would keep one set each for good.
+        bufs = _lib.ActBuffers(m, self.in_features, x2.device)
         gamma = norm_weight.reshape(-1).to(torch.bfloat16).contiguous() if norm_weight is not None else None
         eps = 1e-5 if norm_epsilon is None else float(norm_epsilon)
-        _lib.act_quant(x2, gamma, eps, ws)
         y = torch.empty((m, self.output_features), dtype=torch.bfloat16, device=x2.device)
         res = residual.reshape(m, -1).contiguous() if residual is not None else None
-        self.forward_into(ws, m, y, residual=res)
+        self.forward_fused(x2, gamma, eps, bufs, y, residual=res)
         return y.reshape(*lead, self.output_features)
 
 
