@@ -240,11 +240,12 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     fence_mbar_init();
   }
   pdl_wait();
-  pdl_trigger();  // after the wait: the rows kernel may then start without one of its own
+  if (tid == 0) __threadfence();  // what the wait made visible, before the trigger below lets the rows kernel start
   // Blocks vary slowest: CTAs start in this order, and the longest blocks of all heads come first.
   const int g = blockIdx.x % p.kv.n_kv, bs = blockIdx.x / p.kv.n_kv, bx = bs / p.nsplit, sp = bs - bx * p.nsplit;
   // One warp searches: the code is cold, and all warps at it took longer than one and the exchange.
-  // Tensor memory after pdl_wait: the kernel before this one may need it to end.
+  // Tensor memory after pdl_wait: the kernel before this one may need it to end.  And before
+  // pdl_trigger: a later kernel may take its own ahead of its wait for this one.
   if (warp == 8) {
     PagedBlock found;
     if (!paged_block_search<PCH_R>(p, bx, lane, found)) found.nrows = 0;
@@ -260,6 +261,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();
   const PagedBlock blk = ctrl->block;
   if (blk.nrows == 0) return;
   const int nparts = paged_parts(p, blk.kend);
