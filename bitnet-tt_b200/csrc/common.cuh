@@ -194,6 +194,9 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 // Allow the next kernel in the stream to begin its prologue.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Orders what this thread has seen before what it does next, for the whole GPU.
+__device__ __forceinline__ void fence_acq_rel_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------
 // cluster helpers (distributed shared memory)
 // ---------------------------------------------------------------------------

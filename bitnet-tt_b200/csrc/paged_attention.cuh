@@ -301,13 +301,13 @@ __global__ void __launch_bounds__(PRA_THREADS, 3) paged_rows_kernel(const PagedA
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   const int g = blockIdx.y, sp = blockIdx.z;
-  // Beside the chunk kernel there is nothing to wait for: each of its CTAs waits for what came before,
-  // and fences, ahead of the trigger that allows this launch.  The trigger itself publishes nothing, so
-  // this side fences too: whatever stands in this SM's L1 from before is dropped, and the loads below
+  // Beside the chunk kernel there is nothing to wait for: its CTAs wait for what came before, and the
+  // first one fences, ahead of the triggers that allow this launch.  A trigger publishes nothing, so this
+  // side fences too: whatever stands in this SM's L1 from before is dropped, and the loads below
   // find in L2 what the chunk kernel's wait made visible.  (With a wait for the chunk kernel instead, 3
   // chunks of 1024 beside 45 int8 decode rows take 148 us for 133, 4 of 256 beside 60 in bf16 76 for 48.)
   // The last CTA waits for the chunk kernel before it ends, so that what follows this kernel follows both.
-  if (p.beside) __threadfence();
+  if (p.beside) fence_acq_rel_gpu();
   else pdl_wait();
   const bool closes = p.beside && blockIdx.x == gridDim.x - 1 && g == (int)gridDim.y - 1 && sp == (int)gridDim.z - 1;
   PagedBlock blk;

@@ -240,12 +240,20 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     fence_mbar_init();
   }
   pdl_wait();
-  if (tid == 0) __threadfence();  // what the wait made visible, before the trigger below lets the rows kernel start
+  // The rows kernel may then start without a wait of its own.  What the wait made visible is published first,
+  // once: a fence in every CTA delays those that have no block (16 chunks beside 240 int8 rows: 195 -> 204 us).
+  if (blockIdx.x > 0) {
+    pdl_trigger();
+  } else if (tid == 0) {
+    fence_acq_rel_gpu();
+    pdl_trigger();
+  }
   // Blocks vary slowest: CTAs start in this order, and the longest blocks of all heads come first.
   const int g = blockIdx.x % p.kv.n_kv, bs = blockIdx.x / p.kv.n_kv, bx = bs / p.nsplit, sp = bs - bx * p.nsplit;
   // One warp searches: the code is cold, and all warps at it took longer than one and the exchange.
-  // Tensor memory after pdl_wait: the kernel before this one may need it to end.  And before
-  // pdl_trigger: a later kernel may take its own ahead of its wait for this one.
+  // Tensor memory after pdl_wait: the kernel before this one may need it to end.  (A later kernel cannot
+  // hold it, waiting for this one: the kernels that do need 15,000 registers or more, and beside a CTA of
+  // this one an SM has 6,400.)
   if (warp == 8) {
     PagedBlock found;
     if (!paged_block_search<PCH_R>(p, bx, lane, found)) found.nrows = 0;
@@ -261,7 +269,6 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  pdl_trigger();
   const PagedBlock blk = ctrl->block;
   if (blk.nrows == 0) return;
   const int nparts = paged_parts(p, blk.kend);
