@@ -1176,7 +1176,6 @@ struct PagedCut {
   int blocks, nsplit, span;
   size_t ml, o, found;  // offsets in the workspace
 };
-constexpr int PAGED_ROWS_MOST = 32;
 struct PagedPlan {
   PagedCut rows, chunk;
   int r, most, per;  // rows kernel: rows of a block (8 or 16), of its longest sequence, blocks of that
@@ -1223,14 +1222,15 @@ PagedPlan paged_plan(int B, int tokens, int max_q, int max_kv, int G, int n_kv, 
     at = c.found + (R == PCH_R && rows ? round_up(c.blocks * sizeof(PagedBlock), 16) : 0);
   };
   const long long rows = (long long)max_q * G;
-  const int most_rows = PAGED_ROWS_MOST;
-  const bool chunks = rows > most_rows;
+  const bool chunks = rows > PAGED_FINE;
   pl.r = (chunks ? G : rows) > 8 ? 16 : 8;
   pl.most = chunks ? pl.r : (int)std::max(1LL, rows);
   pl.per = (pl.most + pl.r - 1) / pl.r;
-  // Where most sequences may be as long as the longest, the chunk kernel takes the
-  // short ones along: a launch for none or few of them costs more than they do.
-  pl.small = chunks && (long long)tokens * 2 < (long long)B * max_q ? pl.r : 0;
+  // Sequences whose rows fit one block are the rows kernel's beside chunks, too, unless the bounds say that
+  // there is none: a launch for none costs 1.3 us.  (Rows behind the last sequence count as tokens: such a call
+  // may find its short sequences in the chunk kernel.)
+  const bool all_long = (long long)tokens > (long long)(B - 1) * max_q + pl.r / G;
+  pl.small = chunks && G <= pl.r && !all_long ? pl.r : 0;
   if (!chunks || pl.small) cut(pl.rows, (long long)B * pl.per, pl.r, 3, 128, 0, 200, 128, 32);
   if (chunks)
     cut(pl.chunk, ((long long)tokens * G + PCH_R - 1) / PCH_R + std::min((long long)B, (long long)tokens), PCH_R, 1,

@@ -8,8 +8,11 @@
 //
 // The G = n_heads / n_kv query heads of a KV head share its keys, so a block of
 // work is a run of packed rows of one (sequence, KV head): row r is token r / G,
-// head g G + r % G.  Sequences of up to 8 or 16 rows (decode, a few drafted tokens) go
-// to paged_rows_kernel here, longer ones to paged_chunk_kernel (paged_chunk.cuh).
+// head g G + r % G.  Calls whose sequences have up to 32 rows (decode, a few drafted
+// tokens) go to paged_rows_kernel here; in others the sequences of up to 8 rows (16 if
+// G > 8) do, and longer ones go to paged_chunk_kernel (paged_chunk.cuh).  Both hold the
+// weights of a sequence of up to 32 rows in 16 bits (bf16 caches), so its precision
+// does not depend on what it is batched with.
 #pragma once
 #include <climits>
 
@@ -18,6 +21,8 @@
 #include "paged_kv.cuh"
 
 namespace bitnet {
+
+constexpr int PAGED_FINE = 32;  // rows of the longest sequence whose weights are held in 16 bits
 
 // One block of rows: rows row0 .. row0 + nrows - 1 of sequence b.
 struct PagedBlock {
@@ -179,7 +184,7 @@ __device__ __forceinline__ int paged_parts(const PagedAttnParams& p, int kend) {
 }
 
 // ---------------------------------------------------------------------------
-// up to 8 or 16 rows: mma.sync
+// few rows: mma.sync
 // ---------------------------------------------------------------------------
 // A CTA of 4 warps takes up to 8 H rows of one (sequence, KV head) over one part of
 // the keys; warp w the tiles w, w + 4, ... of 16 keys (int8: 32).  K

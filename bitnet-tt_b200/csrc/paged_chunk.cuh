@@ -29,21 +29,31 @@
 //   warps 12-15 (int8)  write the raw tiles' codes to the slots as f16
 // The softmax's maximum is lazy: O and the sum are rescaled only when a row's
 // maximum grew by more than 2^8, so weights reach at most 2^8 and the pass over
-// O is rare (it waits for the products in flight).  P is rounded to bf16 (half a step: 2^-8 of a weight), the output's
-// own precision; sums and outputs are fp32.  The exponentials are what a tile
-// costs most: 16 a cycle and SM against 4096 products.  A quarter of them is
-// therefore computed on the multiply-add units (ex2_poly2).
+// O is rare (it waits for the products in flight); sums and outputs are fp32.  The
+// exponentials are what a tile costs most: 16 a cycle and SM against 4096 products.
+// A quarter of them is therefore computed on the multiply-add units (ex2_poly2).
+//
+// P of a sequence of more than 32 rows is one bf16 (half a step: 2^-8 of a weight), the
+// output's own precision, which doubles what rounding the output does to it: the two
+// 4096-token chunks come out within 2.2e-3 of the exact result (norms) in 570 us.  As a
+// pair hi + lo, 16 bits, they come within 1.65e-3, the output's rounding alone, in
+// 752 us, since the second product per step adds to the MMAs.  Sequences of up to 32 rows
+// (drafted tokens that stand beside chunks) get the pair and no polynomial: alone they
+// go to paged_rows_kernel, which works to the same precision.  2 chunks of 1024
+// beside 30 x 5 tokens over 4096 keys: 170 us with it, 159 without.
 //
 // int8: everything is f16.  The keys' codes are f16 values exactly, and their
 // scales multiply the scores in fp32, where an error would be raised to a power.
-// The values are code * scale, rounded to f16 (2^-11) at a power of two taken from
-// the largest scale of the part, which keeps rows down to 2^-21 of it at that
-// precision.  Q is scaled by a power of two per row (exact), P has f16's 11 bits.
+// The values are code * scale, the scale and the product rounded to f16 (2^-11 each) at
+// a power of two taken from the largest scale of the part, which keeps rows down to
+// 2^-21 of it at that precision, and smaller ones to 2^-32 of 127 times it.  Q is scaled by a power of two per row (exact), P has f16's 11 bits.
 // Codes come out of their words as (0, 2) and (1, 3) pairs, so every four dims of
 // the slots stand in the order 0, 2, 1, 3: Q is laid out the same way, and the
 // output is put back when it is stored.
 #pragma once
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "paged_attention.cuh"
 
@@ -274,6 +284,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
   const int nparts = paged_parts(p, blk.kend);
   if (sp >= nparts) return;
   const int k0 = sp * p.span, k1 = min(blk.kend, k0 + p.span);
+  const bool fine = !I8 && blk.row0 == 0 && blk.nrows <= PAGED_FINE;  // the whole sequence: weights as hi + lo
   // 64-key steps of the two row tiles (the second sees at least the first's keys)
   const int end0 = min(k1, max(0, blk.past + (blk.row0 + min(blk.nrows, 128) - 1) / p.G + 1));
   const int n0 = max(0, (end0 - k0 + PCH_STEP - 1) / PCH_STEP);
@@ -425,11 +436,15 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         }
         tc_commit(&ctrl->s_full[t][h]);
       };
-      auto pv = [&](int slot, int h, bool first) {
+      auto pv = [&](int slot, int h, bool first, auto fine_tag) {
         const uint64_t b = dv + slot * (S::TILE >> 4) + h * (PCH_STEP * 128 >> 4);
         const uint32_t a = tbase + t * 128 + h * 64, d = tbase + 256 + t * D;
 #pragma unroll
         for (int k = 0; k < PCH_STEP / 16; ++k) mma_f16_ts(d, a + k * 8, b + k * (16 * 128 >> 4), idesc_o, k > 0 || !first);
+        if constexpr (decltype(fine_tag)::value) {
+#pragma unroll
+          for (int k = 0; k < PCH_STEP / 16; ++k) mma_f16_ts(d, a + 32 + k * 8, b + k * (16 * 128 >> 4), idesc_o, 1);
+        }
         tc_commit(&ctrl->o_done[t][h]);
       };
       auto arrived = [&](uint64_t* bar, uint32_t parity, int site) {
@@ -446,6 +461,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         tc_commit(&ctrl->empty[0]);
       }
       __syncwarp();
+      auto steps = [&](auto fine_tag) {
       for (int i = 0; ok && i < nstep; ++i) {
         const int j = i >> 1, h = i & 1;
         const int vs = (2 * j + 1) % S::NSLOT, ks = (2 * j + 2) % S::NSLOT;  // slots of V, and of the next K
@@ -455,13 +471,17 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         }
         if (ok && i < nt) ok = arrived(&ctrl->p_ready[t][h], j & 1, 365);
         if (ok && elect_one()) {
-          if (i < nt) pv(vs, h, i == 0);
+          if (i < nt) pv(vs, h, i == 0, fine_tag);
           if (i + 2 < nt) qk(ks, h);
           if (h == 1 || i + 1 == nstep) tc_commit(&ctrl->empty[vs]);
           if (i + 2 < nstep && (h == 1 || i + 3 == nstep)) tc_commit(&ctrl->empty[ks]);
         }
         __syncwarp();
       }
+      };
+      // two copies of the loop, as of the softmax's: a choice inside it costs the common one 16%
+      if (fine) steps(std::true_type{});
+      else steps(std::false_type{});
       if (!ok) {  // let the MMAs in flight end before tensor memory is freed
         if (elect_one()) tc_commit(&ctrl->drain[t]);
         __syncwarp();
@@ -606,6 +626,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     float m = -INFINITY;
     uint64_t l2[2] = {0, 0};
     bool ok = true;
+    auto steps = [&](auto fine_tag) {
+    constexpr bool FINE = decltype(fine_tag)::value;
     for (int i = 0; i < nt; ++i) {
       const int j = i >> 1, h = i & 1;
       ok = wait(&ctrl->s_full[t][h], j & 1, 371);
@@ -671,12 +693,12 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
         const uint64_t ref2 = f2_splat(m == -INFINITY ? 0.f : S::LIFT - m);
 #pragma unroll
         for (int c = 0; c < PCH_STEP; c += 32) {
-          uint32_t pw[16];
+          uint32_t pw[16], pl[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const uint64_t z = f2_fma(f2_make(s[c + 2 * e], s[c + 2 * e + 1]), scale2, ref2);
             float x, y;
-            if (e % 4 == 3) {
+            if (e % 4 == 3 && !FINE) {
               ex2_poly2(z, x, y);
             } else {
               uint32_t a, b;
@@ -684,9 +706,11 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
               x = ex2(__uint_as_float(a)), y = ex2(__uint_as_float(b));
             }
             l2[e & 1] = f2_add(l2[e & 1], f2_make(__float_as_uint(x), __float_as_uint(y)));
-            pw[e] = I8 ? f16x2_of(x, y) : bf2_of(x, y);
+            if (FINE) split_bf2(x, y, pw[e], pl[e]);
+            else pw[e] = I8 ? f16x2_of(x, y) : bf2_of(x, y);
           }
           tmem_st16(ts + c / 2, pw);
+          if (FINE) tmem_st16(ts + 32 + c / 2, pl);
         }
         tmem_wait_st();
       }
@@ -694,6 +718,9 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctrl->p_ready[t][h]);
     }
+    };
+    if (fine) steps(std::true_type{});
+    else steps(std::false_type{});
     if (ok && nt > 0) ok = __all_sync(0xffffffffu, wait(&ctrl->o_done[t][(nt - 1) & 1], ((nt - 1) >> 1) & 1, 372));
     if (ok && warp_live) {
       tc_fence_after();

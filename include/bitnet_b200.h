@@ -347,7 +347,15 @@ int bitnet_paged_read(const bitnet_paged_kv_t* kv, const int32_t* block_table, i
  * both 16-byte aligned.  n_heads / n_kv_heads is at most 64; scale is positive.  max_seqlen and max_kv_len bound the new
  * tokens and the keys of every sequence; they size the grid and the split of long
  * contexts, so tight bounds keep both small.  Cache rows below kv_lens[b] have to
- * be finite; whatever stands behind them does not matter.  workspace:
+ * be finite; whatever stands behind them does not matter.
+ *   Precision: scores, maxima, sums and outputs are fp32, rounded once to out.
+ * Softmax weights: bf16 caches 16 bits for a sequence of up to 32 rows (new tokens
+ * x n_heads / n_kv_heads), whatever it is batched with, bf16 for a longer one; int8
+ * caches f16, and where longer sequences are in the call the values are rounded to
+ * f16 as well, at a power of two of the largest value scale of the sequence (of the
+ * part that is worked on at once): two half steps, each 2^-11 of the value or
+ * 2^-32 of 127 times that scale, whichever is more.
+ *   workspace:
  * bitnet_paged_attention_workspace_bytes (0: may be NULL), 16-byte aligned,
  * contents irrelevant before and after; calls that may overlap need their own. */
 size_t bitnet_paged_attention_workspace_bytes(int B, int total_tokens, int max_seqlen, int max_kv_len, int n_heads,
