@@ -112,25 +112,28 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
 }
 // 2^y for two values without the exponential unit: n = round(y) by adding 1.5 * 2^23,
 // 2^(y - n) by a cubic (fitted for the least largest relative error on [-1/2, 1/2]:
-// 7.5e-5, an eighth of a bf16's half step), and n added to the exponent.  y is held at
-// -126 and above, where the result is as good as 0.
+// 7.5e-5, a fiftieth of a bf16's half step, a sixth of an f16's), times 2^n by its bits.
+// y is held at -127 and above, where 2^n is 0: so is the weight of a hidden key, and a
+// NaN stays one.  (n added to the cubic's exponent is an operation less a pair, but leaves
+// a hidden key 2^-126, which a large value can raise to anything, and makes a NaN 3e38.)
 __device__ __forceinline__ void ex2_poly2(uint64_t y, float& a, float& b) {
   uint32_t lo, hi;
   f2_split(y, lo, hi);
   float x0, x1;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(__uint_as_float(lo)), "f"(-126.f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(__uint_as_float(hi)), "f"(-126.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(__uint_as_float(lo)), "f"(-127.f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(__uint_as_float(hi)), "f"(-127.f));
   y = f2_make(__float_as_uint(x0), __float_as_uint(x1));
   const uint64_t t = f2_add(y, f2_splat(12582912.f));
   const uint64_t f = f2_fma(f2_add(t, f2_splat(-12582912.f)), f2_splat(-1.f), y);
   uint64_t p = f2_fma(f2_splat(0.05517166852951050f), f, f2_splat(0.2426111251115799f));
   p = f2_fma(p, f, f2_splat(0.6932609677314758f));
   p = f2_fma(p, f, f2_splat(0.9999280571937561f));
-  uint32_t p0, p1, t0, t1;
-  f2_split(p, p0, p1);
+  uint32_t t0, t1;
   f2_split(t, t0, t1);
-  a = __uint_as_float(p0 + (t0 << 23));
-  b = __uint_as_float(p1 + (t1 << 23));
+  uint32_t w0, w1;
+  f2_split(f2_mul(p, f2_make((t0 << 23) + 0x3f800000u, (t1 << 23) + 0x3f800000u)), w0, w1);
+  a = __uint_as_float(w0);
+  b = __uint_as_float(w1);
 }
 __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
   uint32_t d;

@@ -1,0 +1,48 @@
+"""Paged attention on values at the ends of their types: what a token does not see
+does not reach it, and what it sees does."""
+
+import pytest
+import torch
+from test_paged_gpu import BF16, I8, _cache, _cu, _ok, _pages, _rows64
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend(cuda, c, table, qs, kv, q):
+    out = c.attend(q.to(cuda), _cu(qs).to(cuda), torch.tensor(kv, dtype=torch.int32, device=cuda), table.to(cuda),
+                   max(qs), max(kv))
+    torch.cuda.synchronize()
+    _ok()
+    return out.double().cpu()
+
+
+@pytest.mark.parametrize("qs,kv", [([3], [40]), ([120], [130]), ([600], [700]), ([200, 1], [3000, 9])])
+def test_hidden_values_weigh_nothing_however_large(cuda, qs, kv):
+    """The last new token's value is near bf16's largest: the tokens before it are those of any other value, bit
+    for bit."""
+    hq, hk, d, page = 4, 1, 128, 16
+    table, n = _pages(kv, page, 3)
+    c = _cache(cuda, n, page, hk, d, BF16, 3)
+    q = torch.randn((sum(qs), hq * d), generator=torch.Generator().manual_seed(2)).to(BF16)
+    want = _attend(cuda, c, table, qs, kv, q)
+    at = kv[0] - 1
+    c.value_pages[int(table[0, at // page]), :, at % page] = 3e38
+    got = _attend(cuda, c, table, qs, kv, q)
+    assert torch.equal(got[:qs[0] - 1], want[:qs[0] - 1]) and torch.equal(got[qs[0]:], want[qs[0]:])
+    assert not torch.equal(got[qs[0] - 1], want[qs[0] - 1])
+
+
+@pytest.mark.parametrize("qs,kv", [([3], [40]), ([120], [130]), ([100], [3000])])
+def test_a_key_scale_of_nan_reaches_all_that_see_it_and_no_other(cuda, qs, kv):
+    """What append leaves of a key with an infinity in an int8 cache, at every place of a step."""
+    hq, hk, d, page = 4, 1, 64, 16
+    table, n = _pages(kv, page, 3)
+    q = torch.randn((sum(qs), hq * d), generator=torch.Generator().manual_seed(2)).to(BF16)
+    plain = _attend(cuda, _cache(cuda, n, page, hk, d, I8, 3), table, qs, kv, q)
+    past = kv[0] - qs[0]
+    for at in (past, *(past + 1 + i for i in range(0, min(9, qs[0] - 1)))):
+        c = _cache(cuda, n, page, hk, d, I8, 3)
+        c.key_scale[int(table[0, at // page]), :, at % page] = float("nan")
+        got = _attend(cuda, c, table, qs, kv, q)
+        assert bool(got[at - past:].isnan().all())
+        assert torch.equal(got[:at - past], plain[:at - past])
