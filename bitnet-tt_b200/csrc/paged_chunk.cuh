@@ -731,7 +731,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       f2_split(l2[0], a, b);
       f2_split(l2[1], c2, d2);
       const float l = (__uint_as_float(a) + __uint_as_float(b)) + (__uint_as_float(c2) + __uint_as_float(d2));
-      const float inv = m == -INFINITY ? 0.f : 1.f / l;
+      const bool sees = lim > 0;  // else zeros; by the mask, not by m, which is -infinity over NaN scores too
+      const float inv = sees ? 1.f / l : 0.f;
       const size_t pr = (((size_t)sp * p.blocks + bx) * p.kv.n_kv + g) * PCH_R + r;
       if (live && nparts > 1) p.part_ml[pr] = make_float2(m - S::LIFT, l);
       if (I8 && nt > 0) wait(&ctrl->v_full, 0, 377);  // complete: the values were converted after it
@@ -770,8 +771,8 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              w[k] = m == -INFINITY ? 0u
-                                    : bf2_of(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
+              w[k] = !sees ? 0u
+                           : bf2_of(__uint_as_float(o[e + 2 * k]) * inv, __uint_as_float(o[e + 2 * k + 1]) * inv);
             *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }

@@ -46,3 +46,22 @@ def test_a_key_scale_of_nan_reaches_all_that_see_it_and_no_other(cuda, qs, kv):
         got = _attend(cuda, c, table, qs, kv, q)
         assert bool(got[at - past:].isnan().all())
         assert torch.equal(got[:at - past], plain[:at - past])
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("qs,kv", [([1], [40]), ([1], [5000]), ([6], [40]), ([120], [130]), ([60], [3000]), ([20, 1], [16, 3])])
+def test_a_query_of_nan_gives_nan_and_one_without_keys_zeros(cuda, qs, kv, dtype):
+    hq, hk, d, page = 4, 1, 128, 16
+    table, n = _pages(kv, page, 3)
+    c = _cache(cuda, n, page, hk, d, dtype, 3)
+    q = torch.randn((sum(qs), hq * d), generator=torch.Generator().manual_seed(2)).to(BF16)
+    want = _attend(cuda, c, table, qs, kv, q).view(-1, hq, d)
+    blind = max(0, qs[0] - kv[0])  # tokens before the first key
+    assert bool((want[:blind] == 0).all()) and bool((want[blind:qs[0]] != 0).any())
+    for tok in sorted({0, blind, qs[0] - 1}):
+        bad = q.clone()
+        bad[tok, d + 5] = float("nan")  # head 1
+        got = _attend(cuda, c, table, qs, kv, bad).view(-1, hq, d)
+        assert bool((got[tok, 1] == 0).all() if tok < blind else got[tok, 1].isnan().all())
+        got[tok, 1] = want[tok, 1]
+        assert torch.equal(got, want)
