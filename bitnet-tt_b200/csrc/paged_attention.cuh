@@ -104,6 +104,7 @@ __device__ __forceinline__ bool paged_block_ranked(const PagedAttnParams& p, int
       const int n = min(max(len[c], 0), p.max_q);
       past[c] = min(kv[c], p.max_kv) - n;
       rows[c] = n * p.G > p.small ? n * p.G : 0;
+      if (len[c] < 0) rows[c] = 1, past[c] = -1;  // a block that reports it, behind all others
       nb += (rows[c] + R - 1) / R;
     }
   }
@@ -160,8 +161,8 @@ __device__ __forceinline__ bool paged_block_search(const PagedAttnParams& p, int
   bx = p.blocks - 1 - bx;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int i = b0 + lane;
-    const int rows = (i < p.B ? min(max(p.cu[i + 1] - p.cu[i], 0), p.max_q) : 0) * p.G;
-    const int nb = rows > p.small ? (rows + R - 1) / R : 0;
+    const int len = i < p.B ? p.cu[i + 1] - p.cu[i] : 0, rows = min(max(len, 0), p.max_q) * p.G;
+    const int nb = len < 0 ? 1 : rows > p.small ? (rows + R - 1) / R : 0;
     int sum = nb;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {

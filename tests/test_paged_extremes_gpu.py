@@ -65,3 +65,23 @@ def test_a_query_of_nan_gives_nan_and_one_without_keys_zeros(cuda, qs, kv, dtype
         assert bool((got[tok, 1] == 0).all() if tok < blind else got[tok, 1].isnan().all())
         got[tok, 1] = want[tok, 1]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("heads", [(4, 2), (64, 1)])
+@pytest.mark.parametrize("b", [2, 40, 200])
+def test_a_negative_length_is_reported_where_all_sequences_are_long(cuda, b, heads, dtype):
+    """Offsets that go back, with bounds that leave no short sequence: the chunk kernel's alone to find."""
+    from bitnet_tt import _lib
+
+    hq, hk = heads
+    c = _cache(cuda, b, 64, hk, 64, dtype, 1)
+    table = torch.arange(b, dtype=torch.int32, device=cuda).view(b, 1)
+    lens = torch.full((b,), 40, dtype=torch.int32, device=cuda)
+    q = torch.zeros((40 * b, hq * 64), dtype=BF16, device=cuda)
+    cu = [40 * i for i in range(b)] + [40 * (b - 1) - 20]
+    for max_kv in (40, 0):
+        c.attend(q, torch.tensor(cu, dtype=torch.int32, device=cuda), lens if max_kv else lens * 0, table, 40, max_kv)
+        torch.cuda.synchronize()
+        assert _lib.last_device_status() == (-1, 350)
+        _ok()
