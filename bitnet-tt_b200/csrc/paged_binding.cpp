@@ -16,6 +16,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <climits>
 
@@ -236,18 +237,13 @@ PyObject* py_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void *k = nullptr, *v = nullptr;
     bool bad = false;
     const int64_t shape[3] = {rows, c->kv.n_kv_heads, c->kv.head_dim};
-    PyObject* ko = out_arg(a[5], shape, dev, &k, &bad);
+    const THPObjectPtr ko(out_arg(a[5], shape, dev, &k, &bad));  // let go where the next allocation throws
     if (bad) Py_RETURN_NONE;
     if (!ko) return nullptr;
-    PyObject* vo = out_arg(a[6], shape, dev, &v, &bad);
-    if (!vo) {
-      Py_DECREF(ko);
-      if (bad) Py_RETURN_NONE;
-      return nullptr;
-    }
-    PyObject* pair = PyTuple_Pack(2, ko, vo);
-    Py_DECREF(ko);
-    Py_DECREF(vo);
+    const THPObjectPtr vo(out_arg(a[6], shape, dev, &v, &bad));
+    if (bad) Py_RETURN_NONE;
+    if (!vo) return nullptr;
+    PyObject* pair = PyTuple_Pack(2, ko.get(), vo.get());
     if (!pair) return nullptr;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
     return launched(pair, [&] {
