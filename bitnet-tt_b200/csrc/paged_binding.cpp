@@ -61,10 +61,12 @@ const at::Tensor* rows_arg(PyObject* o, int device) {
   if (!THPVariable_Check(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   return on(t, at::kBFloat16, device) && t.dim() == 2 && t.stride(1) == 1 && t.size(0) <= INT_MAX &&
-                 t.stride(0) <= INT_MAX
+                 (t.size(0) <= 1 || t.stride(0) <= INT_MAX)
              ? &t
              : nullptr;
 }
+// The stride of rows: of one row or none it may be anything.  (heads_of() has bounded the features.)
+int ld_of(const at::Tensor& t) { return (int)(t.size(0) <= 1 ? t.size(1) : t.stride(0)); }
 // Lets other Python threads run while this one allocates or launches: either may wait for the GPU,
 // and what the GPU waits for may be a callback in Python.
 struct Unlocked {
@@ -162,7 +164,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
     return launched(out, [&] {
       return bitnet_paged_append(&c->kv, t.data, t.b, t.pages, cu->const_data_ptr<int32_t>(),
-                                 lens->const_data_ptr<int32_t>(), qkv->data_ptr(), (int)qkv->stride(0),
+                                 lens->const_data_ptr<int32_t>(), qkv->data_ptr(), ld_of(*qkv),
                                  (int)qkv->size(0), heads, cos.data_ptr(), sin.data_ptr(), (int)cos.size(0),
                                  2 * (int)cos.size(1), tab == at::kFloat, inter, step, q, stream);
     });
@@ -212,7 +214,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
     return launched(out, [&] {
       return bitnet_paged_attention(&c->kv, t.data, t.b, t.pages, cu->const_data_ptr<int32_t>(),
-                                    lens->const_data_ptr<int32_t>(), q->data_ptr(), (int)q->stride(0), tokens,
+                                    lens->const_data_ptr<int32_t>(), q->data_ptr(), ld_of(*q), tokens,
                                     (int)max_q, (int)max_kv, heads, (float)scale, ws, bytes, o, stream);
     });
   });
