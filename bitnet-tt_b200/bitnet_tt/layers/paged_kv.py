@@ -93,7 +93,7 @@ class PagedKVCache:
                       and s.device == k.device, "int8 pages need contiguous fp32 scales [pages, heads, page_size]")
         else:
             _want(ks is None and vs is None, "bfloat16 pages have no scales")
-        self.key_pages, self.value_pages, self.key_scale, self.value_scale = k, v, ks, vs
+        self._pools = (k, v, ks, vs)
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         self.device = k.device
         self._index = k.get_device()
@@ -104,9 +104,26 @@ class PagedKVCache:
             *(_lib.ptr(t) or 0 for t in (k, v, ks, vs)), self.num_pages, self.page_size, self.num_kv_heads, self.head_dim,
             _lib.KV_INT8 if k.dtype == torch.int8 else _lib.KV_BF16, self._index)
 
+    # The handle holds the pools' addresses: their contents may be written, the tensors not replaced.
+    @property
+    def key_pages(self) -> torch.Tensor:
+        return self._pools[0]
+
+    @property
+    def value_pages(self) -> torch.Tensor:
+        return self._pools[1]
+
+    @property
+    def key_scale(self) -> torch.Tensor | None:
+        return self._pools[2]
+
+    @property
+    def value_scale(self) -> torch.Tensor | None:
+        return self._pools[3]
+
     def nbytes(self) -> int:
-        ts = [t for t in (self.key_pages, self.value_pages, self.key_scale, self.value_scale) if t is not None]
-        return sum(t.numel() * t.element_size() for t in ts)
+        """Bytes of the pools, scales included."""
+        return sum(t.numel() * t.element_size() for t in self._pools if t is not None)
 
     # ---- what is wrong with a call's arguments -------------------------------
     # The module tests all of them at once; these run when it says that something is

@@ -1,0 +1,37 @@
+"""What a PagedKVCache and its module hold on the host."""
+
+import pytest
+import torch
+
+
+def _pool(dtype=torch.bfloat16):
+    return torch.zeros((8, 2, 16, 64), dtype=dtype)
+
+
+@pytest.fixture
+def host(monkeypatch):
+    from bitnet_tt import _lib
+
+    monkeypatch.setattr(_lib, "ptr", lambda t: None if t is None else t.data_ptr())
+
+
+def test_pools_cannot_be_replaced_under_the_handle(host):
+    """The handle keeps addresses: another tensor in an attribute would leave them on freed memory."""
+    from bitnet_tt.layers import PagedKVCache
+
+    k, v, s = _pool(torch.int8), _pool(torch.int8), torch.zeros((8, 2, 16))
+    c = PagedKVCache.from_tensors(k, v, s, s.clone())
+    assert c.key_pages is k and c.value_pages is v and c.key_scale is s
+    for name in ("key_pages", "value_pages", "key_scale", "value_scale"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, torch.ones(4))
+    assert c.key_pages is k and c.key_scale is s
+
+
+def test_nbytes_counts_pools_and_scales(host):
+    from bitnet_tt.layers import PagedKVCache
+
+    n = 8 * 2 * 16
+    assert PagedKVCache.from_tensors(_pool(), _pool()).nbytes() == 2 * n * 64 * 2
+    s = torch.zeros((8, 2, 16))
+    assert PagedKVCache.from_tensors(_pool(torch.int8), _pool(torch.int8), s, s.clone()).nbytes() == 2 * n * (64 + 4)
