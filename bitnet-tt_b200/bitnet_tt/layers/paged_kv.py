@@ -208,6 +208,8 @@ class PagedKVCache:
                             num_heads: int) -> torch.Tensor | None:
         """Workspace of attend() for these bounds (None when it needs none).  Calls
         that may overlap need one each."""
+        _want(all(0 <= x <= _INT_MAX for x in (batch, total_tokens, max_seqlen, max_kv_len, num_heads)),
+              "the workspace's bounds are out of range")
         with torch.cuda.device(self._index):
             n = _lib.paged_attention_workspace_bytes(batch, total_tokens, max_seqlen, max_kv_len, num_heads,
                                                      self.num_kv_heads, self.head_dim)

@@ -43,3 +43,34 @@ def test_one_row_may_have_any_stride(cuda, stride):
     none = c.attend(want[:0].as_strided((0, 4 * 64), (stride, 1)), _cu([0]).to(cuda), lens, table, 1, 20)
     assert none.shape == (0, 4 * 64)
     _ok()
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("qs,kv", [([1], [5000]), ([2, 3], [3000, 40]), ([64, 1, 1], [3000, 2000, 5])])
+def test_a_workspace_of_ones_own(cuda, qs, kv, dtype):
+    """attention_workspace() sizes it, whatever it holds before; captured calls that share one in a row replay right."""
+    table, n = _pages(kv, 64)
+    c = _cache(cuda, n, 64, 2, 128, dtype, 3)
+    cu, lens, table = _cu(qs).to(cuda), torch.tensor(kv, dtype=torch.int32, device=cuda), table.to(cuda)
+    q = torch.randn((sum(qs), 8 * 128), generator=torch.Generator().manual_seed(1)).to(BF16).to(cuda)
+    want = c.attend(q, cu, lens, table, max(qs), max(kv))
+    ws = c.attention_workspace(len(qs), sum(qs), max(qs), max(kv), 8)
+    assert ws is not None
+    ws.fill_(255)
+    assert torch.equal(c.attend(q, cu, lens, table, max(qs), max(kv), workspace=ws), want)
+    with pytest.raises(RuntimeError, match="invalid argument"):
+        c.attend(q, cu, lens, table, max(qs), max(kv), workspace=ws[:-1])
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    graphs = []
+    for o in outs:
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            c.attend(q, cu, lens, table, max(qs), max(kv), out=o, workspace=ws)
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    _ok()

@@ -35,3 +35,16 @@ def test_nbytes_counts_pools_and_scales(host):
     assert PagedKVCache.from_tensors(_pool(), _pool()).nbytes() == 2 * n * 64 * 2
     s = torch.zeros((8, 2, 16))
     assert PagedKVCache.from_tensors(_pool(torch.int8), _pool(torch.int8), s, s.clone()).nbytes() == 2 * n * (64 + 4)
+
+
+def test_workspace_bounds_beyond_32_bits_are_refused(host):
+    """As attend() refuses them; cut to 32 bits they would size another call's workspace."""
+    from bitnet_tt.layers import PagedKVCache
+
+    c = PagedKVCache.from_tensors(_pool(), _pool())
+    good = dict(batch=1, total_tokens=1, max_seqlen=1, max_kv_len=40, num_heads=4)
+    assert c.attention_workspace(**good) is None
+    for name in good:
+        for bad in ((1 << 32) + good[name], 1 << 31, -1):
+            with pytest.raises(ValueError):
+                c.attention_workspace(**(good | {name: bad}))
