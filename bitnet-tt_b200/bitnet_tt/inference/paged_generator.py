@@ -4,7 +4,9 @@ Where Batch32Generator decodes a fixed batch in lock-step over contiguous caches
 a PagedGenerator keeps a pool of pages per layer.  A sequence is added with any
 prompt, may be extended later (a chat turn), and is released when done; every
 step() runs one forward pass over whatever is pending: one token of each decoding
-sequence, and chunks of the prompts that are still being read.
+sequence, and chunks of the prompts that are still being read.  Prompts take pages
+in the order they were added, and only what decoding sequences and the prompts
+before them leave, so that one that has been begun can be read to its end.
 """
 
 from __future__ import annotations
@@ -25,6 +27,7 @@ class _Sequence:
     length: int = 0                                   # tokens in the cache
     pending: list[int] = field(default_factory=list)  # tokens still to be read
     generated: list[int] = field(default_factory=list)
+    limit: int | None = None                          # the length it will end at, if that is known
 
 
 class PagedGenerator:
@@ -79,29 +82,62 @@ class PagedGenerator:
         """Ends a sequence and gives its pages back."""
         self.free_pages += self.sequences.pop(seq).pages
 
-    def _plan(self) -> list[tuple[int, int]]:
+    def _more_pages(self, s: _Sequence, length: int) -> int:
+        """Pages that it needs beyond its own to hold `length` tokens."""
+        return max(0, -(-length // self.page_size) - len(s.pages))
+
+    def _plan(self, only: set[int] | None) -> list[tuple[int, int]]:
         """(sequence, tokens of it) of the next step, within chunk_tokens and the free pages."""
-        ready = [(i, s) for i, s in self.sequences.items() if s.pending]
+        ready = [(i, s) for i, s in self.sequences.items() if s.pending and (only is None or i in only)]
         ready.sort(key=lambda x: len(x[1].pending) > 1)  # single tokens first, else in order
-        room, pages, plan = self.chunk_tokens, len(self.free_pages), []
+        room, pages, plan, late = self.chunk_tokens, len(self.free_pages), [], []
+
+        def take(i: int, s: _Sequence, pages: int) -> int:
+            """Plans what fits; the pages that it costs."""
+            nonlocal room
+            n = min(len(s.pending), room, len(s.pages) * self.page_size - s.length + pages * self.page_size,
+                    self.max_seq_len - s.length)
+            if n <= 0:
+                return 0
+            room -= n
+            plan.append((i, n))
+            return self._more_pages(s, s.length + n)
+
+        # What the decoding sequences need next: all of it where their end is known, else a page each.
+        kept = 0
         for i, s in ready:
-            n = min(len(s.pending), room)
-            have = len(s.pages) * self.page_size - s.length
-            n = min(n, have + pages * self.page_size, self.max_seq_len - s.length)
-            if n > 0:
-                pages -= max(0, -(-(n - have) // self.page_size))
-                room -= n
-                plan.append((i, n))
+            if len(s.pending) == 1:
+                used = take(i, s, pages)
+                pages -= used
+                more = self._more_pages(s, s.limit if s.limit is not None else self.max_seq_len) - used
+                kept += max(0, more) if s.limit is not None else min(1, max(0, more))
+        for i, s in ready:
+            if len(s.pending) == 1:
+                continue
+            end = max(s.length + len(s.pending), s.limit or 0)
+            rest = self._more_pages(s, min(end, self.max_seq_len))
+            if rest > pages - kept:
+                late.append((i, s))  # it cannot be read to its end: not while anything else goes on
+                continue
+            take(i, s, pages)
+            pages -= rest  # whatever is not taken now is kept for it
+        if not plan:
+            for i, s in late:
+                pages -= take(i, s, pages)
         return plan
 
     # ---- steps -----------------------------------------------------------------
     def step(self, keep_logits: bool = False) -> dict[int, int]:
         """One forward pass over pending tokens.  Returns the next token of every
         sequence whose pending tokens are all read; it becomes that sequence's next
-        pending token."""
-        plan = self._plan()
+        pending token.  RuntimeError when nothing that is pending fits the free pages
+        (release a sequence, then go on)."""
+        return self._step(None, keep_logits)
+
+    def _step(self, only: set[int] | None, keep_logits: bool = False) -> dict[int, int]:
+        plan = self._plan(only)
         if not plan:
-            if any(s.pending for s in self.sequences.values()):
+            if any(s.pending for i, s in self.sequences.items() if only is None or i in only):
                 raise RuntimeError("no pages or positions left for the pending tokens")
             return {}
         ids, pages, lens = [], [], []
@@ -129,22 +165,38 @@ class PagedGenerator:
         return out
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 128) -> list[list[int]]:
-        """Greedy continuation of prompts of any lengths: max_new_tokens tokens each."""
+        """Greedy continuation of prompts of any lengths: max_new_tokens tokens each.
+        Prompts start as the pages for all of their tokens are there, in order; a
+        batch may be larger than the pool.  Other sequences stay as they are."""
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
-        if any(len(np.asarray(p).reshape(-1)) + max_new_tokens - 1 > self.max_seq_len for p in prompts):
+        todo = [self._tokens(p) for p in prompts]
+        lengths = [len(p) + max_new_tokens - 1 for p in todo]
+        if any(n > self.max_seq_len for n in lengths):
             raise ValueError("prompt + max_new_tokens exceeds max_seq_len")
-        todo = [self.add(p) for p in prompts]
-        out: dict[int, list[int]] = {}
+        need = [-(-n // self.page_size) for n in lengths]
+        room = len(self.free_pages)  # nothing but what this call starts takes any until it ends
+        if any(n > room for n in need):
+            raise ValueError(f"prompt + max_new_tokens needs more than the {room} free pages")
+        out: list[list[int]] = [[] for _ in todo]
+        active: dict[int, int] = {}  # sequence -> prompt
+        at = 0
         try:
-            while len(out) < len(todo):
-                self.step()
-                for i in todo:
-                    if i in self.sequences and len(self.sequences[i].generated) >= max_new_tokens:
-                        out[i] = self.sequences[i].generated[:max_new_tokens]
-                        self.release(i)
+            while at < len(todo) or active:
+                while at < len(todo) and need[at] <= room:
+                    seq = self.add(todo[at])
+                    self.sequences[seq].limit = lengths[at]
+                    active[seq] = at
+                    room -= need[at]
+                    at += 1
+                self._step(set(active))
+                for seq in list(active):
+                    if len(self.sequences[seq].generated) >= max_new_tokens:
+                        i = active.pop(seq)
+                        out[i] = self.sequences[seq].generated[:max_new_tokens]
+                        room += need[i]
+                        self.release(seq)
         finally:
-            for i in todo:
-                if i in self.sequences:
-                    self.release(i)
-        return [out[i] for i in todo]
+            for seq in active:
+                self.release(seq)
+        return out
