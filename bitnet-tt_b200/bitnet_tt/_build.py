@@ -56,11 +56,15 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     (found beside it at run time) into bitnet_tt/_paged.so; return its path."""
     header = os.path.join(os.path.dirname(ROOT), "include", "bitnet_b200.h")
     deps = [p for p in (EXT_SOURCE, header) if os.path.exists(p)]
-    if not force and os.path.exists(EXT_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(EXT_PATH) for d in deps):
-        return EXT_PATH
     import torch
     from torch.utils import cpp_extension
 
+    # torch's headers are not among the sources whose times count: another torch means another build
+    stamp = EXT_PATH + ".stamp"
+    made_for = f"torch {torch.__version__}, python {sysconfig.get_python_version()}\n"
+    if not force and os.path.exists(EXT_PATH) and all(os.path.getmtime(d) <= os.path.getmtime(EXT_PATH) for d in deps):
+        if os.path.exists(stamp) and open(stamp).read() == made_for:
+            return EXT_PATH
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     inc = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
@@ -75,6 +79,8 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
     os.replace(tmp, EXT_PATH)
+    with open(stamp, "w") as f:
+        f.write(made_for)
     return EXT_PATH
 
 

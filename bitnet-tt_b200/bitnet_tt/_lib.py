@@ -548,6 +548,9 @@ def paged_module():
         spec = importlib.util.spec_from_file_location("bitnet_tt._paged", p)
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
+        made_for = getattr(mod, "torch_version", "of an earlier build")
+        if made_for != torch.__version__.split("+")[0]:
+            raise RuntimeError(f"{p} was built for torch {made_for}, this is {torch.__version__}: build it again")
         _paged = mod
     return _paged
 

@@ -17,6 +17,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
+#include <torch/version.h>
 
 #include <climits>
 
@@ -265,4 +266,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged", nullptr, -1, methods, nul
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__paged(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) Py_CLEAR(m);
+  return m;
+}

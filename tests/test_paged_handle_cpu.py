@@ -48,3 +48,42 @@ def test_workspace_bounds_beyond_32_bits_are_refused(host):
         for bad in ((1 << 32) + good[name], 1 << 31, -1):
             with pytest.raises(ValueError):
                 c.attention_workspace(**(good | {name: bad}))
+
+
+def test_the_module_is_rebuilt_for_another_torch(monkeypatch, tmp_path):
+    import os
+    import subprocess
+
+    from bitnet_tt import _build
+
+    ext = tmp_path / "_paged.so"
+    monkeypatch.setattr(_build, "EXT_PATH", str(ext))
+    built = []
+
+    def compiler(cmd, **kw):
+        built.append(cmd)
+        with open(cmd[cmd.index("-o") + 1], "w") as f:
+            f.write("module")
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(_build.subprocess, "run", compiler)
+    for _ in range(2):
+        assert _build.build_binding() == str(ext)
+    assert len(built) == 1
+    monkeypatch.setattr(torch, "__version__", "2.99.0")
+    for _ in range(2):
+        _build.build_binding()
+    assert len(built) == 2
+    os.utime(ext, (1, 1))  # older than its sources
+    _build.build_binding()
+    assert len(built) == 3
+
+
+def test_a_module_of_another_torch_is_refused(monkeypatch):
+    from bitnet_tt import _lib
+
+    assert _lib.paged_module().torch_version == torch.__version__.split("+")[0]
+    monkeypatch.setattr(_lib, "_paged", None)
+    monkeypatch.setattr(torch, "__version__", "2.99.0")
+    with pytest.raises(RuntimeError, match="2.99.0"):
+        _lib.paged_module()
