@@ -27,14 +27,3 @@ def half_split_tables(head_dim: int, max_len: int, theta: float) -> tuple[torch.
     inv_freq = 1.0 / (theta ** exps)
     ang = torch.arange(max_len, dtype=torch.float32)[:, None] * inv_freq[None, :]
     return ang.cos().to(torch.bfloat16).contiguous(), ang.sin().to(torch.bfloat16).contiguous()
-
-
-def rope_tables(rotary_dim: int, max_len: int, theta: float, dtype: torch.dtype = torch.float32,
-                position_scale: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
-    """cos/sin tables [max_len, rotary_dim // 2] for PagedKVCache.append, the angles
-    in 64 bits: in fp32 the angle of position 100,000 is off by up to 0.004.
-    position_scale below 1 packs a longer context into the trained positions
-    (linear scaling).  half_split_tables holds the model's own bf16 tables."""
-    inv_freq = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
-    ang = torch.arange(max_len, dtype=torch.float64)[:, None] * position_scale * inv_freq[None, :]
-    return ang.cos().to(dtype).contiguous(), ang.sin().to(dtype).contiguous()
