@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) bitlinear_tc_kernel(const TcPar
     fence_mbar_init();
   }
   if (warp == 0) {
+    __syncwarp();  // lane 0 was apart: tensor memory is taken by a whole warp
     tmem_alloc(&ctrl->tmem_base, ncols);
     tmem_relinquish();
   }
@@ -323,6 +324,10 @@ __global__ void __launch_bounds__(TC_THREADS, 2) bitlinear_tc_kernel(const TcPar
       // after griddepcontrol.wait), so the first stages unpack while the
       // previous kernel still runs
       if (ok) ok = wait(&ctrl->w_full[slot], (s / nslot) & 1, 203);
+      // lanes leave their polls one by one: together again for the warp-wide stores, which come after the MMAs
+      // that read this buffer
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
       if (ok) {
         const uint8_t* wsm = ring + (size_t)slot * slot_bytes;
         const uint32_t tst = tbase + ((uint32_t)(quarter * 32) << 16) + b * acols;
@@ -387,6 +392,7 @@ __global__ void __launch_bounds__(TC_THREADS, 2) bitlinear_tc_kernel(const TcPar
       const bool fast = EPI == EPI_RELU2_MUL || seg_uniform;
       for (int c = third * 16; c < T; c += 48) {
         uint32_t sum[16];
+        __syncwarp();
         tmem_ld16(tmem_d + lanes + c, sum);
         tmem_wait_ld();
         for (int a = 1; a < used_acc; ++a) {

@@ -347,6 +347,7 @@ __device__ void mk_unpack(const MkParams& p, MkCtrl* c, const uint8_t* ring, uin
     if (g >= MK_NB) ok = mk_wait(p, &c->a_empty[b], ((g / MK_NB) + 1) & 1, 610);
     if (ok) ok = mk_wait(p, &c->w_full[slot], (g / MK_NSLOT) & 1, 611);
     ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();  // the stores come after the MMAs that read this buffer
     if (ok) {
       const uint8_t* wsm = ring + (size_t)slot * MK_SLOT;
       const uint32_t tst = tbase + ((uint32_t)(quarter * 32) << 16) + b * 64;
@@ -679,6 +680,7 @@ __global__ void __launch_bounds__(MK_THREADS) decode_layers_kernel(const MkParam
     fence_mbar_init();
   }
   if (warp == 0) {
+    __syncwarp();  // lane 0 was apart: tensor memory is taken by a whole warp
     tmem_alloc(&c->tmem_base, 512);
     tmem_relinquish();
   }

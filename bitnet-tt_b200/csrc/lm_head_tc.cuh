@@ -105,6 +105,7 @@ __global__ void __launch_bounds__(LMT_THREADS, 1) lm_head_tc_kernel(const LmTcPa
     fence_mbar_init();
   }
   if (warp == 0) {
+    __syncwarp();  // lane 0 was apart: tensor memory is taken by a whole warp
     tmem_alloc(&ctrl->tmem_base, ncols);
     tmem_relinquish();
   }
@@ -216,13 +217,15 @@ __global__ void __launch_bounds__(LMT_THREADS, 1) lm_head_tc_kernel(const LmTcPa
     asm volatile("bar.sync 1, 128;" ::: "memory");
     for (int i = 0; i < my_tiles; ++i) {
       const int db = i & 1;
-      if (!wait(&ctrl->d_full[db], (i >> 1) & 1, 403)) break;
+      // all lanes of a warp together, which its warp-wide loads need: lanes leave a poll one by one
+      if (!__all_sync(0xffffffffu, wait(&ctrl->d_full[db], (i >> 1) & 1, 403))) break;
       tc_fence_after();
       const int vt = blockIdx.x + i * gridDim.x;
       const int v = vt * 128 + tid;
       const uint32_t tl = tbase + ((uint32_t)(warp * 32) << 16) + db * T;
       for (int c = 0; c < T; c += 16) {
         uint32_t r[16];
+        __syncwarp();
         tmem_ld16(tl + c, r);
         tmem_wait_ld();
 #pragma unroll

@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       ctrl->block = found;
       if (p.nsplit > 1 && sp == 0 && g == 0) p.found[bx] = found;  // for the join
     }
+    __syncwarp();  // lane 0 was apart: tensor memory is taken, read and written by whole warps
     if (found.nrows > 0 && sp < paged_parts(p, found.kend)) {
       tmem_alloc(&ctrl->tmem, 512);
       tmem_relinquish();
@@ -741,6 +742,7 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
+        __syncwarp();
         if (nt > 0) {
           tmem_ld32(to + c, o);
           tmem_wait_ld();
