@@ -23,8 +23,9 @@ from test_paged_gpu import BF16, I8, _cache, _cu, _ok, _pages, _rows64, _scales
 pytestmark = pytest.mark.gpu
 
 
-def _check(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, sharp=0.1, scales=None, max_q=None, extra=0):
-    """scales(g, shape): value scales of an int8 cache."""
+def _check(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, sharp=0.1, scales=None, spread=0, lift=0, max_q=None, extra=0):
+    """scales(g, shape): value scales of an int8 cache.  spread: queries' elements span 2^spread.  lift: queries are
+    2^lift times what they are, and the scale 2^-lift."""
     g = torch.Generator().manual_seed(seed)
     table, n = _pages(kv, page, seed)
     c = _cache(cuda, n, page, hk, d, dtype, seed)
@@ -38,9 +39,12 @@ def _check(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, sharp=0.1, scales=None,
             c.value_scale.copy_(scales(g, tuple(c.value_scale.shape)))
     cu = _cu(qs)
     toks = int(cu[-1]) + extra
-    q = (torch.randn((toks, hq * d), generator=g) * sharp).to(BF16)
-    out = c.attend(q.to(cuda), cu.to(cuda), torch.tensor(kv, dtype=torch.int32).to(cuda), table.to(cuda),
-                   max_q or max(qs), max(kv))
+    q = torch.randn((toks, hq * d), generator=g) * sharp
+    if spread:
+        q = q * 2.0 ** (-spread * torch.rand(q.shape, generator=g))
+    q = q.to(BF16)
+    out = c.attend((q.float() * 2.0 ** lift).to(BF16).to(cuda), cu.to(cuda), torch.tensor(kv, dtype=torch.int32).to(cuda),
+                   table.to(cuda), max_q or max(qs), max(kv), d ** -0.5 * 2.0 ** -lift)
     torch.cuda.synchronize()
     _ok()
     got = out.double().cpu().view(toks, hq, d)
@@ -66,7 +70,8 @@ def _check(cuda, qs, kv, hq, hk, d, page, dtype, seed=0, sharp=0.1, scales=None,
             if dtype == I8:
                 vs = _scales(c, table, b, k)[:, h // grp, None]
                 if small:
-                    room = room + 2.0 ** -32 * (p * vs[:, 0]).amax(-1, keepdim=True) * (v.abs() / vs).sum(0)
+                    codes = torch.where(vs > 0, v.abs() / vs.clamp(min=1e-300), torch.zeros_like(v)).sum(0)
+                    room = room + 2.0 ** -32 * (p * vs[:, 0]).amax(-1, keepdim=True) * codes
                 else:
                     room = room + 2.0 ** -32 * (p.amax(-1, keepdim=True) * v.abs().sum(0) + 128 * float(vs.max()))
             worst = float(((got[int(cu[b]):int(cu[b + 1]), h] - want).abs() - room).max())
@@ -95,3 +100,41 @@ def test_precision_with_rows_behind_the_last_sequence(cuda, dtype):
 @pytest.mark.parametrize("qs,kv", [([3, 1], [900, 700]), ([60, 2, 1], [1000, 900, 5])])
 def test_precision_over_split_contexts(cuda, qs, kv, dtype):
     _check(cuda, qs, kv, 4, 1, 128, 32, dtype, seed=7)
+
+
+RANGES = [([1, 1], [90, 700]), ([6], [300]), ([60], [100]), ([100, 2], [600, 33])]
+
+
+@pytest.mark.parametrize("spread", [10, 30, 60])
+@pytest.mark.parametrize("qs,kv", RANGES)
+def test_value_scales_of_any_spread(cuda, qs, kv, spread):
+    """Scales from 1 down to 2^-spread, rows without any scale among them (a scale of 0)."""
+    def scales(g, shape):
+        s = 2.0 ** (-spread * torch.rand(shape, generator=g))
+        return s * (torch.rand(shape, generator=g) > 0.1)
+
+    _check(cuda, qs, kv, 4, 1, 128, 16, I8, seed=spread, scales=scales)
+
+
+@pytest.mark.parametrize("qs,kv", RANGES)
+def test_small_values_behind_a_large_one_that_is_not_seen(cuda, qs, kv):
+    """The last key's value scale is 2^18 times the others': the tokens before it keep their own precision."""
+    def scales(g, shape):
+        return torch.full(shape, 2.0 ** -20)
+
+    def with_last(g, shape):
+        s = scales(g, shape)
+        table, _ = _pages(kv, 16, 5)
+        for b, k in enumerate(kv):
+            s[int(table[b, (k - 1) // 16]), :, (k - 1) % 16] = 2.0 ** -2
+        return s
+
+    _check(cuda, qs, kv, 4, 1, 64, 16, I8, seed=5, scales=with_last)
+
+
+@pytest.mark.parametrize("dtype", [BF16, I8])
+@pytest.mark.parametrize("qs,kv", RANGES)
+def test_queries_of_any_spread_and_size(cuda, qs, kv, dtype):
+    _check(cuda, qs, kv, 4, 1, 128, 16, dtype, seed=8, sharp=0.5, spread=27)
+    for lift in (-60, 60):
+        _check(cuda, qs, kv, 4, 1, 64, 16, dtype, seed=9, lift=lift)
