@@ -10,8 +10,8 @@
 // the next step is there when the softmax of one is done, and neither waits for
 // the other: with one S of 128 keys a tile, the products that follow a softmax and
 // the signals between them (about 1300 cycles) stood in every step's chain, and
-// two 4096-token chunks over 16384 keys took 690 us (576 now, 1190 TFLOP/s; int8
-// 802).  What bounds a step now (1670 cycles, int8 2150) is a tile's softmax chain
+// two 4096-token chunks over 16384 keys took 690 us (589 now, 1167 TFLOP/s; int8
+// 824).  What bounds a step now (1670 cycles, int8 2150) is a tile's softmax chain
 // beside the MMAs: 190 until it sees the scores, 230 to load them, 330 for the
 // maximum, 790 for exponentials, sums and P; the MMAs alone take 1280 and the
 // softmax of both tiles alone 1000.  The price of short steps is that 64-key
@@ -34,10 +34,12 @@
 // A quarter of them is therefore computed on the multiply-add units (ex2_poly2).
 //
 // P of a sequence of more than 32 rows is one bf16 (half a step: 2^-8 of a weight), the
-// output's own precision, which doubles what rounding the output does to it: the two
-// 4096-token chunks come out within 2.2e-3 of the exact result (norms) in 570 us.  As a
-// pair hi + lo, 16 bits, they come within 1.65e-3, the output's rounding alone, in
-// 752 us, since the second product per step adds to the MMAs.  Sequences of up to 32 rows
+// output's own precision; the sums take the weights before they are rounded.  The two
+// 4096-token chunks come out within 2.2e-3 of the exact result (norms).  With a pair
+// hi + lo, 16 bits, for all they come within 1.65e-3, which is the output's rounding
+// alone, but took 752 us where one bf16 took 570: the second product per step adds to
+// the MMAs.  A third of the time for an error that stays below the output's own step
+// is not taken.  Sequences of up to 32 rows
 // (drafted tokens that stand beside chunks) get the pair and no polynomial: alone they
 // go to paged_rows_kernel, which works to the same precision.  2 chunks of 1024
 // beside 30 x 5 tokens over 4096 keys: 170 us with it, 159 without.

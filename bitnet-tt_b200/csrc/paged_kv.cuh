@@ -94,8 +94,11 @@ __device__ __forceinline__ uint32_t codes_of_f32(float a, float b, float c, floa
 // chunks that hold eight pairs (or two chunks of the dims that only move), so a
 // rotation needs no shuffle and reads each table entry once; the row's maximum
 // is a short shuffle tree.  In bf16 two heads a lane are loaded before the first is
-// worked on (one in int8, whose work needs the registers).  B200: 32 x 512 tokens,
-// 20 + 2 x 5 heads of 128, 47.3 us, 5.3 TB/s.
+// worked on (one in int8, whose work needs the registers); at 48 registers, for five
+// CTAs an SM, that costs 56 to 60 bytes of spills.  Rows are loaded behind the barrier
+// after the look-ups, and table entries again for each head.  B200: 32 x 512 tokens,
+// 20 + 2 x 5 heads of 128, 48.1 us, 5.2 TB/s; stepwise, whose roundings are four more
+// a value, 66.4 us.
 struct PagedAppendParams {
   PagedKV kv;
   const int32_t* cu;       // [B + 1] token offsets
