@@ -372,7 +372,7 @@ def bitlinear_fused(x: torch.Tensor, gamma: torch.Tensor | None, eps: float, buf
     M <= SIMT_FUSED_MAX_M one kernel; otherwise the act-quant and BitLinear
     launches (bufs holds the codes)."""
     m, k = x.shape
-    if x.dtype != torch.bfloat16 or x.stride(0) != k:
+    if x.dtype != torch.bfloat16 or not x.is_contiguous():  # of one row the stride may be anything
         raise ValueError("x must be contiguous bf16 [M, K]")
     seg = ctypes.byref(segments) if segments is not None else None
     check(load().bitnet_bitlinear(ptr(x), m, k, ptr(gamma), float(eps), ptr(w_packed), n, seg, epilogue,

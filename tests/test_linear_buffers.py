@@ -69,3 +69,20 @@ def test_many_token_counts_keep_no_memory(cuda):
         lin(x[:m])
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated(cuda) == before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stride", [1, 0, 2563, 2560])
+def test_one_row_of_any_stride(cuda, stride):
+    """A row that torch counts as contiguous whatever its stride: a slice of wider rows, a transposed column."""
+    lin = _linear(cuda, 2560, 640, 4)
+    x = torch.randn((1, 2560), generator=torch.Generator().manual_seed(2)).to(BF16).to(cuda)
+    assert torch.equal(lin(x.as_strided((1, 2560), (stride, 1))), lin(x.clone()))
+
+
+def test_rows_that_are_apart_are_refused_where_they_cannot_be():
+    from bitnet_tt import _lib
+
+    for x in (torch.zeros((3, 80), dtype=BF16)[:, :64], torch.zeros((64, 3), dtype=BF16).t(), torch.zeros((3, 64))):
+        with pytest.raises(ValueError, match="contiguous"):
+            _lib.bitlinear_fused(x, None, 1e-5, None, None, 64, None, 0, None, None)
