@@ -39,16 +39,17 @@
 // hi + lo, 16 bits, for all they come within 1.65e-3, which is the output's rounding
 // alone, but took 752 us where one bf16 took 570: the second product per step adds to
 // the MMAs.  A third of the time for an error that stays below the output's own step
-// is not taken.  Sequences of up to 32 rows
-// (drafted tokens that stand beside chunks) get the pair and no polynomial: alone they
-// go to paged_rows_kernel, which works to the same precision.  2 chunks of 1024
-// beside 30 x 5 tokens over 4096 keys: 170 us with it, 159 without.
+// is not taken.  Sequences of up to 32 rows (drafted tokens that stand beside chunks)
+// get the pair and no polynomial: alone they go to paged_rows_kernel, which works to
+// the same precision.  2 chunks of 1024 beside 30 x 5 tokens over 4096 keys: 170 us
+// with it, 159 without.
 //
 // int8: everything is f16.  The keys' codes are f16 values exactly, and their
 // scales multiply the scores in fp32, where an error would be raised to a power.
 // The values are code * scale, the scale and the product rounded to f16 (2^-11 each) at
 // a power of two taken from the largest scale of the part, which keeps rows down to
-// 2^-21 of it at that precision, and smaller ones to 2^-32 of 127 times it.  Q is scaled by a power of two per row (exact), P has f16's 11 bits.
+// 2^-21 of it at that precision, and smaller ones to 2^-32 of 127 times it.  Q is scaled
+// by a power of two per row (exact), P has f16's 11 bits.
 // Codes come out of their words as (0, 2) and (1, 3) pairs, so every four dims of
 // the slots stand in the order 0, 2, 1, 3: Q is laid out the same way, and the
 // output is put back when it is stored.
@@ -468,22 +469,22 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
       }
       __syncwarp();
       auto steps = [&](auto fine_tag) {
-      for (int i = 0; ok && i < nstep; ++i) {
-        const int j = i >> 1, h = i & 1;
-        const int vs = (2 * j + 1) % S::NSLOT, ks = (2 * j + 2) % S::NSLOT;  // slots of V, and of the next K
-        if (h == 0) {
-          ok = filled(2 * j + 1, 364);
-          if (ok && i + 2 < nstep) ok = filled(2 * j + 2, 366);
+        for (int i = 0; ok && i < nstep; ++i) {
+          const int j = i >> 1, h = i & 1;
+          const int vs = (2 * j + 1) % S::NSLOT, ks = (2 * j + 2) % S::NSLOT;  // slots of V, and of the next K
+          if (h == 0) {
+            ok = filled(2 * j + 1, 364);
+            if (ok && i + 2 < nstep) ok = filled(2 * j + 2, 366);
+          }
+          if (ok && i < nt) ok = arrived(&ctrl->p_ready[t][h], j & 1, 365);
+          if (ok && elect_one()) {
+            if (i < nt) pv(vs, h, i == 0, fine_tag);
+            if (i + 2 < nt) qk(ks, h);
+            if (h == 1 || i + 1 == nstep) tc_commit(&ctrl->empty[vs]);
+            if (i + 2 < nstep && (h == 1 || i + 3 == nstep)) tc_commit(&ctrl->empty[ks]);
+          }
+          __syncwarp();
         }
-        if (ok && i < nt) ok = arrived(&ctrl->p_ready[t][h], j & 1, 365);
-        if (ok && elect_one()) {
-          if (i < nt) pv(vs, h, i == 0, fine_tag);
-          if (i + 2 < nt) qk(ks, h);
-          if (h == 1 || i + 1 == nstep) tc_commit(&ctrl->empty[vs]);
-          if (i + 2 < nstep && (h == 1 || i + 3 == nstep)) tc_commit(&ctrl->empty[ks]);
-        }
-        __syncwarp();
-      }
       };
       // two copies of the loop, as of the softmax's: a choice inside it costs the common one 16%
       if (fine) steps(std::true_type{});
@@ -633,97 +634,97 @@ __global__ void __launch_bounds__(PchShape<D, I8>::THREADS, 1)
     uint64_t l2[2] = {0, 0};
     bool ok = true;
     auto steps = [&](auto fine_tag) {
-    constexpr bool FINE = decltype(fine_tag)::value;
-    for (int i = 0; i < nt; ++i) {
-      const int j = i >> 1, h = i & 1;
-      ok = wait(&ctrl->s_full[t][h], j & 1, 371);
-      if (!__all_sync(0xffffffffu, ok)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (warp_live) {
-        const uint32_t ts = tbase + lanes + t * 128 + h * 64;
-        uint32_t s[PCH_STEP];
-        tmem_ld32(ts, s);
-        tmem_ld32(ts + 32, s + 32);
-        tmem_wait_ld();
-        if (I8) {
-          const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(sm_scale + (j % S::RING) * 128 + h * 64);
-#pragma unroll
-          for (int c = 0; c < PCH_STEP / 4; ++c) {
-            const ulonglong2 k = sc[c];
-            f2_split(f2_mul(f2_make(s[4 * c], s[4 * c + 1]), k.x), s[4 * c], s[4 * c + 1]);
-            f2_split(f2_mul(f2_make(s[4 * c + 2], s[4 * c + 3]), k.y), s[4 * c + 2], s[4 * c + 3]);
-          }
+      constexpr bool FINE = decltype(fine_tag)::value;
+      for (int i = 0; i < nt; ++i) {
+        const int j = i >> 1, h = i & 1;
+        ok = wait(&ctrl->s_full[t][h], j & 1, 371);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
         }
-        const int base = k0 + i * PCH_STEP;
-        if (base + PCH_STEP > min(lim_min, k1)) {
-          const int see = min(lim, k1) - base;
+        tc_fence_after();
+        if (warp_live) {
+          const uint32_t ts = tbase + lanes + t * 128 + h * 64;
+          uint32_t s[PCH_STEP];
+          tmem_ld32(ts, s);
+          tmem_ld32(ts + 32, s + 32);
+          tmem_wait_ld();
+          if (I8) {
+            const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(sm_scale + (j % S::RING) * 128 + h * 64);
 #pragma unroll
-          for (int c = 0; c < PCH_STEP; ++c)
-            if (c >= see) s[c] = 0xff800000u;
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < PCH_STEP; c += 2)
-          mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-        const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
-        if (i == 0) {
-          m = top;
-        } else if (__any_sync(0xffffffffu, top > m + PCH_GROWTH)) {
-          const float mn = fmaxf(m, top);
-          const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
-          m = mn;
-          const uint64_t f2 = f2_splat(f);
-          l2[0] = f2_mul(l2[0], f2);
-          l2[1] = f2_mul(l2[1], f2);
-          // O holds all steps so far once the product of step i - 1 is in (that of step i - 3, one
-          // phase earlier on this barrier, is: S of step i - 1 came after it)
-          ok = wait(&ctrl->o_done[t][h ^ 1], ((i - 1) >> 1) & 1, 374);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(to + c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st32(to + c, o);
-          }
-        }
-        const uint64_t ref2 = f2_splat(m == -INFINITY ? 0.f : S::LIFT - m);
-#pragma unroll
-        for (int c = 0; c < PCH_STEP; c += 32) {
-          uint32_t pw[16], pl[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint64_t z = f2_fma(f2_make(s[c + 2 * e], s[c + 2 * e + 1]), scale2, ref2);
-            float x, y;
-            if (e % 4 == 3 && !FINE) {
-              ex2_poly2(z, x, y);
-            } else {
-              uint32_t a, b;
-              f2_split(z, a, b);
-              x = ex2(__uint_as_float(a)), y = ex2(__uint_as_float(b));
+            for (int c = 0; c < PCH_STEP / 4; ++c) {
+              const ulonglong2 k = sc[c];
+              f2_split(f2_mul(f2_make(s[4 * c], s[4 * c + 1]), k.x), s[4 * c], s[4 * c + 1]);
+              f2_split(f2_mul(f2_make(s[4 * c + 2], s[4 * c + 3]), k.y), s[4 * c + 2], s[4 * c + 3]);
             }
-            l2[e & 1] = f2_add(l2[e & 1], f2_make(__float_as_uint(x), __float_as_uint(y)));
-            if (FINE) split_bf2(x, y, pw[e], pl[e]);
-            else pw[e] = I8 ? f16x2_of(x, y) : bf2_of(x, y);
           }
-          tmem_st16(ts + c / 2, pw);
-          if (FINE) tmem_st16(ts + 32 + c / 2, pl);
+          const int base = k0 + i * PCH_STEP;
+          if (base + PCH_STEP > min(lim_min, k1)) {
+            const int see = min(lim, k1) - base;
+#pragma unroll
+            for (int c = 0; c < PCH_STEP; ++c)
+              if (c >= see) s[c] = 0xff800000u;
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < PCH_STEP; c += 2)
+            mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+          const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
+          if (i == 0) {
+            m = top;
+          } else if (__any_sync(0xffffffffu, top > m + PCH_GROWTH)) {
+            const float mn = fmaxf(m, top);
+            const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
+            m = mn;
+            const uint64_t f2 = f2_splat(f);
+            l2[0] = f2_mul(l2[0], f2);
+            l2[1] = f2_mul(l2[1], f2);
+            // O holds all steps so far once the product of step i - 1 is in (that of step i - 3, one
+            // phase earlier on this barrier, is: S of step i - 1 came after it)
+            ok = wait(&ctrl->o_done[t][h ^ 1], ((i - 1) >> 1) & 1, 374);
+            if (!__all_sync(0xffffffffu, ok)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(to + c, o);
+            }
+          }
+          const uint64_t ref2 = f2_splat(m == -INFINITY ? 0.f : S::LIFT - m);
+#pragma unroll
+          for (int c = 0; c < PCH_STEP; c += 32) {
+            uint32_t pw[16], pl[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const uint64_t z = f2_fma(f2_make(s[c + 2 * e], s[c + 2 * e + 1]), scale2, ref2);
+              float x, y;
+              if (e % 4 == 3 && !FINE) {
+                ex2_poly2(z, x, y);
+              } else {
+                uint32_t a, b;
+                f2_split(z, a, b);
+                x = ex2(__uint_as_float(a)), y = ex2(__uint_as_float(b));
+              }
+              l2[e & 1] = f2_add(l2[e & 1], f2_make(__float_as_uint(x), __float_as_uint(y)));
+              if (FINE) split_bf2(x, y, pw[e], pl[e]);
+              else pw[e] = I8 ? f16x2_of(x, y) : bf2_of(x, y);
+            }
+            tmem_st16(ts + c / 2, pw);
+            if (FINE) tmem_st16(ts + 32 + c / 2, pl);
+          }
+          tmem_wait_st();
         }
-        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctrl->p_ready[t][h]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctrl->p_ready[t][h]);
-    }
     };
     if (fine) steps(std::true_type{});
     else steps(std::false_type{});
